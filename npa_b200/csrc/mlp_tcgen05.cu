@@ -502,6 +502,11 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) linear_umma_kernel(const __gr
                 if (fuse && pass == 2 && !(ok = umma_wait(&sh->y_copied, (it & 1) ^ 1, &sh->abort))) break;
                 int last_block = first_block;
                 while (last_block + 2 < nblocks) last_block += 2;
+                if (pass == 1 && first_block >= nblocks) {  // up to 16 columns: the second half of the warps has none to read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->acc_empty[acc]);
+                }
 #pragma unroll 1
                 for (int b = first_block; b < nblocks; b += 2) {
                     const int c0 = b << 4;
