@@ -632,6 +632,60 @@ int npa_step_perceive_backward(const npa_grid *g, int32_t channels, const float 
                                float coef, int32_t log_norm_grad, const float *grad_s_add, float *grad_s, void *scratch,
                                int64_t scratch_bytes, const int32_t *bin_offsets, const int32_t *pair_cache, int32_t pair_stride,
                                void *stream);
+/* ---- 8-bit rows ------------------------------------------------------------------------------------
+ * Element types of the arrays that come in more than one. */
+enum { NPA_FLOAT32 = 0, NPA_FLOAT16 = 1, NPA_BFLOAT16 = 2, NPA_INT8 = 3, NPA_UINT8 = 4 };
+
+/* Rows into 8-bit codes with one scale each: scale = max(fl32(max |x| / most), 2^-126), code = x / scale rounded to
+ * nearest, ties to even; most = 127 (codes_type NPA_INT8), or 255 (NPA_UINT8: numbers below zero count as zero).  A row
+ * that holds an infinity or a NaN gets the scale NaN and codes of zero.  Pitches are in elements; x_pitch may be 0 (one
+ * row repeated).  npa_dequantize_rows writes code * scale, contiguous. */
+int npa_quantize_rows(const void *x, int32_t x_type, int64_t x_pitch, int64_t rows, int32_t cols, void *codes,
+                      int32_t codes_type, int64_t codes_pitch, float *scales, void *stream);
+int npa_dequantize_rows(const void *codes, int32_t codes_type, int64_t codes_pitch, const float *scales, int64_t rows,
+                        int32_t cols, void *out, int32_t out_type, void *stream);
+
+/* out[m, n] = act(float(sum_k x[m, k] w[n, k]) * (x_scales[m] * w_scales[n]) + bias[n]), each operation rounded to 32
+ * bits, the sum exact (in_dim <= 65536); w int8 codes, x codes with x_scales, or floating rows, which are quantised
+ * into scratch (npa_linear_int8_scratch_bytes() bytes, 16-byte aligned; 0 for codes).  bias may be NULL; out is
+ * contiguous. */
+int64_t npa_linear_int8_scratch_bytes(int32_t x_type, int64_t rows, int32_t in_dim);
+int npa_linear_int8(const void *x, int32_t x_type, int64_t x_pitch, const float *x_scales, const void *w, int64_t w_pitch,
+                    const float *w_scales, const void *bias, int32_t bias_type, int32_t relu, void *out, int32_t out_type,
+                    int64_t rows, int32_t in_dim, int32_t out_dim, void *scratch, int64_t scratch_bytes, void *stream);
+
+/* Both layers of the adaptation MLP in integers: z quantised to signed codes, the hidden layer (relu, 32 bits) to
+ * unsigned ones. */
+int64_t npa_mlp_int8_scratch_bytes(int64_t rows, int32_t in_dim, int32_t hidden, int32_t out_dim);
+int npa_mlp_int8(const float *z, int64_t z_pitch, const void *w1, int64_t w1_pitch, const float *w1_scales, const float *b1,
+                 const void *w2, int64_t w2_pitch, const float *w2_scales, float *y, int64_t rows, int32_t in_dim,
+                 int32_t hidden, int32_t out_dim, void *scratch, int64_t scratch_bytes, void *stream);
+
+/* Activations in 8 bits for a backward pass: groups of 32 columns share a power of two, value = code * 2^(E - 133),
+ * |code| <= 127, E = clamp((bits(max |x|) + 0x10000) >> 23, 7, 254), one byte per group, exponents [rows, ceil(cols / 32)];
+ * a group that holds an infinity or a NaN has E = 255 and is restored as NaN.  Restored values beyond the largest
+ * number of float16 become it. */
+int npa_rows8_compress(const void *x, int32_t type, int64_t x_pitch, int64_t rows, int32_t cols, void *codes,
+                       int64_t codes_pitch, uint8_t *exponents, void *stream);
+int npa_rows8_restore(const void *codes, int64_t codes_pitch, const uint8_t *exponents, int64_t rows, int32_t cols,
+                      void *out, int32_t type, void *stream);
+
+/* The adaptation MLP (hidden width 128, in <= 175, out <= 48) whose backward reads z in 8 bits.  The forward leaves
+ * codes [rows, in rounded up to 16], exponents, and mask [rows, 4] with the bits of h > 0 (unit 32 w + i is bit i of word
+ * w); the backward makes the hidden layer again from them.  dz may be NULL, and dW1, db1 and dW2 together.  codes, mask,
+ * dy and scratch 16-byte aligned; waits are bounded as in npa_linear_tcgen05. */
+int64_t npa_mlp_checkpoint_forward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim);
+int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1, const float *W2, float *y, int64_t rows,
+                               int32_t in_dim, int32_t out_dim, int64_t w1_stride_out, int64_t w1_stride_in,
+                               int64_t w2_stride_out, int64_t w2_stride_in, void *codes, uint8_t *exponents, uint32_t *mask,
+                               void *scratch, int64_t scratch_bytes, void *stream);
+int64_t npa_mlp_checkpoint_backward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim);
+int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, const uint32_t *mask, const float *W1,
+                                const float *b1, const float *W2, const float *dy, float *dz, float *dW1, float *db1,
+                                float *dW2, int64_t rows, int32_t in_dim, int32_t out_dim, int64_t w1_stride_out,
+                                int64_t w1_stride_in, int64_t w2_stride_out, int64_t w2_stride_in, void *scratch,
+                                int64_t scratch_bytes, void *stream);
+
 /* Self-test of those bounded waits: a two-warp kernel in which warp 0 waits `limit_us` (1..1,000,000)
  * on an mbarrier that nothing completes, gives up and raises the kernel's leave flag, and warp 1,
  * waiting on a second such mbarrier with the full limit, leaves through the flag.  device_result[0]

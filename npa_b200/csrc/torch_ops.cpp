@@ -727,6 +727,276 @@ Tensor mlp(const Tensor &z, const Tensor &w1, const Tensor &b1, const Tensor &w2
     return y;
 }
 
+// ---- 8-bit rows: products in integers, checkpoints (int8.cu, rows8.cu) ------------------------------------------------
+int value_type(const Tensor &t, const char *name) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return NPA_FLOAT32;
+        case at::kHalf: return NPA_FLOAT16;
+        case at::kBFloat16: return NPA_BFLOAT16;
+        case at::kChar: return NPA_INT8;
+        case at::kByte: return NPA_UINT8;
+        default: throw py::type_error(std::string(name) + ": expected float32, float16, bfloat16, int8 or uint8, got " + toString(t.scalar_type()));
+    }
+}
+bool is_codes(int type) { return type == NPA_INT8 || type == NPA_UINT8; }
+int float_type(const Tensor &t, const char *name) {
+    const int type = value_type(t, name);
+    if (is_codes(type)) throw py::type_error(std::string(name) + ": expected float32, float16 or bfloat16, got " + toString(t.scalar_type()));
+    return type;
+}
+at::ScalarType float_type(at::ScalarType t, const char *name) {
+    if (t != at::kFloat && t != at::kHalf && t != at::kBFloat16)
+        throw py::type_error(std::string(name) + ": expected float32, float16 or bfloat16, got " + toString(t));
+    return t;
+}
+int type_code(at::ScalarType t) { return t == at::kFloat ? NPA_FLOAT32 : t == at::kHalf ? NPA_FLOAT16 : NPA_BFLOAT16; }
+void on_device(const Tensor &t, const char *name, const Tensor &like) {
+    if (!t.is_cuda() || t.device() != like.device())
+        throw py::type_error(std::string(name) + ": expected a tensor on " + like.device().str() + ", got one on " + t.device().str());
+}
+void on_cuda(const Tensor &t, const char *name) {
+    if (!t.is_cuda()) throw py::type_error(std::string(name) + ": expected a CUDA tensor, got one on " + t.device().str());
+}
+void of_shape(const Tensor &t, at::IntArrayRef shape, const char *name) {
+    if (t.sizes() != shape) throw std::runtime_error(std::string(name) + " must have shape " + shape_text(shape) + ", got " + shape_text(t.sizes()));
+}
+template <typename... In>
+void refuse_gradients(const char *name, const In &...inputs) {
+    refuse_tangents(name, inputs...);
+    if (recording(inputs...)) throw std::runtime_error(std::string(name) + " has no backward: call it under torch.no_grad(), or detach its inputs");
+}
+// The rows of a tensor [..., k] as the kernels read them: elements next to each other, one distance between rows.
+struct Rows {
+    Tensor t;  // keeps the memory
+    int64_t rows, cols, pitch;
+    Rows(const Tensor &x, const char *name) {
+        if (x.dim() < 1) throw std::runtime_error(std::string(name) + " must have at least 1 dimension");
+        cols = x.size(-1);
+        if (cols < 1) throw std::runtime_error(std::string(name) + " must have at least one column, got " + shape_text(x.sizes()));
+        rows = x.numel() / cols;
+        t = x.is_contiguous() ? x : x.dim() == 2 ? x : x.reshape({rows, cols});
+        if (t.dim() == 2 && !t.is_contiguous() && ((t.stride(1) != 1 && cols > 1) || t.stride(0) < 0)) t = t.contiguous();
+        pitch = t.dim() == 2 && rows > 1 ? t.stride(0) : cols;
+    }
+    const void *data() const { return t.const_data_ptr(); }
+};
+// Memory for the codes of rows: a multiple of 16 bytes from row to row.
+int64_t code_pitch(int64_t cols) { return (cols + 15) / 16 * 16; }
+Tensor code_rows(const Tensor &like, int64_t rows, int64_t cols, at::ScalarType type) { return fresh(like, {rows, code_pitch(cols)}, type); }
+Tensor as_codes(const Tensor &padded, at::IntArrayRef shape) {
+    const int64_t cols = shape.back(), pitch = padded.size(1);
+    if (cols == pitch && shape.size() == 2) return padded;
+    std::vector<int64_t> strides(shape.size());
+    strides.back() = 1;
+    int64_t step = pitch;
+    for (int d = (int)shape.size() - 2; d >= 0; --d) {
+        strides[d] = step;
+        step *= shape[d];
+    }
+    return padded.as_strided(shape, strides);
+}
+
+py::tuple quantize_rows(const Tensor &x, bool is_unsigned) {
+    refuse_gradients("quantize_rows", x);
+    on_cuda(x, "x");
+    const int type = float_type(x, "x");
+    c10::cuda::CUDAGuard guard(x.device());
+    const Rows r(x, "x");
+    Tensor codes = code_rows(x, r.rows, r.cols, is_unsigned ? at::kByte : at::kChar), scales = floats(x, x.sizes().slice(0, x.dim() - 1));
+    if (r.rows)
+        check_status(npa_quantize_rows(r.data(), type, r.pitch, r.rows, (int)r.cols, codes.mutable_data_ptr(), is_unsigned ? NPA_UINT8 : NPA_INT8, codes.size(1),
+                                       fmut(scales), stream_of(x)));
+    return py::make_tuple(as_codes(codes, x.sizes()), scales);
+}
+
+void need_scales(const Tensor &scales, const Tensor &codes, const char *name) {
+    on_device(scales, name, codes);
+    if (scales.scalar_type() != at::kFloat) throw py::type_error(std::string(name) + ": expected float32, got " + toString(scales.scalar_type()));
+    of_shape(scales, codes.sizes().slice(0, codes.dim() - 1), name);
+}
+
+Tensor dequantize_rows(const Tensor &codes, const Tensor &scales, at::ScalarType dtype) {
+    refuse_gradients("dequantize_rows", scales);
+    on_cuda(codes, "codes");
+    const int type = value_type(codes, "codes");
+    if (!is_codes(type)) throw py::type_error("codes: expected int8 or uint8, got " + std::string(toString(codes.scalar_type())));
+    float_type(dtype, "dtype");
+    const Rows r(codes, "codes");
+    need_scales(scales, codes, "scales");
+    c10::cuda::CUDAGuard guard(codes.device());
+    const Tensor s = scales.contiguous();
+    Tensor out = fresh(codes, codes.sizes(), dtype);
+    if (r.rows)
+        check_status(npa_dequantize_rows(r.data(), type, r.pitch, fptr(s), r.rows, (int)r.cols, out.mutable_data_ptr(), type_code(dtype), stream_of(codes)));
+    return out;
+}
+
+// Weight codes [out, in] as the kernels read them.
+Rows weight_rows(const Tensor &w, const Tensor &scales, const Tensor &like, int64_t in, const char *name, const char *scales_name) {
+    on_device(w, name, like);
+    if (w.scalar_type() != at::kChar) throw py::type_error(std::string(name) + ": expected int8, got " + toString(w.scalar_type()));
+    if (w.dim() != 2) throw std::runtime_error(std::string(name) + " must have 2 dimensions, got " + std::to_string(w.dim()));
+    if (in >= 0 && w.size(1) != in) throw std::runtime_error(std::string(name) + " must have " + std::to_string(in) + " columns, got " + shape_text(w.sizes()));
+    need_scales(scales, w, scales_name);
+    return Rows(w, name);
+}
+
+Tensor linear_int8(const Tensor &x, const Tensor &w, const Tensor &w_scales, const OptTensor &bias_, bool relu, const OptTensor &x_scales_,
+                   std::optional<at::ScalarType> out_dtype) {
+    const Tensor bias = or_none(bias_), given = or_none(x_scales_);
+    refuse_gradients("linear_int8", x, w_scales, bias, given);
+    on_cuda(x, "x");
+    const int type = value_type(x, "x");
+    const Rows r(x, "x");
+    c10::cuda::CUDAGuard guard(x.device());
+    const Rows wr = weight_rows(w, w_scales, x, r.cols, "w", "w_scales");
+    const int64_t n = w.size(0);
+    if (is_codes(type) != given.defined())
+        throw std::runtime_error(given.defined() ? "x_scales belong to rows of codes; rows of numbers are given their own" : "rows of codes need x_scales");
+    if (given.defined()) need_scales(given, x, "x_scales");
+    int bias_type = 0;
+    Tensor b;
+    if (bias.defined()) {
+        on_device(bias, "bias", x);
+        bias_type = float_type(bias, "bias");
+        of_shape(bias, {n}, "bias");
+        b = bias.contiguous();
+    }
+    const at::ScalarType to = float_type(out_dtype.has_value() ? *out_dtype : is_codes(type) ? at::kFloat : x.scalar_type(), "out_dtype");
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = n;
+    const Tensor ws = w_scales.contiguous(), xs = given.defined() ? given.contiguous() : Tensor();
+    Tensor out = fresh(x, shape, to);
+    if (!r.rows || !n) return out;
+    const int64_t bytes = npa_linear_int8_scratch_bytes(type, r.rows, (int)r.cols);
+    Tensor scratch = bytes ? fresh(x, {bytes}, at::kByte) : Tensor();
+    check_status(npa_linear_int8(r.data(), type, r.pitch, fptr(xs), wr.data(), wr.pitch, fptr(ws), b.defined() ? b.const_data_ptr() : nullptr, bias_type, relu,
+                                 out.mutable_data_ptr(), type_code(to), r.rows, (int)r.cols, (int)n, bytes ? scratch.mutable_data_ptr() : nullptr, bytes,
+                                 stream_of(x)));
+    return out;
+}
+
+Tensor mlp_int8(const Tensor &z, const Tensor &w1, const Tensor &w1_scales, const Tensor &b1, const Tensor &w2, const Tensor &w2_scales) {
+    refuse_gradients("mlp_int8", z, w1_scales, b1, w2_scales);
+    on_cuda(z, "z");
+    if (z.scalar_type() != at::kFloat) throw py::type_error(std::string("z: expected float32, got ") + toString(z.scalar_type()));
+    const Rows r(z, "z");
+    c10::cuda::CUDAGuard guard(z.device());
+    const Rows r1 = weight_rows(w1, w1_scales, z, r.cols, "w1", "w1_scales");
+    const int64_t hidden = w1.size(0), n = w2.dim() == 2 ? w2.size(0) : 0;
+    on_device(b1, "b1", z);
+    if (b1.scalar_type() != at::kFloat) throw py::type_error(std::string("b1: expected float32, got ") + toString(b1.scalar_type()));
+    of_shape(b1, {hidden}, "b1");
+    const Rows r2 = weight_rows(w2, w2_scales, z, hidden, "w2", "w2_scales");
+    const Tensor b = b1.contiguous(), s1 = w1_scales.contiguous(), s2 = w2_scales.contiguous();
+    std::vector<int64_t> shape = z.sizes().vec();
+    shape.back() = n;
+    Tensor y = floats(z, shape);
+    if (!r.rows || !n) return y;
+    const int64_t bytes = npa_mlp_int8_scratch_bytes(r.rows, (int)r.cols, (int)hidden, (int)n);
+    Tensor scratch = bytes ? fresh(z, {bytes}, at::kByte) : Tensor();
+    check_status(npa_mlp_int8(fptr(r.t), r.pitch, r1.data(), r1.pitch, fptr(s1), fptr(b), r2.data(), r2.pitch, fptr(s2), fmut(y), r.rows, (int)r.cols, (int)hidden,
+                              (int)n, bytes ? scratch.mutable_data_ptr() : nullptr, bytes, stream_of(z)));
+    return y;
+}
+
+int64_t row_groups(int64_t cols) { return (cols + 31) / 32; }
+
+py::tuple compress_rows(const Tensor &x) {
+    refuse_gradients("compress_rows", x);
+    on_cuda(x, "x");
+    const int type = float_type(x, "x");
+    c10::cuda::CUDAGuard guard(x.device());
+    const Rows r(x, "x");
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = row_groups(r.cols);
+    Tensor codes = code_rows(x, r.rows, r.cols, at::kChar), exps = fresh(x, shape, at::kByte);
+    if (r.rows)
+        check_status(npa_rows8_compress(r.data(), type, r.pitch, r.rows, (int)r.cols, codes.mutable_data_ptr(), codes.size(1), exps.mutable_data_ptr<uint8_t>(),
+                                        stream_of(x)));
+    return py::make_tuple(as_codes(codes, x.sizes()), exps);
+}
+
+Tensor restore_rows(const Tensor &codes, const Tensor &exponents, at::ScalarType dtype) {
+    on_cuda(codes, "codes");
+    if (codes.scalar_type() != at::kChar) throw py::type_error(std::string("codes: expected int8, got ") + toString(codes.scalar_type()));
+    float_type(dtype, "dtype");
+    const Rows r(codes, "codes");
+    on_device(exponents, "exponents", codes);
+    if (exponents.scalar_type() != at::kByte) throw py::type_error(std::string("exponents: expected uint8, got ") + toString(exponents.scalar_type()));
+    std::vector<int64_t> shape = codes.sizes().vec();
+    shape.back() = row_groups(r.cols);
+    of_shape(exponents, shape, "exponents");
+    c10::cuda::CUDAGuard guard(codes.device());
+    const Tensor e = exponents.contiguous();
+    Tensor out = fresh(codes, codes.sizes(), dtype);
+    if (r.rows)
+        check_status(npa_rows8_restore(r.data(), r.pitch, e.const_data_ptr<uint8_t>(), r.rows, (int)r.cols, out.mutable_data_ptr(), type_code(dtype),
+                                       stream_of(codes)));
+    return out;
+}
+
+// The adaptation MLP with its input kept in 8 bits and its hidden layer as the bits of the ReLU.
+struct MlpCheckpointNode : Node {
+    SavedVariable w1_, b1_, w2_, codes_, exps_, mask_;
+    std::vector<int64_t> z_shape;
+    variable_list apply(variable_list &&g) override {
+        const Tensor w1 = w1_.unpack(), b1 = b1_.unpack(), w2 = w2_.unpack(), codes = codes_.unpack(), exps = exps_.unpack(), mask = mask_.unpack();
+        const bool nz = should_compute_output(0), n1 = should_compute_output(1), nb = should_compute_output(2), n2 = should_compute_output(3);
+        const bool weights = n1 || nb || n2;
+        if (!g[0].defined() || !(nz || weights)) return variable_list(4);
+        c10::cuda::CUDAGuard guard(w1.device());
+        const Tensor dy = solid(g[0]);
+        const int64_t k = w1.size(1), o = w2.size(0), m = codes.size(0);
+        Tensor gz = nz ? floats(w1, z_shape) : Tensor(), gw1, gb1, gw2;
+        if (weights) {
+            gw1 = blank(w1);
+            gb1 = blank(b1);
+            gw2 = blank(w2);
+        }
+        if (m == 0) {
+            if (weights) gw1.zero_(), gb1.zero_(), gw2.zero_();
+        } else {
+            const int64_t bytes = npa_mlp_checkpoint_backward_scratch_bytes(m, (int)k, (int)o);
+            Tensor scratch = fresh(w1, {bytes}, at::kByte);
+            check_status(npa_mlp_checkpoint_backward(codes.const_data_ptr(), exps.const_data_ptr<uint8_t>(), reinterpret_cast<const uint32_t *>(iptr(mask)), fptr(w1),
+                                                     fptr(b1), fptr(w2), fptr(dy), fmut(gz), fmut(gw1), fmut(gb1), fmut(gw2), m, (int)k, (int)o, w1.stride(0),
+                                                     w1.stride(1), w2.stride(0), w2.stride(1), scratch.mutable_data_ptr(), bytes, stream_of(w1)));
+        }
+        return {gz, n1 ? gw1 : Tensor(), nb ? gb1 : Tensor(), n2 ? gw2 : Tensor()};
+    }
+    void release_variables() override {
+        w1_.reset_data(); b1_.reset_data(); w2_.reset_data(); codes_.reset_data(); exps_.reset_data(); mask_.reset_data();
+    }
+};
+
+// The caller has checked types, devices and widths (mlp.supported); z is contiguous.
+Tensor mlp_checkpoint(const Tensor &z, const Tensor &w1, const Tensor &b1, const Tensor &w2) {
+    if (!recording(z, w1, b1, w2) && z.numel()) return mlp(z, w1, b1, w2);
+    refuse_tangents("the adaptation MLP", z, w1, b1, w2);
+    c10::cuda::CUDAGuard guard(z.device());
+    const int64_t k = w1.size(1), o = w2.size(0);
+    if (z.dim() < 1 || z.size(-1) != k) throw std::runtime_error("z must have " + std::to_string(k) + " columns, got " + shape_text(z.sizes()));
+    const int64_t m = z.numel() / k;
+    std::vector<int64_t> shape = z.sizes().vec();
+    shape.back() = o;
+    Tensor y = floats(z, shape), codes = code_rows(z, m, k, at::kChar), exps = fresh(z, {m, row_groups(k)}, at::kByte), mask = ints(z, {m, kHidden / 32});
+    if (m) {
+        const int64_t bytes = npa_mlp_checkpoint_forward_scratch_bytes(m, (int)k, (int)o);
+        Tensor scratch = fresh(z, {bytes}, at::kByte);
+        check_status(npa_mlp_checkpoint_forward(fptr(z), fptr(w1), fptr(b1), fptr(w2), fmut(y), m, (int)k, (int)o, w1.stride(0), w1.stride(1), w2.stride(0),
+                                                w2.stride(1), codes.mutable_data_ptr(), exps.mutable_data_ptr<uint8_t>(), reinterpret_cast<uint32_t *>(imut(mask)),
+                                                scratch.mutable_data_ptr(), bytes, stream_of(z)));
+    }
+    if (recording(z, w1, b1, w2)) {
+        auto n = node_for<MlpCheckpointNode>(z, w1, b1, w2);
+        n->w1_ = saved(w1); n->b1_ = saved(b1); n->w2_ = saved(w2);
+        n->codes_ = saved(codes); n->exps_ = saved(exps); n->mask_ = saved(mask); n->z_shape = z.sizes().vec();
+        torch::autograd::set_history(y, n);
+    }
+    return y;
+}
+
 // ---- a whole Euler step as one node ------------------------------------------------------------------------------
 // Binning, reorder, packed perception, MLP and update of stepping.step_euler: the same kernels as the operators above, but
 // one crossing from Python and one node.  Four nodes cost ~60 us of host time more per training step (graph bookkeeping,
@@ -947,6 +1217,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("packed_perception", op("packed_perception", &packed_perception));
     m.def("step_update", op("step_update", &step_update));
     m.def("mlp", op("mlp", &mlp));
+    m.def("quantize_rows", op("quantize_rows", &quantize_rows));
+    m.def("dequantize_rows", op("dequantize_rows", &dequantize_rows));
+    m.def("linear_int8", op("linear_int8", &linear_int8));
+    m.def("mlp_int8", op("mlp_int8", &mlp_int8));
+    m.def("compress_rows", op("compress_rows", &compress_rows));
+    m.def("restore_rows", op("restore_rows", &restore_rows));
+    m.def("mlp_checkpoint", op("mlp_checkpoint", &mlp_checkpoint));
     m.def("euler_step", op("euler_step", &euler_step));
     m.def("splat", op("splat", &splat));
 }

@@ -92,8 +92,13 @@ def _one_node(model, x, s, grid) -> bool:
             and last.out_features == grid.dim + C)
 
 
-def step_euler(model, x, s, grid, dt=1.0, update_prob=0.5, intermediate=False, noise_std=0.0, wrap=False):
+def step_euler(model, x, s, grid, dt=1.0, update_prob=0.5, intermediate=False, noise_std=0.0, wrap=False,
+               checkpoint=False):
     """``x, s, stats`` after one step; the particles come back in cell order, as in the reference.
+
+    ``checkpoint=True`` keeps the perception rows in 8 bits for the backward, and of the hidden layer the bits of its ReLU
+    (``mlp.apply_mlp``): a long training rollout holds a fraction of the memory, and the gradients of the MLP's two weight
+    matrices see rounded rows.
 
     ``wrap=True`` additionally applies ``grid.wrap_positions`` (the reference's trainers call it
     after the rollout, train.py:238); the 3D padding column is kept either way.
@@ -101,7 +106,7 @@ def step_euler(model, x, s, grid, dt=1.0, update_prob=0.5, intermediate=False, n
     B, N, C = s.shape
     alpha = _buffer_scalar(model, "alpha")
     stats = None
-    if not intermediate and _one_node(model, x, s, grid):
+    if not intermediate and not (checkpoint and torch.is_grad_enabled()) and _one_node(model, x, s, grid):
         first, _, last = model.model
         x_new, s_new, model.last_snapshot, uniforms = sph_ops.euler_step(
             grid, x, s, (first.weight, first.bias, last.weight), _buffer_scalar(model, "eps0"), alpha, dt, update_prob, wrap,
@@ -110,7 +115,7 @@ def step_euler(model, x, s, grid, dt=1.0, update_prob=0.5, intermediate=False, n
     else:
         z, x_bin, s_bin, snapshot = perceive(model, x, s, grid)
         model.last_snapshot = snapshot
-        y = apply_mlp(model.model, z)  # (B, N, dim + C)
+        y = apply_mlp(model.model, z, checkpoint)  # (B, N, dim + C)
         if intermediate:
             d = y[..., : model.spatial_dims]
             dx = alpha * d * grid.eps / (1.0 + d.norm(dim=-1, keepdim=True))
