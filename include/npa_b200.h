@@ -647,16 +647,20 @@ int npa_dequantize_rows(const void *codes, int32_t codes_type, int64_t codes_pit
 
 /* out[m, n] = act(float(sum_k x[m, k] w[n, k]) * (x_scales[m] * w_scales[n]) + bias[n]), each operation rounded to 32
  * bits, the sum exact (in_dim <= 65536); w int8 codes, x codes with x_scales, or floating rows, which are quantised
- * into scratch (npa_linear_int8_scratch_bytes() bytes, 16-byte aligned; 0 for codes).  bias may be NULL; out is
- * contiguous. */
-int64_t npa_linear_int8_scratch_bytes(int32_t x_type, int64_t rows, int32_t in_dim);
+ * on the way.  scratch holds npa_linear_int8_scratch_bytes() bytes, 16-byte aligned: codes of the rows, and copies of
+ * codes that do not start on 16 bytes in every row, or are unsigned (addresses are only looked at, none is read).
+ * bias may be NULL; out is contiguous.  Bounded waits report through npa_linear_tcgen05_status (bits 128, 256, 512:
+ * loads, MMA lane, epilogue of this kernel). */
+int64_t npa_linear_int8_scratch_bytes(const void *x, int32_t x_type, int64_t x_pitch, const void *w, int64_t w_pitch,
+                                      int64_t rows, int32_t in_dim, int32_t out_dim);
 int npa_linear_int8(const void *x, int32_t x_type, int64_t x_pitch, const float *x_scales, const void *w, int64_t w_pitch,
                     const float *w_scales, const void *bias, int32_t bias_type, int32_t relu, void *out, int32_t out_type,
                     int64_t rows, int32_t in_dim, int32_t out_dim, void *scratch, int64_t scratch_bytes, void *stream);
 
 /* Both layers of the adaptation MLP in integers: z quantised to signed codes, the hidden layer (relu, 32 bits) to
  * unsigned ones. */
-int64_t npa_mlp_int8_scratch_bytes(int64_t rows, int32_t in_dim, int32_t hidden, int32_t out_dim);
+int64_t npa_mlp_int8_scratch_bytes(const void *z, int64_t z_pitch, const void *w1, int64_t w1_pitch, const void *w2,
+                                   int64_t w2_pitch, int64_t rows, int32_t in_dim, int32_t hidden, int32_t out_dim);
 int npa_mlp_int8(const float *z, int64_t z_pitch, const void *w1, int64_t w1_pitch, const float *w1_scales, const float *b1,
                  const void *w2, int64_t w2_pitch, const float *w2_scales, float *y, int64_t rows, int32_t in_dim,
                  int32_t hidden, int32_t out_dim, void *scratch, int64_t scratch_bytes, void *stream);

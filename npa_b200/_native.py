@@ -130,9 +130,9 @@ SIGNATURES = {
     "npa_linear_tcgen05_scratch_bytes": (ctypes.c_int64, [_I32, _I32]),
     "npa_quantize_rows": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _P, _I32, _I64, _P, _P]),
     "npa_dequantize_rows": (ctypes.c_int, [_P, _I32, _I64, _P, _I64, _I32, _P, _I32, _P]),
-    "npa_linear_int8_scratch_bytes": (_I64, [_I32, _I64, _I32]),
+    "npa_linear_int8_scratch_bytes": (_I64, [_P, _I32, _I64, _P, _I64, _I64, _I32, _I32]),
     "npa_linear_int8": (ctypes.c_int, [_P, _I32, _I64, _P, _P, _I64, _P, _P, _I32, _I32, _P, _I32, _I64, _I32, _I32, _P, _I64, _P]),
-    "npa_mlp_int8_scratch_bytes": (_I64, [_I64, _I32, _I32, _I32]),
+    "npa_mlp_int8_scratch_bytes": (_I64, [_P, _I64, _P, _I64, _P, _I64, _I64, _I32, _I32, _I32]),
     "npa_mlp_int8": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _P, _I64, _I32, _I32, _I32, _P, _I64, _P]),
     "npa_rows8_compress": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _P, _I64, _P, _P]),
     "npa_rows8_restore": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _P, _I32, _P]),

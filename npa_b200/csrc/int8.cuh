@@ -58,4 +58,71 @@ __device__ __forceinline__ int row_code(float x, float scale, float inverse) {
 
 __device__ __forceinline__ unsigned warp_max(unsigned v) { return __reduce_max_sync(kFull, v); }
 
+// V values at p, of which `left` exist.
+template <typename T, int V>
+__device__ __forceinline__ void load_values(const T *__restrict__ p, int left, float (&v)[V]) {
+    if constexpr (V == 1) {
+        v[0] = left > 0 ? as_float(p[0]) : 0.f;
+    } else {
+        if (left >= V) {
+            constexpr int kQuads = V * (int)sizeof(T) / 16;
+            union {
+                uint4 quad[kQuads];
+                T value[V];
+            } u;
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) u.quad[q] = __ldg(reinterpret_cast<const uint4 *>(p) + q);
+#pragma unroll
+            for (int q = 0; q < V; ++q) v[q] = as_float(u.value[q]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < V; ++q) v[q] = q < left ? as_float(p[q]) : 0.f;
+        }
+    }
+}
+// V codes to p, of which `left` exist; `aligned`: p is a multiple of V.
+template <int V>
+__device__ __forceinline__ void store_codes(uint8_t *p, int left, bool aligned, const int (&code)[V]) {
+    if (V == 8 && left >= V && aligned) {
+        unsigned w[2] = {};
+#pragma unroll
+        for (int q = 0; q < V; ++q) w[q / 4] |= ((unsigned)code[q] & 0xffu) << (8 * (q % 4));
+        *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < V; ++q)
+            if (q < left) p[q] = (uint8_t)code[q];
+    }
+}
+
+// ---- the product -----------------------------------------------------------------------------------------------------
+struct Int8Args {
+    const void *x;       // [rows, in] codes, or values that the kernel for few rows quantises
+    const int8_t *w;     // [out, in], rows 16-byte aligned
+    long long x_pitch, w_pitch;  // in elements
+    int x_type;
+    const float *x_scales, *w_scales;
+    const int *w_sums;   // rows of codes that were shifted from unsigned to signed by 128: sums of the channels' weights, else NULL
+    const void *bias;    // [out] or NULL
+    int bias_type, relu, out_type;
+    void *out;           // [rows, out]
+    long long rows;
+    int in, out_dim;
+};
+
+__device__ __forceinline__ float load_value(const void *p, int type, long long at) {
+    if (type == NPA_FLOAT32) return static_cast<const float *>(p)[at];
+    if (type == NPA_FLOAT16) return __half2float(static_cast<const __half *>(p)[at]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[at]);
+}
+// No product is contracted with the sum behind it: the roundings are those of the definition.
+__device__ __forceinline__ float int8_value(int sum, float s, float t, bool has_bias, float bias, bool relu) {
+    float v = __fmul_rn(__int2float_rn(sum), __fmul_rn(s, t));
+    if (has_bias) v = __fadd_rn(v, bias);
+    return relu && v < 0.f ? 0.f : v;  // (a NaN stays one)
+}
+
+// int8_tcgen05.cu: the product of codes on the tensor cores; x and w 16-byte aligned with pitches of multiples of 16, x signed.
+int launch_int8_tcgen05(const char *me, const Int8Args &a, cudaStream_t st);
+
 }  // namespace npa

@@ -12,19 +12,68 @@ namespace npa {
 
 constexpr int kMaskHidden = 128;
 
+// Rows whose addresses are multiples of 16 bytes: a thread takes eight values, four neighbours a group.
 template <typename T>
 __global__ void __launch_bounds__(256) rows8_compress_kernel(const T *__restrict__ x, long long pitch, long long rows, int cols, int8_t *__restrict__ codes,
                                                              long long codes_pitch, uint8_t *__restrict__ exps) {
     after_previous_kernel();
+    const int groups = rows8_groups(cols), each = 4 * groups;
+    const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x, row = at / each;
+    const int part = (int)(at - row * each), k = 8 * part;
+    const int left = row < rows ? cols - k : 0;
+    float v[8];
+    load_values<T, 8>(x + (left > 0 ? row * pitch + k : 0), left, v);
+    unsigned largest = 0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) largest = max(largest, magnitude(v[q]));
+    largest = max(largest, __shfl_xor_sync(kFull, largest, 1));
+    largest = max(largest, __shfl_xor_sync(kFull, largest, 2));
+    if (row >= rows) return;
+    const unsigned e = rows8_exponent(largest);
+    const float to_units = rows8_to_units(e);
+    int code[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) code[q] = rows8_code(v[q], to_units);
+    if (left > 0) store_codes<8>(reinterpret_cast<uint8_t *>(codes) + row * codes_pitch + k, left, (reinterpret_cast<uintptr_t>(codes) | codes_pitch) % 8 == 0, code);
+    if (part % 4 == 0) exps[row * groups + part / 4] = (uint8_t)e;
+}
+
+// Other rows: a warp takes a group, lane = column, so that its loads are lines; eight groups in flight.
+constexpr int kRowsFlight = 8;
+template <typename T>
+__global__ void __launch_bounds__(256) rows8_compress_lanes_kernel(const T *__restrict__ x, long long pitch, long long rows, int cols,
+                                                                   int8_t *__restrict__ codes, long long codes_pitch, uint8_t *__restrict__ exps) {
+    after_previous_kernel();
     const int lane = threadIdx.x & 31, groups = rows8_groups(cols);
-    const long long unit = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);  // a warp per group
-    if (unit >= rows * groups) return;
-    const long long row = unit / groups;
-    const int g = (int)(unit - row * groups), k = g * kRowsGroup + lane;
-    const float v = k < cols ? as_float(x[row * pitch + k]) : 0.f;
-    const unsigned e = rows8_exponent(warp_max(magnitude(v)));
-    if (k < cols) codes[row * codes_pitch + k] = (int8_t)rows8_code(v, rows8_to_units(e));
-    if (lane == 0) exps[unit] = (uint8_t)e;
+    const long long first = ((long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kRowsFlight, units = rows * groups;
+    if (first >= units) return;
+    long long row = first / groups;
+    int g = (int)(first - row * groups);
+    float v[kRowsFlight];
+    long long r = row;
+    int h = g;
+#pragma unroll
+    for (int i = 0; i < kRowsFlight; ++i) {
+        const int k = h * kRowsGroup + lane;
+        v[i] = r < rows && k < cols ? as_float(x[r * pitch + k]) : 0.f;
+        if (++h == groups) {
+            h = 0;
+            ++r;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsFlight; ++i) {
+        const unsigned e = rows8_exponent(warp_max(magnitude(v[i])));
+        const int k = g * kRowsGroup + lane;
+        if (row < rows) {
+            if (k < cols) codes[row * codes_pitch + k] = (int8_t)rows8_code(v[i], rows8_to_units(e));
+            if (lane == 0) exps[row * groups + g] = (uint8_t)e;
+        }
+        if (++g == groups) {
+            g = 0;
+            ++row;
+        }
+    }
 }
 
 template <typename T>
@@ -34,15 +83,60 @@ __device__ __forceinline__ __half restored<__half>(float v) {  // the largest nu
     return __float2half_rn(fabsf(v) > 65504.f ? copysignf(65504.f, v) : v);
 }
 
+// A thread writes 16 bytes, wherever in a row they lie (rows of an odd number of columns follow one another without a gap).
 template <typename T>
 __global__ void __launch_bounds__(256) rows8_restore_kernel(const int8_t *__restrict__ codes, long long codes_pitch, const uint8_t *__restrict__ exps,
                                                             long long rows, int cols, T *__restrict__ out) {
     after_previous_kernel();
-    const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (at >= rows * cols) return;
-    const long long row = at / cols;
-    const int k = (int)(at - row * cols);
-    out[at] = restored<T>((float)codes[row * codes_pitch + k] * rows8_unit(exps[row * rows8_groups(cols) + k / kRowsGroup]));
+    constexpr int V = 16 / sizeof(T);
+    const long long first = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * V, total = rows * cols;
+    if (first >= total) return;
+    const int groups = rows8_groups(cols);
+    long long row = first / cols;
+    int k = (int)(first - row * cols);
+    union {
+        uint4 quad;
+        T value[V];
+    } u;
+    const int8_t *c = codes + row * codes_pitch;
+    const uint8_t *e = exps + row * groups;
+    if (k + V <= cols && k / kRowsGroup == (k + V - 1) / kRowsGroup) {  // within one group of one row
+        const float unit = rows8_unit(e[k / kRowsGroup]);
+        int code[V];
+        if ((reinterpret_cast<uintptr_t>(c + k)) % V == 0) {
+            if constexpr (V == 4) {
+                const char4 q = *reinterpret_cast<const char4 *>(c + k);
+                code[0] = q.x; code[1] = q.y; code[2] = q.z; code[3] = q.w;
+            } else {
+                const uint2 q = *reinterpret_cast<const uint2 *>(c + k);
+#pragma unroll
+                for (int i = 0; i < V; ++i) code[i] = (int)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i % 4)));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) code[i] = c[k + i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) u.value[i] = restored<T>((float)code[i] * unit);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            u.value[i] = row < rows ? restored<T>((float)c[k] * rows8_unit(e[k / kRowsGroup])) : T();
+            if (++k == cols) {
+                k = 0;
+                ++row;
+                c += codes_pitch;
+                e += groups;
+            }
+        }
+    }
+    if (first + V <= total && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+        *reinterpret_cast<uint4 *>(out + first) = u.quad;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (first + i < total) out[first + i] = u.value[i];
+    }
 }
 
 // Bits of h > 0: unit 32 w + i is bit i of word w.
@@ -91,10 +185,12 @@ int npa_rows8_compress(const void *x, int32_t type, int64_t x_pitch, int64_t row
     const int rc = check_rows8(me, x, type, codes, exponents, rows, cols, codes_pitch);
     if (rc != NPA_OK) return rc;
     if (x_pitch < 0) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: x_pitch must not be negative", me);
-    const long long units = rows * rows8_groups(cols);
     by_float_type(type, [&](auto t) {
-        launch_early(rows8_compress_kernel<decltype(t)>, (unsigned)((units + 7) / 8), 256, 0, (cudaStream_t)stream, static_cast<const decltype(t) *>(x), x_pitch,
-                     rows, cols, static_cast<int8_t *>(codes), codes_pitch, exponents);
+        using T = decltype(t);
+        const bool vectors = ((uintptr_t)x | (uintptr_t)(x_pitch * (int64_t)sizeof(T))) % 16 == 0;
+        const long long units = rows * rows8_groups(cols), blocks = vectors ? (4 * units + 255) / 256 : (units + 8 * kRowsFlight - 1) / (8 * kRowsFlight);
+        launch_early(vectors ? rows8_compress_kernel<T> : rows8_compress_lanes_kernel<T>, (unsigned)blocks, 256, 0, (cudaStream_t)stream,
+                     static_cast<const T *>(x), x_pitch, rows, cols, static_cast<int8_t *>(codes), codes_pitch, exponents);
     });
     return check_launch("rows8_compress_kernel");
 }
@@ -104,8 +200,10 @@ int npa_rows8_restore(const void *codes, int64_t codes_pitch, const uint8_t *exp
     const int rc = check_rows8(me, out, type, codes, exponents, rows, cols, codes_pitch);
     if (rc != NPA_OK) return rc;
     by_float_type(type, [&](auto t) {
-        launch_early(rows8_restore_kernel<decltype(t)>, (unsigned)((rows * cols + 255) / 256), 256, 0, (cudaStream_t)stream, static_cast<const int8_t *>(codes),
-                     codes_pitch, exponents, rows, cols, static_cast<decltype(t) *>(out));
+        using T = decltype(t);
+        const long long threads = (rows * cols * (int64_t)sizeof(T) + 15) / 16;
+        launch_early(rows8_restore_kernel<T>, (unsigned)((threads + 255) / 256), 256, 0, (cudaStream_t)stream, static_cast<const int8_t *>(codes), codes_pitch,
+                     exponents, rows, cols, static_cast<T *>(out));
     });
     return check_launch("rows8_restore_kernel");
 }

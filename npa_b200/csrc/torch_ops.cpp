@@ -868,7 +868,7 @@ Tensor linear_int8(const Tensor &x, const Tensor &w, const Tensor &w_scales, con
     const Tensor ws = w_scales.contiguous(), xs = given.defined() ? given.contiguous() : Tensor();
     Tensor out = fresh(x, shape, to);
     if (!r.rows || !n) return out;
-    const int64_t bytes = npa_linear_int8_scratch_bytes(type, r.rows, (int)r.cols);
+    const int64_t bytes = npa_linear_int8_scratch_bytes(r.data(), type, r.pitch, wr.data(), wr.pitch, r.rows, (int)r.cols, (int)n);
     Tensor scratch = bytes ? fresh(x, {bytes}, at::kByte) : Tensor();
     check_status(npa_linear_int8(r.data(), type, r.pitch, fptr(xs), wr.data(), wr.pitch, fptr(ws), b.defined() ? b.const_data_ptr() : nullptr, bias_type, relu,
                                  out.mutable_data_ptr(), type_code(to), r.rows, (int)r.cols, (int)n, bytes ? scratch.mutable_data_ptr() : nullptr, bytes,
@@ -893,7 +893,7 @@ Tensor mlp_int8(const Tensor &z, const Tensor &w1, const Tensor &w1_scales, cons
     shape.back() = n;
     Tensor y = floats(z, shape);
     if (!r.rows || !n) return y;
-    const int64_t bytes = npa_mlp_int8_scratch_bytes(r.rows, (int)r.cols, (int)hidden, (int)n);
+    const int64_t bytes = npa_mlp_int8_scratch_bytes(r.data(), r.pitch, r1.data(), r1.pitch, r2.data(), r2.pitch, r.rows, (int)r.cols, (int)hidden, (int)n);
     Tensor scratch = bytes ? fresh(z, {bytes}, at::kByte) : Tensor();
     check_status(npa_mlp_int8(fptr(r.t), r.pitch, r1.data(), r1.pitch, fptr(s1), fptr(b), r2.data(), r2.pitch, fptr(s2), fmut(y), r.rows, (int)r.cols, (int)hidden,
                               (int)n, bytes ? scratch.mutable_data_ptr() : nullptr, bytes, stream_of(z)));

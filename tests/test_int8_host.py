@@ -32,8 +32,8 @@ def test_bad_arguments_of_the_c_abi():
         (inv, "positive", lib.npa_linear_int8(ok, F32, 8, None, ok, 8, ok, None, 0, 0, ok, F32, 1, 8, 0, ok, 1 << 20, None)),
         (uns, "65536", lib.npa_linear_int8(ok, F32, 8, None, ok, 8, ok, None, 0, 0, ok, F32, 1, 65537, 8, ok, 1 << 20, None)),
         (inv, "scales", lib.npa_linear_int8(ok, I8, 8, None, ok, 8, ok, None, 0, 0, ok, F32, 1, 8, 8, None, 0, None)),
-        (inv, "scratch", lib.npa_linear_int8(ok, F32, 8, None, ok, 8, ok, None, 0, 0, ok, F32, 1, 8, 8, None, 0, None)),
-        (small, "needed", lib.npa_linear_int8(ok, F32, 8, None, ok, 8, ok, None, 0, 0, ok, F32, 1, 8, 8, ok, 8, None)),
+        (inv, "scratch", lib.npa_linear_int8(ok, F32, 8, None, ok, 16, ok, None, 0, 0, ok, F32, 100, 8, 8, None, 0, None)),
+        (small, "needed", lib.npa_linear_int8(ok, F32, 8, None, ok, 16, ok, None, 0, 0, ok, F32, 100, 8, 8, ok, 8, None)),
         (inv, "unknown type", lib.npa_linear_int8(ok, 9, 8, None, ok, 8, ok, None, 0, 0, ok, F32, 1, 8, 8, ok, 1 << 20, None)),
         (inv, "must be there", lib.npa_mlp_int8(ok, 8, ok, 16, ok, None, ok, 128, ok, ok, 1, 8, 128, 4, ok, 1 << 20, None)),
         (inv, "positive", lib.npa_rows8_compress(ok, F32, 8, 1, 0, ok, 16, ok, None)),
@@ -50,7 +50,10 @@ def test_bad_arguments_of_the_c_abi():
     assert [rc for _, _, rc in calls] == [want for want, _, _ in calls]
     rc = lib.npa_mlp_checkpoint_backward(ok, ok, ok, ok, ok, ok, ok, ok, None, ok, ok, 1, 8, 4, 8, 1, 128, 1, ok, 1 << 24, None)
     assert rc == inv and "together" in n.last_error()
-    assert lib.npa_linear_int8_scratch_bytes(I8, 10, 8) == 0 and lib.npa_linear_int8_scratch_bytes(F32, 10, 8) >= 10 * 16 + 40
+    room = lib.npa_linear_int8_scratch_bytes
+    assert room(ok, I8, 16, ok, 16, 100, 8, 4) == 0 and room(ok, F32, 8, ok, 16, 100, 8, 4) >= 100 * 16 + 400  # codes and scales of the rows
+    assert room(odd, I8, 16, ok, 16, 100, 8, 4) >= 100 * 16 and room(ok, I8, 8, ok, 16, 100, 8, 4) >= 100 * 16 and room(ok, I8, 16, odd, 16, 100, 8, 4) >= 4 * 16
+    assert room(ok, F32, 8, ok, 16, 1, 8, 4) == 0  # few rows: inside the kernel
 
 
 def test_int8_module_checks_its_shape_first():
