@@ -139,13 +139,6 @@ __global__ void __launch_bounds__(256) rows8_restore_kernel(const int8_t *__rest
     }
 }
 
-// Bits of h > 0: unit 32 w + i is bit i of word w.
-__global__ void __launch_bounds__(256) mask_bits_kernel(const float *__restrict__ h, long long rows, unsigned *__restrict__ mask) {
-    after_previous_kernel();
-    const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const unsigned bits = __ballot_sync(kFull, at < rows * kMaskHidden && h[at] > 0.f);
-    if ((threadIdx.x & 31) == 0 && at < rows * kMaskHidden) mask[at / 32] = bits;
-}
 __global__ void __launch_bounds__(256) apply_mask_kernel(float *__restrict__ a, float *__restrict__ b, long long rows, const unsigned *__restrict__ mask) {
     after_previous_kernel();
     const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -170,6 +163,14 @@ static int check_rows8(const char *me, const void *floats, int type, const void 
     if (!floats || !codes || !exps) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be non-NULL", me);
     if ((uintptr_t)floats % float_size(type)) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: the values must be aligned to their type", me);
     if (codes_pitch < cols) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: the rows of codes overlap", me);
+    return NPA_OK;
+}
+
+int check_mlp8(const char *me, int64_t rows, int32_t in_dim, int32_t out_dim) {
+    if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: rows, in_dim and out_dim must be positive", me);
+    if (rows > ((int64_t)1 << 31) - 1 || in_dim > 175 || out_dim > 48)
+        return fail(NPA_ERR_UNSUPPORTED, "%s: supports fewer than 2^31 rows, in <= 175 and out <= 48 (hidden width 128), got %lld, %d and %d", me, (long long)rows,
+                    in_dim, out_dim);
     return NPA_OK;
 }
 
@@ -209,38 +210,6 @@ int npa_rows8_restore(const void *codes, int64_t codes_pitch, const uint8_t *exp
 }
 
 static int64_t round_floats(int64_t n) { return (n + 63) / 64 * 64; }
-
-static int check_mlp8(const char *me, int64_t rows, int32_t in_dim, int32_t out_dim) {
-    if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: rows, in_dim and out_dim must be positive", me);
-    if (rows > ((int64_t)1 << 31) - 1 || in_dim > 175 || out_dim > 48)
-        return fail(NPA_ERR_UNSUPPORTED, "%s: supports fewer than 2^31 rows, in <= 175 and out <= 48 (hidden width 128), got %lld, %d and %d", me, (long long)rows,
-                    in_dim, out_dim);
-    return NPA_OK;
-}
-
-int64_t npa_mlp_checkpoint_forward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim) {
-    if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return 0;
-    return npa_mlp_forward_tcgen05_scratch_bytes(in_dim, out_dim) + rows * kMaskHidden * 4;
-}
-
-int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1, const float *W2, float *y, int64_t rows, int32_t in_dim, int32_t out_dim,
-                               int64_t w1_stride_out, int64_t w1_stride_in, int64_t w2_stride_out, int64_t w2_stride_in, void *codes, uint8_t *exponents,
-                               uint32_t *mask, void *scratch, int64_t scratch_bytes, void *stream) {
-    const char *me = "npa_mlp_checkpoint_forward";
-    int rc = check_mlp8(me, rows, in_dim, out_dim);
-    if (rc != NPA_OK) return rc;
-    if (!z || !W1 || !b1 || !W2 || !y || !codes || !exponents || !mask) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be non-NULL", me);
-    if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)mask) % 16)
-        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, mask and scratch must be there, 16-byte aligned", me);
-    const int64_t need = npa_mlp_checkpoint_forward_scratch_bytes(rows, in_dim, out_dim), image = npa_mlp_forward_tcgen05_scratch_bytes(in_dim, out_dim);
-    if (scratch_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: scratch has %lld bytes, %lld needed", me, (long long)scratch_bytes, (long long)need);
-    float *h = reinterpret_cast<float *>(static_cast<char *>(scratch) + image);
-    rc = npa_mlp_forward_tcgen05(z, W1, b1, W2, h, y, rows, in_dim, out_dim, w1_stride_out, w1_stride_in, w2_stride_out, w2_stride_in, scratch, image, stream);
-    if (rc != NPA_OK) return rc;
-    launch_early(mask_bits_kernel, (unsigned)((rows * kMaskHidden + 255) / 256), 256, 0, (cudaStream_t)stream, h, rows, mask);
-    if ((rc = check_launch("mask_bits_kernel")) != NPA_OK) return rc;
-    return npa_rows8_compress(z, NPA_FLOAT32, in_dim, rows, in_dim, codes, rows8_pitch(in_dim), exponents, stream);
-}
 
 int64_t npa_mlp_checkpoint_backward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim) {
     if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return 0;

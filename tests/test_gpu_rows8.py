@@ -144,15 +144,16 @@ def test_gradients_match_float64_truth(rows, k, o):
 
 
 def test_against_the_plain_backward():
-    """y bit by bit; dz and db1 those of the 32-bit backward; dW1 and dW2 within what half a unit of each code can move them."""
+    """y, dz and db1 those of the 32-bit pass to the rounding of both (twice the bar above); dW1 and dW2 within what half a unit of each
+    code can move them."""
     from npa_b200.rows8 import compress_rows
     module = _mlp(66, 18)
     w1, b1, w2 = (p.detach().double() for p in module.parameters())
     z, up = ref.clear_of_the_corner(_rand(5000, 66, seed=1), w1, b1)[:4000], _rand(4000, 18, seed=2)
     kept, plain = _run(module, z, up), _run(module, z, up, checkpoint=False)
-    assert torch.equal(kept[0], plain[0])
-    for k in (1, 3):
-        assert float((kept[k] - plain[k]).abs().max()) <= 4e-6 * float(plain[k].abs().max())
+    size = _magnitudes(z, *module.parameters(), up)
+    for k in (0, 1, 3):
+        assert float((kept[k] - plain[k]).abs().max()) <= 1e-5 * float(size[k].max())
     half = torch.repeat_interleave(torch.exp2(compress_rows(z).exponents.double() - 134), 32, -1)[:, :66]
     alive = (z.double() @ w1.t() + b1 > 0).double()
     dh = (up.double() @ w2) * alive
@@ -214,7 +215,7 @@ def test_what_is_asked_for_and_what_is_kept():
         p.requires_grad_(False)
     assert torch.equal(torch.autograd.grad(apply_mlp(module, zr, checkpoint=True), zr, up)[0], full[1])
     with torch.no_grad():
-        assert torch.equal(apply_mlp(module, zr, checkpoint=True), full[0])
+        assert torch.equal(apply_mlp(module, zr, checkpoint=True), apply_mlp(module, zr))
     for p in module.parameters():
         p.requires_grad_(True)
     y = apply_mlp(module, z[:, :0], checkpoint=True)
