@@ -1,0 +1,762 @@
+// Backward of the adaptation MLP from an 8-bit checkpoint (rows8.cuh; hidden width 128):
+//
+//     zh = restore(codes),  dh = bits * (dy W2),  h = bits * (zh W1^T + b1)
+//     dz = dh W1            (mlp_checkpoint_dz_kernel)
+//     dW1 = dh^T zh,  db1 = sum of dh,  dW2 = dy^T h      (mlp_checkpoint_weights_kernel)
+//
+// on the fifth-generation tensor cores at 32-bit accuracy with half the work of TF32: kind::f16 runs at twice its rate.  A number is
+// taken apart into a head and a tail of float16, 22 bits (the dropped tail x tail is 2^-24); zh needs no tail, its codes have 8 bits.
+// The price is float16's range, paid in powers of two, all exact:
+//
+//   * weights in units of their matrix, so that the largest is between 1 and 2;
+//   * dy in units of its row, again 1 to 2; dz's rows are independent and get their unit back in the epilogue, so that rows of any
+//     size keep their accuracy.  Sums over rows take a row with its unit relative to the largest of the tile of 128 rows (a factor on
+//     the operand that is rounded anyway), and the tile's unit comes in when its sum leaves the accumulator;
+//   * zh in units of the largest group of its tile: exact down to 2^-32 of it, below that towards zero.
+//
+// dh is |dy'| |W2'| <= 48 x 4 at most, so it fits float16 with 2^-25 below; nothing here can overflow.
+//
+// What goes through memory is the checkpoint, dy and dz: no kernel writes a hidden layer (dh is made twice: 6 of 86 or 18 of 127
+// thousand products a row, against 512 bytes each way).
+//
+// The layouts use that a swizzled tile of 16-bit numbers serves both ways: rows of 64 numbers (128 bytes, 128-byte swizzle) are a
+// K-major operand for sums over the columns and an MN-major one for sums over the rows.  So one image of W1 ([hidden][in]) is A of
+// zh W1^T and B of dh W1, and one tile of zh is B of both of its products, as is dy's.
+//
+// Waits are bounded as in umma.cuh; they report through npa_linear_tcgen05_status (bits 1024, 2048, 4096: MMA lane, producers, epilogue).
+#include <mutex>
+
+#include "mlp_grad_reduce.cuh"
+#include "rows8.cuh"
+#include "umma.cuh"
+
+namespace npa {
+
+constexpr int kCkRows = 128;
+constexpr int kCkTile = kCkRows * 128;   // bytes of 128 rows of 64 numbers
+constexpr int kCkThreads = 12 * 32, kCkProducer0 = 8, kCkProducers = 4;  // (twelve warps: 168 registers a thread; a thirteenth would cost 40 of them)
+constexpr int kCkMaxIn = 176, kCkMaxOut = 48;
+constexpr int kCkHeader = 1024;          // bytes of the image in front of the matrices
+constexpr int kCkRowRing = 8;            // tiles whose rows' units are kept
+
+enum { CK_STATUS_MMA = 1024, CK_STATUS_PRODUCER = 2048, CK_STATUS_EPILOGUE = 4096 };
+
+unsigned *umma_status_word();  // mlp_tcgen05.cu
+int launch_grad_reduce(const GradReduce &a, cudaStream_t st);  // mlp_grad_tcgen05.cu
+
+// ---- numbers ---------------------------------------------------------------------------------------------------------
+// Exponent of the power of two at or below a magnitude; 0 for zero and for what is not finite (it goes through unscaled).
+__device__ __forceinline__ int binade(unsigned magnitude_bits) {
+    return magnitude_bits == 0 || magnitude_bits >= 0x7f800000u ? 0 : max((int)(magnitude_bits >> 23), 1) - 127;
+}
+__device__ __forceinline__ float power_of_two(int e) { return e < -126 ? 0.f : __uint_as_float((unsigned)(min(e, 127) + 127) << 23); }
+// a in the lower half.
+__device__ __forceinline__ unsigned pack_halves(float a, float b) {
+    unsigned r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_halves(unsigned v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+// Heads and tails of two numbers.
+__device__ __forceinline__ void split_halves(float a, float b, unsigned &head, unsigned &tail) {
+    head = pack_halves(a, b);
+    const float2 h = unpack_halves(head);
+    tail = pack_halves(a - h.x, b - h.y);
+}
+// Byte of number (row, k), k < 64, in a swizzled tile.
+__host__ __device__ constexpr int half_place(int row, int k) { return row * 128 + ((((k >> 3) ^ row) & 7) << 4) + (k & 7) * 2; }
+
+// ---- the weights' image ------------------------------------------------------------------------------------------------
+struct CkHeader {
+    int w1, w2, b1;  // exponents of the units of W1 and W2, and of the largest bias (-1000: there is none)
+};
+struct CkImageArgs {
+    const float *W1, *b1, *W2;
+    long long s1o, s1i, s2o, s2i;
+    int in, out, chunks;
+    uint8_t *image;  // header | W1 heads [chunks] | W1 tails [chunks] | W2 heads | W2 tails, each 128 rows of 64 numbers
+};
+__global__ void __launch_bounds__(512) mlp_checkpoint_image_kernel(const __grid_constant__ CkImageArgs a) {
+    after_previous_kernel();
+    __shared__ unsigned most[3];
+    if (threadIdx.x < 3) most[threadIdx.x] = 0;
+    __syncthreads();
+    unsigned m[3] = {};
+    // every block looks at all weights: they are few, and a launch in between would cost more
+#pragma unroll 8
+    for (int q = threadIdx.x; q < 128 * a.in; q += 512) {
+        const int j = q / a.in, k = q - j * a.in;
+        m[0] = max(m[0], magnitude(__ldg(a.W1 + j * a.s1o + k * a.s1i)));
+    }
+#pragma unroll 4
+    for (int q = threadIdx.x; q < 128 * a.out; q += 512) m[1] = max(m[1], magnitude(__ldg(a.W2 + (q >> 7) * a.s2o + (q & 127) * a.s2i)));
+    if (threadIdx.x < 128) m[2] = magnitude(__ldg(a.b1 + threadIdx.x));
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        m[q] = warp_max(m[q]);
+        if (threadIdx.x % 32 == 0) atomicMax(&most[q], m[q]);
+    }
+    __syncthreads();
+    const int e1 = min(binade(most[0]), 126), e2 = min(binade(most[1]), 126);
+    const float u1 = power_of_two(-e1), u2 = power_of_two(-e2);
+    const int pairs1 = a.chunks * 128 * 32, total = pairs1 + 128 * 32;
+    for (int q = blockIdx.x * 512 + threadIdx.x; q < total; q += gridDim.x * 512) {
+        const bool first = q < pairs1;
+        const int at = first ? q : q - pairs1, row = (at >> 5) & 127, c = at >> 12, k = c * 64 + 2 * (at & 31);
+        float v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            v[i] = first ? (k + i < a.in ? __ldg(a.W1 + row * a.s1o + (k + i) * a.s1i) * u1 : 0.f)
+                         : (k + i < a.out ? __ldg(a.W2 + (k + i) * a.s2o + row * a.s2i) * u2 : 0.f);
+        unsigned head, tail;
+        split_halves(v[0], v[1], head, tail);
+        uint8_t *base = a.image + kCkHeader + (first ? (long long)c : 2ll * a.chunks) * kCkTile;
+        const int place = half_place(row, k & 63);
+        *reinterpret_cast<unsigned *>(base + place) = head;
+        *reinterpret_cast<unsigned *>(base + (first ? a.chunks : 1) * kCkTile + place) = tail;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<CkHeader *>(a.image) = CkHeader{e1, e2, most[2] == 0 ? -1000 : binade(most[2])};
+}
+
+// ---- what both kernels share ---------------------------------------------------------------------------------------------
+// Operand of rows of 64 numbers with the summed index along the rows (MN-major): groups of eight rows 1024 bytes apart, the next 64
+// columns `next_bytes` further.
+__device__ inline uint64_t umma_desc_rows(unsigned smem_addr, unsigned next_bytes) {
+    return (uint64_t)((smem_addr >> 4) & 0x3fffu) | ((uint64_t)((next_bytes >> 4) & 0x3fffu) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ inline void umma_f16(unsigned d_tmem, uint64_t a_desc, uint64_t b_desc, unsigned idesc, int accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// A from tensor memory: 128 lanes x 8 columns of two numbers.
+__device__ inline void umma_f16_ts(unsigned d_tmem, unsigned a_tmem, uint64_t b_desc, unsigned idesc, int accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// M = 128, float16 x float16 -> 32 bits; `rows_b`: B is summed along its rows.
+__device__ constexpr unsigned f16_idesc(int n, bool rows_b) {
+    return (1u << 4) | (rows_b ? 1u << 16 : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(128 >> 4) << 24);
+}
+
+struct CkArgs {
+    const int8_t *codes;
+    const uint8_t *exponents;
+    const uint4 *mask;
+    const float *dy, *b1;
+    const uint8_t *image;
+    float *dz, *partial;   // dz [rows, in]; partial [ctas][128][N1p + N2p], db1 in column `in`
+    long long rows;
+    int in, out, pitch, chunks, N1p, N2p, tiles;
+    unsigned *status;
+};
+
+// One producer warp's 32 rows of dy, lane = column: loaded (two columns a lane) ...
+template <bool TWO>
+struct DyRows {
+    float v[32][TWO ? 2 : 1];
+    __device__ __forceinline__ void load(const CkArgs &a, long long row0, int lane) {
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+            const bool there = row0 + r < a.rows;
+            const float *p = a.dy + (row0 + r) * a.out + lane;
+            v[r][0] = there && lane < a.out ? __ldg(p) : 0.f;
+            if constexpr (TWO) v[r][1] = there && lane + 32 < a.out ? __ldg(p + 32) : 0.f;
+        }
+    }
+    // ... and stored as heads and tails in units of their rows, whose exponents go to `units`.
+    __device__ __forceinline__ void store(uint8_t *heads, uint8_t *tails, int *units, int first, int lane) const {
+        int mine = 0;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+            unsigned m = magnitude(v[r][0]);
+            if constexpr (TWO) m = max(m, magnitude(v[r][1]));
+            m = warp_max(m);
+            const int e = m == 0 ? -126 : binade(m);
+            if (lane == r) mine = e;
+            const float unit = power_of_two(-e);  // (e = 127: 2^-127 is not a normal number; zero would lose the row)
+            const float s = e == 127 ? 0.5f * power_of_two(-126) : unit;
+#pragma unroll
+            for (int c = 0; c < (TWO ? 2 : 1); ++c) {
+                const float x = v[r][c] * s;
+                const __half h = __float2half_rn(x);
+                const int place = half_place(first + r, lane + 32 * c);
+                *reinterpret_cast<__half *>(heads + place) = h;
+                *reinterpret_cast<__half *>(tails + place) = __float2half_rn(x - __half2float(h));
+            }
+        }
+        units[first + lane] = mine;
+    }
+};
+
+__device__ __forceinline__ void ck_copy_image(uint8_t *dst, const CkArgs &a, uint64_t *bar) {
+    const int tiles = 2 * a.chunks + 2;
+    mbar_arrive_expect(bar, (unsigned)(tiles * kCkTile));
+    for (int q = 0; q < tiles; ++q) bulk_copy_g2s(dst + q * kCkTile, a.image + kCkHeader + (long long)q * kCkTile, kCkTile, bar);
+}
+
+// ---- dz ----------------------------------------------------------------------------------------------------------------
+// Warp-specialised, one persistent CTA per SM, tiles of 128 rows: four producer warps (32 rows of dy each, a tile ahead in registers;
+// a lane of the first issues the MMAs), four warps that mask dh and take it apart in place (lane = row; head and tail of 16 columns fill the 16 columns
+// of the accumulator they came from), four that store dz.  dh has two accumulators, so that the next tile's is made meanwhile.
+struct CkDzShared {
+    uint64_t image, op_full[2], op_empty[2], dh_full[2], dh_ready[2], dz_full, dz_empty;
+    int units[kCkRowRing][kCkRows];
+    uint32_t tmem_base;
+    int abort;
+};
+constexpr int kCkStagePitch = 36;  // floats of a staged row of 32 columns
+constexpr int kCkDzCol = 256;
+static int ck_dz_smem(int chunks) { return 1024 + (2 * chunks + 2) * kCkTile + 4 * kCkTile + 4 * 32 * kCkStagePitch * 4; }
+
+// 32 staged rows of 32 columns to rows of `pitch` floats, V at a time.
+template <int V>
+__device__ __forceinline__ void store_block(const float *stg, float *out, long long pitch, int nrows, int ncols, int lane) {
+    constexpr int kLanes = 32 / V, kStep = 32 / kLanes;
+    const int c = (lane % kLanes) * V, r0 = lane / kLanes;
+    if (c >= ncols) return;
+#pragma unroll 8
+    for (int r = r0; r < nrows; r += kStep) {
+        if constexpr (V == 4) *reinterpret_cast<float4 *>(out + r * pitch + c) = *reinterpret_cast<const float4 *>(stg + r * kCkStagePitch + c);
+        else if constexpr (V == 2) *reinterpret_cast<float2 *>(out + r * pitch + c) = *reinterpret_cast<const float2 *>(stg + r * kCkStagePitch + c);
+        else out[r * pitch + c] = stg[r * kCkStagePitch + c];
+    }
+}
+
+template <bool TWO>
+__global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const __grid_constant__ CkArgs a) {
+    after_previous_kernel();
+    extern __shared__ uint8_t ck_raw[];
+    __shared__ CkDzShared sh;
+    uint8_t *base = ck_raw + ((1024u - (smem_u32(ck_raw) & 1023u)) & 1023u);
+    uint8_t *w2 = base + 2 * a.chunks * kCkTile, *ops = w2 + 2 * kCkTile;  // ops: [2][head | tail]
+    float *staged = reinterpret_cast<float *>(ops + 4 * kCkTile);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(&sh.image, 1);
+        for (int q = 0; q < 2; ++q) {
+            mbar_init(&sh.op_full[q], kCkProducers);
+            mbar_init(&sh.op_empty[q], 1);
+            mbar_init(&sh.dh_full[q], 1);
+            mbar_init(&sh.dh_ready[q], 4);
+        }
+        mbar_init(&sh.dz_full, 2);  // the products, and the MMA lane itself: what it has seen of the producers' writes the epilogue sees
+        mbar_init(&sh.dz_empty, 4);
+        sh.abort = 0;
+        mbar_fence_init();
+    }
+    if (warp == kCkProducer0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = sh.tmem_base;
+    const int ntile = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+    auto row_of = [&](int it) { return ((long long)blockIdx.x + (long long)it * gridDim.x) * kCkRows; };
+    bool ok = true;
+
+    if (warp >= kCkProducer0) {
+        // the first of the producers issues the MMAs as well (one lane): dh of a tile as soon as its operands are there, then dz of the
+        // tile before
+        const bool issues = warp == kCkProducer0;
+        const int mine = (warp - kCkProducer0) * 32;
+        if (issues && lane == 0) ck_copy_image(base, a, &sh.image);
+        const unsigned id1 = f16_idesc(128, false), id2 = f16_idesc((a.in + 15) / 16 * 16, true);
+        const int ks1 = (a.out + 15) / 16;
+        const uint64_t w2h = umma_desc(smem_u32(w2)), w2l = umma_desc(smem_u32(w2 + kCkTile));
+        const unsigned w1h = smem_u32(base), w1l = smem_u32(base + a.chunks * kCkTile);
+        auto first = [&](int t) -> bool {
+            const int b = t & 1;
+            if (t == 0 && !umma_wait(&sh.image, 0, &sh.abort)) return false;
+            if (!umma_wait(&sh.op_full[b], (t >> 1) & 1, &sh.abort)) return false;
+            if (t > 1 && !umma_wait(&sh.dz_full, t & 1, &sh.abort)) return false;  // this accumulator was the operand of tile t - 2
+            tc_fence_after();
+            const uint64_t dh = umma_desc(smem_u32(ops + b * 2 * kCkTile)), dl = umma_desc(smem_u32(ops + b * 2 * kCkTile + kCkTile));
+            const unsigned d = tmem + b * 128;
+            for (int ks = 0; ks < ks1; ++ks) {  // the small products first: an addition cuts off what lies below the sum's last bit
+                umma_f16(d, dl + 2 * ks, w2h + 2 * ks, id1, ks != 0);
+                umma_f16(d, dh + 2 * ks, w2l + 2 * ks, id1, 1);
+            }
+            for (int ks = 0; ks < ks1; ++ks) umma_f16(d, dh + 2 * ks, w2h + 2 * ks, id1, 1);
+            umma_commit(&sh.op_empty[b]);
+            umma_commit(&sh.dh_full[b]);
+            return true;
+        };
+        auto second = [&](int t) -> bool {
+            const int b = t & 1;
+            if (!umma_wait(&sh.dh_ready[b], (t >> 1) & 1, &sh.abort)) return false;
+            if (!umma_wait(&sh.dz_empty, (t & 1) ^ 1, &sh.abort)) return false;
+            tc_fence_after();
+            const unsigned d = tmem + kCkDzCol, ah = tmem + b * 128;
+            for (int ks = 0; ks < 8; ++ks) {  // 16 hidden units: 2048 bytes of W1's rows
+                umma_f16_ts(d, ah + 16 * ks + 8, umma_desc_rows(w1h + 2048 * ks, kCkTile), id2, ks != 0);
+                umma_f16_ts(d, ah + 16 * ks, umma_desc_rows(w1l + 2048 * ks, kCkTile), id2, 1);
+            }
+            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(d, ah + 16 * ks, umma_desc_rows(w1h + 2048 * ks, kCkTile), id2, 1);
+            umma_commit(&sh.dz_full);
+            mbar_arrive(&sh.dz_full);
+            return true;
+        };
+        DyRows<TWO> rows;
+        if (ntile > 0) rows.load(a, row_of(0) + mine, lane);
+#pragma unroll 1
+        for (int t = 0; t < ntile && ok; ++t) {
+            const int b = t & 1;
+            if (!(ok = umma_wait(&sh.op_empty[b], ((t >> 1) & 1) ^ 1, &sh.abort))) break;
+            rows.store(ops + b * 2 * kCkTile, ops + b * 2 * kCkTile + kCkTile, sh.units[t % kCkRowRing], mine, lane);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.op_full[b]);
+            if (t + 1 < ntile) rows.load(a, row_of(t + 1) + mine, lane);
+            if (issues) {
+                if (lane == 0) {
+                    ok = first(t) && (t == 0 || second(t - 1));
+                    if (ok && t + 1 == ntile) ok = second(t);
+                }
+                ok = __shfl_sync(kFull, (int)ok, 0) != 0;
+            }
+        }
+        if (!ok && lane == 0) {
+            atomicOr(a.status, issues ? CK_STATUS_MMA : CK_STATUS_PRODUCER);
+            __nanosleep(20000);  // copies in flight land before the CTA leaves
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        const unsigned tlane = tmem + ((unsigned)(warp * 32) << 16);
+#pragma unroll 1
+        for (int t = 0; t < ntile; ++t) {
+            const int b = t & 1;
+            const long long row = row_of(t) + warp * 32 + lane;
+            const uint4 m = row < a.rows ? __ldg(a.mask + row) : make_uint4(0, 0, 0, 0);
+            if (!(ok = umma_wait(&sh.dh_full[b], (t >> 1) & 1, &sh.abort))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const unsigned word = c < 2 ? m.x : c < 4 ? m.y : c < 6 ? m.z : m.w, bits = c & 1 ? word >> 16 : word;
+                unsigned r[16], parts[16];
+                tmem_ld16(tlane + b * 128 + 16 * c, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    split_halves(bits >> (2 * j) & 1u ? __uint_as_float(r[2 * j]) : 0.f, bits >> (2 * j + 1) & 1u ? __uint_as_float(r[2 * j + 1]) : 0.f, parts[j],
+                                 parts[8 + j]);
+                tmem_st16(tlane + b * 128 + 16 * c, parts);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.dh_ready[b]);
+        }
+        if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_EPILOGUE);
+    } else {
+        const int quarter = warp & 3;
+        const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16) + kCkDzCol;
+        float *stg = staged + quarter * 32 * kCkStagePitch;
+        const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
+        const float u1 = power_of_two(head.w1), u2 = power_of_two(head.w2);
+        const int vec = a.in % 4 == 0 && (uintptr_t)a.dz % 16 == 0 ? 4 : a.in % 2 == 0 && (uintptr_t)a.dz % 8 == 0 ? 2 : 1;
+#pragma unroll 1
+        for (int t = 0; t < ntile; ++t) {
+            const long long row0 = row_of(t) + quarter * 32;
+            const int nrows = a.rows - row0 < 32 ? (int)(a.rows - row0) : 32;  // may be <= 0
+            if (!(ok = umma_wait(&sh.dz_full, t & 1, &sh.abort))) break;
+            tc_fence_after();
+            const float unit = power_of_two(sh.units[t % kCkRowRing][quarter * 32 + lane]);
+#pragma unroll 1
+            for (int c0 = 0; c0 < a.in; c0 += 32) {
+                unsigned r[2][16];
+                tmem_ld16(tlane + c0, r[0]);
+                if (c0 + 16 < a.in) tmem_ld16(tlane + c0 + 16, r[1]);
+                tc_wait_ld();
+                if (c0 + 32 >= a.in) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.dz_empty);
+                }
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    float v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[q / 4][4 * (q % 4) + j]) * u1 * u2 * unit;
+                    *reinterpret_cast<float4 *>(stg + lane * kCkStagePitch + 4 * q) = make_float4(v[0], v[1], v[2], v[3]);
+                }
+                __syncwarp();
+                float *out = a.dz + row0 * a.in + c0;
+                if (vec == 4) store_block<4>(stg, out, a.in, nrows, a.in - c0, lane);
+                else if (vec == 2) store_block<2>(stg, out, a.in, nrows, a.in - c0, lane);
+                else store_block<1>(stg, out, a.in, nrows, a.in - c0, lane);
+                __syncwarp();
+            }
+        }
+        if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_EPILOGUE);
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kCkProducer0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// ---- the weights' gradients -----------------------------------------------------------------------------------------------
+// The same tiles with lane = hidden unit: zh W1^T and dy W2 come out transposed, masked and taken apart in place they are the A operands
+// of the sums over the tile's rows.  The bits of 32 units and a row are one word, the same for a warp.  A tile's sums leave the
+// accumulators with the tile's unit and are added in 32 bits, in registers: up to 7 blocks of 16 columns a thread (kBlocks).
+struct CkWeightsShared {
+    uint64_t image, op_full, op_empty, p1_full, a_ready, p2_full;
+    alignas(16) unsigned mask[4][kCkRows];
+    alignas(16) int units[kCkRows];
+    float both[kCkRows];
+    int z_unit;
+    uint32_t tmem_base;
+    int abort;
+};
+constexpr int kCkPreCol = 0, kCkDhCol = 128, kCkW1Col = 256, kCkW2Col = 448;
+static int ck_weights_smem(int chunks) { return 1024 + (2 * chunks + 2) * kCkTile + chunks * kCkTile + 2 * kCkTile; }
+
+// Sixteen codes as numbers of float16 in units of 2^-8 of the tile's: exact while they are normal or fit the subnormal ones.
+__device__ __forceinline__ void decode_codes(const uint4 &q, __half2 scale, uint4 &lo, uint4 &hi) {
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
+    unsigned out[8];
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1024 + 128
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned u = w[i] ^ 0x80808080u;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const unsigned p = __byte_perm(u, 0x64646464u, j ? 0x4342 : 0x4140);  // 0x64uu: 1024 + code + 128
+            const __half2 v = __hmul2(__hsub2(*reinterpret_cast<const __half2 *>(&p), bias), scale);
+            out[2 * i + j] = *reinterpret_cast<const unsigned *>(&v);
+        }
+    }
+    lo = make_uint4(out[0], out[1], out[2], out[3]);
+    hi = make_uint4(out[4], out[5], out[6], out[7]);
+}
+
+template <int kBlocks, bool TWO>
+__global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(const __grid_constant__ CkArgs a) {
+    after_previous_kernel();
+    extern __shared__ uint8_t ck_raw[];
+    __shared__ CkWeightsShared sh;
+    uint8_t *base = ck_raw + ((1024u - (smem_u32(ck_raw) & 1023u)) & 1023u);
+    uint8_t *w2 = base + 2 * a.chunks * kCkTile, *zt = w2 + 2 * kCkTile, *dyt = zt + a.chunks * kCkTile;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(&sh.image, 1);
+        mbar_init(&sh.op_full, kCkProducers);
+        mbar_init(&sh.op_empty, 1);
+        mbar_init(&sh.p1_full, 2);  // the products, and the MMA lane itself: what it has seen of the producers' writes the epilogue sees
+        mbar_init(&sh.a_ready, 8);
+        mbar_init(&sh.p2_full, 1);
+        sh.abort = 0;
+        mbar_fence_init();
+    }
+    if (warp == kCkProducer0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = sh.tmem_base;
+    const int ntile = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+    auto row_of = [&](int it) { return ((long long)blockIdx.x + (long long)it * gridDim.x) * kCkRows; };
+    bool ok = true;
+
+    if (warp >= kCkProducer0) {
+        // the first of the producers issues the MMAs as well (one lane): the operands have one buffer, so it would wait for them anyway
+        const bool issues = warp == kCkProducer0;
+        if (issues && lane == 0) ck_copy_image(base, a, &sh.image);
+        const int n1 = (a.in + 15) / 16 * 16, n2 = (a.out + 15) / 16 * 16, ks1 = n1 / 16, ks2 = n2 / 16;
+        const unsigned id = f16_idesc(128, false), id1 = f16_idesc(n1, true), id2 = f16_idesc(n2, true);
+        const uint64_t w1h = umma_desc(smem_u32(base)), w1l = umma_desc(smem_u32(base + a.chunks * kCkTile));
+        const uint64_t w2h = umma_desc(smem_u32(w2)), w2l = umma_desc(smem_u32(w2 + kCkTile));
+        const uint64_t zk = umma_desc(smem_u32(zt)), dyh = umma_desc(smem_u32(dyt)), dyl = umma_desc(smem_u32(dyt + kCkTile));
+        const unsigned z0 = smem_u32(zt), dy0 = smem_u32(dyt);
+        auto products = [&](int t) -> bool {
+            if (t == 0 && !umma_wait(&sh.image, 0, &sh.abort)) return false;
+            if (!umma_wait(&sh.op_full, t & 1, &sh.abort)) return false;
+            tc_fence_after();
+            // (the A operands of tile t - 1 lay where these go: the producers have waited for its products)
+            auto k = [](int ks) { return (uint64_t)((ks >> 2) * (kCkTile >> 4) + 2 * (ks & 3)); };  // 16 columns further
+            const unsigned pre = tmem + kCkPreCol, dh = tmem + kCkDhCol;
+            for (int ks = 0; ks < ks2; ++ks) {
+                umma_f16(dh, w2l + 2 * ks, dyh + 2 * ks, id, ks != 0);
+                umma_f16(dh, w2h + 2 * ks, dyl + 2 * ks, id, 1);
+            }
+            for (int ks = 0; ks < ks2; ++ks) umma_f16(dh, w2h + 2 * ks, dyh + 2 * ks, id, 1);
+            for (int ks = 0; ks < ks1; ++ks) umma_f16(pre, w1l + k(ks), zk + k(ks), id, ks != 0);
+            for (int ks = 0; ks < ks1; ++ks) umma_f16(pre, w1h + k(ks), zk + k(ks), id, 1);
+            umma_commit(&sh.p1_full);
+            mbar_arrive(&sh.p1_full);
+            if (!umma_wait(&sh.a_ready, t & 1, &sh.abort)) return false;  // which also says that tile t - 1 has left its accumulators
+            tc_fence_after();
+            const unsigned g1 = tmem + kCkW1Col, g2 = tmem + kCkW2Col;
+            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks + 8, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, ks != 0);
+            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, 1);
+            for (int ks = 0; ks < 8; ++ks) {
+                umma_f16_ts(g2, pre + 16 * ks + 8, umma_desc_rows(dy0 + 2048 * ks, kCkTile), id2, ks != 0);
+                umma_f16_ts(g2, pre + 16 * ks, umma_desc_rows(dy0 + kCkTile + 2048 * ks, kCkTile), id2, 1);
+            }
+            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g2, pre + 16 * ks, umma_desc_rows(dy0 + 2048 * ks, kCkTile), id2, 1);
+            umma_commit(&sh.op_empty);
+            umma_commit(&sh.p2_full);
+            return true;
+        };
+        const int first = (warp - kCkProducer0) * 32, groups = (a.in + 31) / 32, units = a.pitch / 16;  // units of 16 codes in a row
+        DyRows<TWO> rows;
+        uint4 mask;
+        constexpr int kUnits = 11;
+        uint4 code[kUnits];
+        auto load = [&](int t) {
+            const long long row0 = row_of(t) + first;
+            rows.load(a, row0, lane);
+            mask = row0 + lane < a.rows ? __ldg(a.mask + row0 + lane) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {  // unit u of a row to 32 / ... lanes: flat, so that lines are read whole
+                const int q = i * 32 + lane;
+                code[i] = q < 32 * units && row0 + q / units < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.codes + row0 * a.pitch) + q) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        if (ntile > 0) load(0);
+#pragma unroll 1
+        for (int t = 0; t < ntile && ok; ++t) {
+            // the largest exponent of the tile, by each warp for itself
+            const long long tile0 = row_of(t);
+            const int there = a.rows - tile0 < kCkRows ? (int)(a.rows - tile0) : kCkRows;
+            int largest = 7;
+            for (int q = lane; q < there * groups; q += 32) {
+                const int e = __ldg(a.exponents + tile0 * groups + q);
+                if (e != 255) largest = max(largest, e);
+            }
+            largest = (int)warp_max((unsigned)largest);
+            if (!(ok = umma_wait(&sh.op_empty, (t & 1) ^ 1, &sh.abort))) break;
+            rows.store(dyt, dyt + kCkTile, sh.units, first, lane);
+            sh.mask[0][first + lane] = mask.x;
+            sh.mask[1][first + lane] = mask.y;
+            sh.mask[2][first + lane] = mask.z;
+            sh.mask[3][first + lane] = mask.w;
+            if (warp == kCkProducer0 && lane == 0) sh.z_unit = largest - 133 - 8;
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int q = i * 32 + lane, row = q / units, u = q - row * units;
+                if (row >= 32) continue;
+                const int e = tile0 + first + row < a.rows ? __ldg(a.exponents + (tile0 + first + row) * groups + u / 2) : 7;
+                const int d = e - largest + 8;  // (e of a group that is not finite lies above)
+                const __half s = e == 255 ? __ushort_as_half(0x7e00) : d < -24 ? __ushort_as_half(0) : __float2half_rn(power_of_two(d));
+                uint4 lo, hi;
+                decode_codes(code[i], __half2half2(s), lo, hi);
+                uint8_t *to = zt + (u / 4) * kCkTile;
+                const int k = 16 * (u % 4);
+                *reinterpret_cast<uint4 *>(to + half_place(first + row, k)) = lo;
+                *reinterpret_cast<uint4 *>(to + half_place(first + row, k + 8)) = hi;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.op_full);
+            if (t + 1 < ntile) load(t + 1);
+            if (issues) {
+                if (lane == 0) ok = products(t);
+                ok = __shfl_sync(kFull, (int)ok, 0) != 0;
+            }
+        }
+        if (!ok && lane == 0) {
+            atomicOr(a.status, issues ? CK_STATUS_MMA : CK_STATUS_PRODUCER);
+            __nanosleep(20000);  // copies in flight land before the CTA leaves
+        }
+        __syncwarp();
+    } else {
+        const int quarter = warp & 3, half = warp >> 2;  // hidden units 32 quarter + lane, rows 64 half .. + 63 of a tile
+        const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
+        const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
+        const float b1 = __ldg(a.b1 + quarter * 32 + lane);
+        const int nb1 = (a.in + 15) / 16, nb = nb1 + (a.out + 15) / 16;
+        float sums[kBlocks][16], db = 0.f;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[b][j] = 0.f;
+#pragma unroll 1
+        for (int t = 0; t < ntile; ++t) {
+            if (!(ok = umma_wait(&sh.p1_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
+            tc_fence_after();
+            // rows' units relative to the largest of the tile: a warp makes those of its half
+            int unit = -126;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) unit = max(unit, sh.units[32 * q + lane]);
+            unit = __reduce_max_sync(kFull, unit);
+            // units: zh 2^zu, W1 2^w1; h in units of 2^hu, which the largest sum (176 x 2 x 32512 in the accumulator's) and bias leave below 2^15
+            const int zu = sh.z_unit, hu = max(zu + head.w1 + 24, head.b1 + 2) - 15;
+            const float to_h = power_of_two(max(zu + head.w1 - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
+            float partial = 0.f;
+#pragma unroll 1
+            for (int c = 4 * half; c < 4 * half + 4; ++c) {
+                unsigned r[16], parts[16];
+                tmem_ld16(tlane + kCkDhCol + 16 * c, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const uint4 m = *reinterpret_cast<const uint4 *>(&sh.mask[quarter][16 * c + j]);
+                    const int4 u = *reinterpret_cast<const int4 *>(&sh.units[16 * c + j]);
+                    const unsigned mw[4] = {m.x, m.y, m.z, m.w};
+                    const int uw[4] = {u.x, u.y, u.z, u.w};
+                    float v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        v[q] = mw[q] >> lane & 1u ? __uint_as_float(r[j + q]) * power_of_two(uw[q] - unit) : 0.f;
+                        partial += v[q];
+                    }
+                    split_halves(v[0], v[1], parts[j / 2], parts[8 + j / 2]);
+                    split_halves(v[2], v[3], parts[j / 2 + 1], parts[8 + j / 2 + 1]);
+                }
+                tmem_st16(tlane + kCkDhCol + 16 * c, parts);
+                tmem_ld16(tlane + kCkPreCol + 16 * c, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const uint4 m = *reinterpret_cast<const uint4 *>(&sh.mask[quarter][16 * c + j]);
+                    const int4 u = *reinterpret_cast<const int4 *>(&sh.units[16 * c + j]);
+                    const unsigned mw[4] = {m.x, m.y, m.z, m.w};
+                    const int uw[4] = {u.x, u.y, u.z, u.w};
+                    float v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        v[q] = mw[q] >> lane & 1u ? __fmaf_rn(__uint_as_float(r[j + q]), to_h, bias) * power_of_two(uw[q] - unit) : 0.f;
+                    split_halves(v[0], v[1], parts[j / 2], parts[8 + j / 2]);
+                    split_halves(v[2], v[3], parts[j / 2 + 1], parts[8 + j / 2 + 1]);
+                }
+                tmem_st16(tlane + kCkPreCol + 16 * c, parts);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.a_ready);
+            const float unit_dh = power_of_two(unit), unit_w2 = power_of_two(head.w2);
+            db += partial * unit_w2 * unit_dh;
+            if (!(ok = umma_wait(&sh.p2_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
+            tc_fence_after();
+            const float unit_z = power_of_two(zu + 8) * 0.00390625f, unit_h = power_of_two(max(min(hu, 127), -126));
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) {
+                const int b = 2 * i + half;
+                if (b >= nb) break;
+                unsigned r[16];
+                tmem_ld16(tlane + (b < nb1 ? kCkW1Col + 16 * b : kCkW2Col + 16 * (b - nb1)), r);
+                tc_wait_ld();
+                const float f = b < nb1 ? unit_w2 * unit_z : unit_h;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sums[i][j] = __fadd_rn(sums[i][j], __uint_as_float(r[j]) * f * unit_dh);
+            }
+            tc_fence_before();
+        }
+        if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_EPILOGUE);
+        // db1 in column `in`: both halves of the rows through shared memory.  (A warp that gave up comes here as well: the barriers want all.)
+        float *prow = a.partial + ((long long)blockIdx.x * 128 + quarter * 32 + lane) * (a.N1p + a.N2p);
+        if (half == 1) sh.both[quarter * 32 + lane] = db;
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const int b = 2 * i + half;
+            if (b >= nb) break;
+            float *to = prow + (b < nb1 ? 16 * b : a.N1p + 16 * (b - nb1));
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4 *>(to + j) = make_float4(sums[i][j], sums[i][j + 1], sums[i][j + 2], sums[i][j + 3]);
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // (column `in` may lie in a block of the other half)
+        if (half == 0) prow[a.in] = db + sh.both[quarter * 32 + lane];
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kCkProducer0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+static int64_t ck_image_bytes(int in_dim) { return kCkHeader + (int64_t)(2 * ((in_dim + 63) / 64) + 2) * kCkTile; }
+static GradReduce ck_reduce(int64_t rows, int in_dim, int out_dim) {
+    GradReduce r = {};
+    const int64_t tiles = (rows + kCkRows - 1) / kCkRows;
+    r.in_dim = in_dim; r.out_dim = out_dim; r.N1p = grad_round16(in_dim + 1); r.N2p = grad_round16(out_dim);
+    r.ctas = (int)(tiles < 148 ? tiles : 148);
+    return r;
+}
+static int64_t ck_partial_floats(const GradReduce &r) { return (int64_t)r.ctas * kCkRows * (r.N1p + r.N2p); }
+
+template <typename Kernel>
+static int ck_launch(Kernel kernel, const char *name, const CkArgs &a, int smem, int ctas, cudaStream_t st) {
+    int unused = 0;  // raises the kernel's limit of shared memory on this device
+    const int rc = persistent_ctas(kernel, kCkThreads, (size_t)smem, &unused);
+    if (rc != NPA_OK) return rc;
+    launch_early(kernel, ctas, kCkThreads, (size_t)smem, st, a);
+    return check_launch(name);
+}
+
+int check_mlp8(const char *me, int64_t rows, int32_t in_dim, int32_t out_dim) {
+    if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: rows, in_dim and out_dim must be positive", me);
+    if (rows > ((int64_t)1 << 31) - 1 || in_dim > kCkMaxIn || out_dim > kCkMaxOut)
+        return fail(NPA_ERR_UNSUPPORTED, "%s: supports fewer than 2^31 rows, in <= %d and out <= %d (hidden width 128), got %lld, %d and %d", me, kCkMaxIn,
+                    kCkMaxOut, (long long)rows, in_dim, out_dim);
+    return NPA_OK;
+}
+
+}  // namespace npa
+
+using namespace npa;
+
+extern "C" {
+
+int64_t npa_mlp_checkpoint_backward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim) {
+    if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return 0;
+    return ck_image_bytes(in_dim) + 4 * ck_partial_floats(ck_reduce(rows, in_dim, out_dim));
+}
+
+int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, const uint32_t *mask, const float *W1, const float *b1, const float *W2,
+                                const float *dy, float *dz, float *dW1, float *db1, float *dW2, int64_t rows, int32_t in_dim, int32_t out_dim,
+                                int64_t w1_stride_out, int64_t w1_stride_in, int64_t w2_stride_out, int64_t w2_stride_in, void *scratch,
+                                int64_t scratch_bytes, void *stream) {
+    const char *me = "npa_mlp_checkpoint_backward";
+    int rc = check_mlp8(me, rows, in_dim, out_dim);
+    if (rc != NPA_OK) return rc;
+    if (!codes || !exponents || !mask || !W1 || !b1 || !W2 || !dy) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every input must be non-NULL", me);
+    if ((!dW1 || !db1 || !dW2) && (dW1 || db1 || dW2)) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: dW1, db1 and dW2 come together", me);
+    if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)mask | (uintptr_t)dy) % 16)
+        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, mask, dy and scratch must be there, 16-byte aligned", me);
+    if ((uintptr_t)dz % 4) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: dz must be float aligned", me);
+    const int64_t need = npa_mlp_checkpoint_backward_scratch_bytes(rows, in_dim, out_dim);
+    if (scratch_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: scratch has %lld bytes, %lld needed", me, (long long)scratch_bytes, (long long)need);
+    if (!dz && !dW1) return NPA_OK;
+    const cudaStream_t st = (cudaStream_t)stream;
+    GradReduce r = ck_reduce(rows, in_dim, out_dim);
+    CkArgs a = {};
+    a.codes = static_cast<const int8_t *>(codes); a.exponents = exponents; a.mask = reinterpret_cast<const uint4 *>(mask); a.dy = dy; a.b1 = b1;
+    a.image = static_cast<const uint8_t *>(scratch); a.dz = dz; a.partial = reinterpret_cast<float *>(static_cast<char *>(scratch) + ck_image_bytes(in_dim));
+    a.rows = rows; a.in = in_dim; a.out = out_dim; a.pitch = (int)rows8_pitch(in_dim); a.chunks = (in_dim + 63) / 64; a.N1p = r.N1p; a.N2p = r.N2p;
+    a.tiles = (int)((rows + kCkRows - 1) / kCkRows);
+    if (!(a.status = umma_status_word())) return fail(NPA_ERR_CUDA, "%s: no status word", me);
+    const CkImageArgs image{W1, b1, W2, w1_stride_out, w1_stride_in, w2_stride_out, w2_stride_in, in_dim, out_dim, a.chunks, static_cast<uint8_t *>(scratch)};
+    launch_early(mlp_checkpoint_image_kernel, 8 * (a.chunks + 1), 512, 0, st, image);
+    if ((rc = check_launch("mlp_checkpoint_image_kernel")) != NPA_OK) return rc;
+    const bool two = out_dim > 32;
+    if (dz && (rc = ck_launch(two ? mlp_checkpoint_dz_kernel<true> : mlp_checkpoint_dz_kernel<false>, "mlp_checkpoint_dz_kernel", a, ck_dz_smem(a.chunks), r.ctas, st)) !=
+                  NPA_OK)
+        return rc;
+    if (!dW1) return NPA_OK;
+    const bool few = (in_dim + 15) / 16 + (out_dim + 15) / 16 <= 8;
+    const auto kernel = few ? (two ? mlp_checkpoint_weights_kernel<4, true> : mlp_checkpoint_weights_kernel<4, false>)
+                            : (two ? mlp_checkpoint_weights_kernel<7, true> : mlp_checkpoint_weights_kernel<7, false>);
+    if ((rc = ck_launch(kernel, "mlp_checkpoint_weights_kernel", a, ck_weights_smem(a.chunks), r.ctas, st)) != NPA_OK) return rc;
+    r.partial = a.partial; r.dW1 = dW1; r.dW2 = dW2; r.db1 = db1;
+    return launch_grad_reduce(r, st);
+}
+
+}  // extern "C"

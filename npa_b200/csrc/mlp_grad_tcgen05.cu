@@ -354,6 +354,11 @@ __global__ void __launch_bounds__(kReduceQuads * kReduceRuns) mlp_grad_umma_redu
 }
 
 
+int launch_grad_reduce(const GradReduce &a, cudaStream_t st) {
+    mlp_grad_umma_reduce_kernel<<<a.blocks(kReduceQuads), kReduceQuads * kReduceRuns, 0, st>>>(a);
+    return check_launch("mlp_grad_umma_reduce_kernel");
+}
+
 struct GradDevice {
     unsigned *status = nullptr;
     bool smem_set[2] = {false, false};  // per shape
@@ -387,8 +392,7 @@ int npa_mlp_weight_grad_tcgen05(const float *z, const float *dh, const float *h,
     if (rc != NPA_OK) return rc;
     GradReduce a = grad_plan(rows, in_dim, out_dim);
     a.partial = scratch; a.dW1 = dW1; a.dW2 = dW2; a.db1 = db1;
-    mlp_grad_umma_reduce_kernel<<<a.blocks(kReduceQuads), kReduceQuads * kReduceRuns, 0, (cudaStream_t)stream>>>(a);
-    return check_launch("mlp_grad_umma_reduce_kernel");
+    return launch_grad_reduce(a, (cudaStream_t)stream);
 }
 
 int npa_mlp_weight_grad_tcgen05_partial(const float *z, const float *dh, const float *h, const float *dy, int64_t rows, int32_t in_dim,

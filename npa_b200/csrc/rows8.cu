@@ -1,16 +1,7 @@
-// Activations into 8 bits and back (rows8.cuh), and the adaptation MLP whose backward reads its input that way.
-//
-//     forward    y = relu(z W1^T + b1) W2^T                       keeps codes(z) and the bits of h > 0
-//     backward   h = bits * (restore(codes) W1^T + b1)            dh = bits * (dy W2)
-//                dz = dh W1,  dW1 = dh^T restore(codes),  db1 = sum of dh,  dW2 = dy^T h
-//
-// 1 + 1/32 byte per input and 16 bytes for the hidden layer instead of 4 per input and 512.  dz and db1 are those of the 32-bit
-// backward, because the bits are those of the forward; dW1 and dW2 see the rounding of z to codes.
+// Activations into 8 bits and back (rows8.cuh).  Reading and writing memory is all there is to either way.
 #include "rows8.cuh"
 
 namespace npa {
-
-constexpr int kMaskHidden = 128;
 
 // Rows whose addresses are multiples of 16 bytes: a thread takes eight values, four neighbours a group.
 template <typename T>
@@ -139,14 +130,6 @@ __global__ void __launch_bounds__(256) rows8_restore_kernel(const int8_t *__rest
     }
 }
 
-__global__ void __launch_bounds__(256) apply_mask_kernel(float *__restrict__ a, float *__restrict__ b, long long rows, const unsigned *__restrict__ mask) {
-    after_previous_kernel();
-    const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (at >= rows * kMaskHidden || (mask[at / 32] >> (at % 32) & 1u)) return;
-    a[at] = 0.f;
-    b[at] = 0.f;
-}
-
 template <typename F>
 static void by_float_type(int type, F f) {
     if (type == NPA_FLOAT32) f(float());
@@ -163,14 +146,6 @@ static int check_rows8(const char *me, const void *floats, int type, const void 
     if (!floats || !codes || !exps) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be non-NULL", me);
     if ((uintptr_t)floats % float_size(type)) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: the values must be aligned to their type", me);
     if (codes_pitch < cols) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: the rows of codes overlap", me);
-    return NPA_OK;
-}
-
-int check_mlp8(const char *me, int64_t rows, int32_t in_dim, int32_t out_dim) {
-    if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: rows, in_dim and out_dim must be positive", me);
-    if (rows > ((int64_t)1 << 31) - 1 || in_dim > 175 || out_dim > 48)
-        return fail(NPA_ERR_UNSUPPORTED, "%s: supports fewer than 2^31 rows, in <= 175 and out <= 48 (hidden width 128), got %lld, %d and %d", me, (long long)rows,
-                    in_dim, out_dim);
     return NPA_OK;
 }
 
@@ -207,44 +182,6 @@ int npa_rows8_restore(const void *codes, int64_t codes_pitch, const uint8_t *exp
                      exponents, rows, cols, static_cast<T *>(out));
     });
     return check_launch("rows8_restore_kernel");
-}
-
-static int64_t round_floats(int64_t n) { return (n + 63) / 64 * 64; }
-
-int64_t npa_mlp_checkpoint_backward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim) {
-    if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return 0;
-    return 4 * (round_floats(rows * in_dim) + 2 * round_floats(rows * kMaskHidden) + round_floats(npa_mlp_weight_grad_tcgen05_scratch_floats(rows, in_dim, out_dim))) +
-           npa_linear_tcgen05_scratch_bytes(in_dim, kMaskHidden) + npa_linear_tcgen05_scratch_bytes(out_dim, kMaskHidden) +
-           npa_linear_tcgen05_scratch_bytes(kMaskHidden, in_dim);
-}
-
-int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, const uint32_t *mask, const float *W1, const float *b1, const float *W2,
-                                const float *dy, float *dz, float *dW1, float *db1, float *dW2, int64_t rows, int32_t in_dim, int32_t out_dim,
-                                int64_t w1_stride_out, int64_t w1_stride_in, int64_t w2_stride_out, int64_t w2_stride_in, void *scratch,
-                                int64_t scratch_bytes, void *stream) {
-    const char *me = "npa_mlp_checkpoint_backward";
-    int rc = check_mlp8(me, rows, in_dim, out_dim);
-    if (rc != NPA_OK) return rc;
-    if (!codes || !exponents || !mask || !W1 || !b1 || !W2 || !dy) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every input must be non-NULL", me);
-    if ((!dW1 || !db1 || !dW2) && (dW1 || db1 || dW2)) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: dW1, db1 and dW2 come together", me);
-    if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)mask | (uintptr_t)dy) % 16)
-        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, mask, dy and scratch must be there, 16-byte aligned", me);
-    const int64_t need = npa_mlp_checkpoint_backward_scratch_bytes(rows, in_dim, out_dim);
-    if (scratch_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: scratch has %lld bytes, %lld needed", me, (long long)scratch_bytes, (long long)need);
-    float *z = static_cast<float *>(scratch), *h = z + round_floats(rows * in_dim), *dh = h + round_floats(rows * kMaskHidden),
-          *partial = dh + round_floats(rows * kMaskHidden);
-    const int64_t floats = npa_mlp_weight_grad_tcgen05_scratch_floats(rows, in_dim, out_dim), i1 = npa_linear_tcgen05_scratch_bytes(in_dim, kMaskHidden),
-                  i2 = npa_linear_tcgen05_scratch_bytes(out_dim, kMaskHidden), i3 = npa_linear_tcgen05_scratch_bytes(kMaskHidden, in_dim);
-    char *image = reinterpret_cast<char *>(partial + round_floats(floats));
-    if ((rc = npa_rows8_restore(codes, rows8_pitch(in_dim), exponents, rows, in_dim, z, NPA_FLOAT32, stream)) != NPA_OK) return rc;
-    if ((rc = npa_linear_tcgen05(z, W1, b1, nullptr, h, rows, in_dim, kMaskHidden, w1_stride_out, w1_stride_in, 0, image, i1, stream)) != NPA_OK) return rc;
-    if ((rc = npa_linear_tcgen05(dy, W2, nullptr, nullptr, dh, rows, out_dim, kMaskHidden, w2_stride_in, w2_stride_out, 0, image + i1, i2, stream)) != NPA_OK) return rc;
-    launch_early(apply_mask_kernel, (unsigned)((rows * kMaskHidden + 255) / 256), 256, 0, (cudaStream_t)stream, h, dh, rows, mask);
-    if ((rc = check_launch("apply_mask_kernel")) != NPA_OK) return rc;
-    if (dz && (rc = npa_linear_tcgen05(dh, W1, nullptr, nullptr, dz, rows, kMaskHidden, in_dim, w1_stride_in, w1_stride_out, 0, image + i1 + i2, i3, stream)) != NPA_OK)
-        return rc;
-    if (!dW1) return NPA_OK;
-    return npa_mlp_weight_grad_tcgen05(z, dh, h, dy, rows, in_dim, kMaskHidden, out_dim, partial, floats, dW1, dW2, db1, stream);
 }
 
 }  // extern "C"

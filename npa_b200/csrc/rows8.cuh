@@ -29,7 +29,7 @@ __device__ __forceinline__ int rows8_code(float x, float to_units) {
     return to_units == 0.f ? 0 : max(-127, min(127, __float2int_rn(x * to_units)));
 }
 
-// rows8.cu: the sizes that the MLP with a checkpoint takes.
+// mlp_checkpoint.cu: the sizes that the MLP with a checkpoint takes.
 int check_mlp8(const char *me, int64_t rows, int32_t in_dim, int32_t out_dim);
 
 }  // namespace npa

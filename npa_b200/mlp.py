@@ -134,12 +134,12 @@ def apply_mlp(module, z, checkpoint=False):
     ``checkpoint=True`` keeps for the backward, instead of ``z`` and the hidden layer in 32 bits (``4 (in + 128)`` bytes a
     row), ``z`` in 8 bits (``rows8``) and the bits of the ReLU (``in + in / 32 + 16`` bytes): values and the gradients of
     ``z`` and of the bias are those of the plain call, the gradients of the two weight matrices see ``z`` rounded to 8 bits.
-    It needs a ``supported`` module of at most 175 inputs on the default engine, and is refused (``ValueError``) otherwise;
+    It needs a ``supported`` module on the default engine, and is refused (``ValueError``) otherwise;
     without a gradient to record the call is the plain one."""
     if checkpoint and torch.is_grad_enabled():
-        if not (on_tensor_memory(module) and module[0].in_features <= MAX_IN_TCGEN05):
+        if not on_tensor_memory(module):
             raise ValueError("checkpoint=True needs Sequential(Linear(in, 128), ReLU, Linear(128, out, bias=False)) in float32 on a CUDA device "
-                             f"with in <= {MAX_IN_TCGEN05} and out <= {MAX_OUT}, on the default engine")
+                             f"with in <= {MAX_IN} and out <= {MAX_OUT}, on the default engine")
         if not (z.device == module[0].weight.device and z.dtype == torch.float32):
             raise TypeError(f"z: expected a float32 tensor on {module[0].weight.device}, got {z.dtype} on {z.device}")
         return N.ops.mlp_checkpoint(z.contiguous(), module[0].weight, module[0].bias, module[2].weight)

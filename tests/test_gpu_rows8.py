@@ -115,7 +115,7 @@ def _magnitudes(z, w1, b1, w2, up):
 
 
 NAMES = ["y", "dz", "dW1", "db1", "dW2"]
-SHAPES = [(1, 66, 18), (3, 1, 1), (31, 175, 48), (127, 43, 11), (128, 163, 35), (129, 66, 18), (1000, 34, 10), (2048, 5, 48), (4103, 163, 35), (20001, 83, 19),
+SHAPES = [(1, 66, 18), (3, 1, 1), (31, 175, 48), (127, 43, 11), (128, 163, 35), (129, 66, 18), (1000, 34, 10), (2048, 5, 48), (4103, 163, 35), (20001, 83, 19), (5000, 176, 33), (777, 64, 16), (300, 96, 32),
           (50000, 130, 34), (65536, 16, 16), (262144, 163, 35)]
 
 
