@@ -42,12 +42,7 @@ __global__ void __launch_bounds__(T > 128 ? T : 128) quantize_rows_kernel(const 
 #pragma unroll
         for (int q = 0; q < V; ++q) largest = max(largest, magnitude(quantizable<UNSIGNED>(w[q])));
     }
-    if constexpr (T >= 32) {
-        largest = warp_max(largest);
-    } else {
-#pragma unroll
-        for (int d = 1; d < T; d *= 2) largest = max(largest, __shfl_xor_sync(kFull, largest, d));
-    }
+    largest = warp_max<(T < 32 ? T : 32)>(largest);
     if constexpr (T > 32) {
         __shared__ unsigned most[T / 32];
         if (t % 32 == 0) most[t / 32] = largest;

@@ -56,7 +56,32 @@ __device__ __forceinline__ int row_code(float x, float scale, float inverse) {
     return (int)r;
 }
 
-__device__ __forceinline__ unsigned warp_max(unsigned v) { return __reduce_max_sync(kFull, v); }
+template <int LANES = 32>
+__device__ __forceinline__ unsigned warp_max(unsigned v) {
+#pragma unroll
+    for (int d = 1; d < LANES; d *= 2) v = max(v, __shfl_xor_sync(kFull, v, d));
+    return v;
+}
+// Eight maxima over the lanes of a group of LANES at once, each to all of its lanes: the lanes share the values out while they halve,
+// 8 or 9 shuffles for the maxima and 8 to hand them back instead of 32 or 40.
+template <int LANES = 32>
+__device__ __forceinline__ void warp_max8(unsigned (&v)[8]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int n = 4, d = LANES / 2; n >= 1; n /= 2, d /= 2) {
+        const bool up = lane & d;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const unsigned keep = up ? v[i + n] : v[i], send = up ? v[i] : v[i + n];
+            v[i] = max(keep, __shfl_xor_sync(kFull, send, d));
+        }
+    }
+    unsigned m = v[0];
+#pragma unroll
+    for (int d = LANES / 16; d >= 1; d /= 2) m = max(m, __shfl_xor_sync(kFull, m, d));
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] = __shfl_sync(kFull, m, (lane & ~(LANES - 1)) + r * (LANES / 8));
+}
 
 // V values at p, of which `left` exist.
 template <typename T, int V>

@@ -83,12 +83,20 @@ __global__ void __launch_bounds__(512) mlp_checkpoint_image_kernel(const __grid_
     __syncthreads();
     unsigned m[3] = {};
     // every block looks at all weights: they are few, and a launch in between would cost more
+    if (a.s1i == 1 && a.s1o == a.in && (uintptr_t)a.W1 % 16 == 0) {
+#pragma unroll 12
+        for (int q = threadIdx.x; q < 32 * a.in; q += 512) {
+            const float4 v = __ldg(reinterpret_cast<const float4 *>(a.W1) + q);
+            m[0] = max(m[0], max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w))));
+        }
+    } else {
 #pragma unroll 8
-    for (int q = threadIdx.x; q < 128 * a.in; q += 512) {
-        const int j = q / a.in, k = q - j * a.in;
-        m[0] = max(m[0], magnitude(__ldg(a.W1 + j * a.s1o + k * a.s1i)));
+        for (int q = threadIdx.x; q < 128 * a.in; q += 512) {
+            const int j = q / a.in, k = q - j * a.in;
+            m[0] = max(m[0], magnitude(__ldg(a.W1 + j * a.s1o + k * a.s1i)));
+        }
     }
-#pragma unroll 4
+#pragma unroll 12
     for (int q = threadIdx.x; q < 128 * a.out; q += 512) m[1] = max(m[1], magnitude(__ldg(a.W2 + (q >> 7) * a.s2o + (q & 127) * a.s2i)));
     if (threadIdx.x < 128) m[2] = magnitude(__ldg(a.b1 + threadIdx.x));
 #pragma unroll
@@ -156,41 +164,57 @@ struct CkArgs {
     unsigned *status;
 };
 
-// One producer warp's 32 rows of dy, lane = column: loaded (two columns a lane) ...
+// Exponent field of the unit of a row from its largest finite magnitude (a multiple of that unit is below 4; zero rows have the
+// smallest), and 1 / unit.
+__device__ __forceinline__ unsigned row_unit(unsigned largest) { return min(max(largest >> 23, 1u), 253u); }
+__device__ __forceinline__ float from_row_unit(unsigned field) { return __uint_as_float((254u - field) << 23); }
+// A magnitude as the unit sees it: what is not finite has no part in it, so that its neighbours keep their accuracy.
+__device__ __forceinline__ unsigned finite_magnitude(float v) {
+    const unsigned m = magnitude(v);
+    return m < 0x7f800000u ? m : 0u;
+}
+
+// One producer warp's 32 rows of dy, two neighbouring columns a lane: half a warp for a row of up to 32 columns, 24 lanes for one of up
+// to 48 (TWO).  Loaded a tile ahead ...
 template <bool TWO>
 struct DyRows {
-    float v[32][TWO ? 2 : 1];
+    static constexpr int kEach = TWO ? 1 : 2, kPasses = 32 / kEach;  // rows a pass
+    float2 v[kPasses];
     __device__ __forceinline__ void load(const CkArgs &a, long long row0, int lane) {
+        const int k = TWO ? 2 * lane : 2 * (lane & 15), r0 = TWO ? 0 : lane >> 4;
+        const float *p = a.dy + (row0 + r0) * a.out + k;
+        const int rows = a.rows - row0 < 32 ? (int)(a.rows - row0) : 32;
+        const bool one = k < a.out, two = k + 1 < a.out;
 #pragma unroll
-        for (int r = 0; r < 32; ++r) {
-            const bool there = row0 + r < a.rows;
-            const float *p = a.dy + (row0 + r) * a.out + lane;
-            v[r][0] = there && lane < a.out ? __ldg(p) : 0.f;
-            if constexpr (TWO) v[r][1] = there && lane + 32 < a.out ? __ldg(p + 32) : 0.f;
+        for (int i = 0; i < kPasses; ++i) {
+            const bool there = r0 + i * kEach < rows;
+            v[i].x = there && one ? __ldg(p + i * kEach * a.out) : 0.f;
+            v[i].y = there && two ? __ldg(p + i * kEach * a.out + 1) : 0.f;
         }
     }
     // ... and stored as heads and tails in units of their rows, whose exponents go to `units`.
     __device__ __forceinline__ void store(uint8_t *heads, uint8_t *tails, int *units, int first, int lane) const {
-        int mine = 0;
+        const int k = TWO ? 2 * lane : 2 * (lane & 15), r0 = first + (TWO ? 0 : lane >> 4);
 #pragma unroll
-        for (int r = 0; r < 32; ++r) {
-            unsigned m = magnitude(v[r][0]);
-            if constexpr (TWO) m = max(m, magnitude(v[r][1]));
-            m = warp_max(m);
-            const int e = m == 0 ? -126 : binade(m);
-            if (lane == r) mine = e;
-            const float unit = power_of_two(-e);  // (e = 127: 2^-127 is not a normal number; zero would lose the row)
-            const float s = e == 127 ? 0.5f * power_of_two(-126) : unit;
+        for (int i0 = 0; i0 < kPasses; i0 += 8) {
+            unsigned m[8];
 #pragma unroll
-            for (int c = 0; c < (TWO ? 2 : 1); ++c) {
-                const float x = v[r][c] * s;
-                const __half h = __float2half_rn(x);
-                const int place = half_place(first + r, lane + 32 * c);
-                *reinterpret_cast<__half *>(heads + place) = h;
-                *reinterpret_cast<__half *>(tails + place) = __float2half_rn(x - __half2float(h));
+            for (int i = 0; i < 8; ++i) m[i] = max(finite_magnitude(v[i0 + i].x), finite_magnitude(v[i0 + i].y));
+            warp_max8<TWO ? 32 : 16>(m);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned field = row_unit(m[i]);
+                const float s = from_row_unit(field);
+                unsigned head, tail;
+                split_halves(v[i0 + i].x * s, v[i0 + i].y * s, head, tail);
+                const int row = r0 + (i0 + i) * kEach, place = half_place(row, k);
+                if (!TWO || lane < 24) {
+                    *reinterpret_cast<unsigned *>(heads + place) = head;
+                    *reinterpret_cast<unsigned *>(tails + place) = tail;
+                }
+                if ((lane & (TWO ? 31 : 15)) == 0) units[row] = (int)field - 127;
             }
         }
-        units[first + lane] = mine;
     }
 };
 
@@ -313,11 +337,15 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             rows.store(ops + b * 2 * kCkTile, ops + b * 2 * kCkTile + kCkTile, sh.units[t % kCkRowRing], mine, lane);
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.op_full[b]);
+            if (lane == 0) {
+                mbar_arrive(&sh.op_full[b]);
+                if (issues) ok = first(t);
+            }
+            __syncwarp();
             if (t + 1 < ntile) rows.load(a, row_of(t + 1) + mine, lane);
             if (issues) {
                 if (lane == 0) {
-                    ok = first(t) && (t == 0 || second(t - 1));
+                    ok = ok && (t == 0 || second(t - 1));
                     if (ok && t + 1 == ntile) ok = second(t);
                 }
                 ok = __shfl_sync(kFull, (int)ok, 0) != 0;
@@ -360,7 +388,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16) + kCkDzCol;
         float *stg = staged + quarter * 32 * kCkStagePitch;
         const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
-        const float u1 = power_of_two(head.w1), u2 = power_of_two(head.w2);
         const int vec = a.in % 4 == 0 && (uintptr_t)a.dz % 16 == 0 ? 4 : a.in % 2 == 0 && (uintptr_t)a.dz % 8 == 0 ? 2 : 1;
 #pragma unroll 1
         for (int t = 0; t < ntile; ++t) {
@@ -368,7 +395,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             const int nrows = a.rows - row0 < 32 ? (int)(a.rows - row0) : 32;  // may be <= 0
             if (!(ok = umma_wait(&sh.dz_full, t & 1, &sh.abort))) break;
             tc_fence_after();
-            const float unit = power_of_two(sh.units[t % kCkRowRing][quarter * 32 + lane]);
+            // the row's unit times those of the weights: one power of two unless it is out of range
+            const int e = sh.units[t % kCkRowRing][quarter * 32 + lane] + head.w1 + head.w2, e1 = max(min(e, 127), -126);
+            const float unit = power_of_two(e1), rest = power_of_two(max(e - e1, -126));
+            const bool far = __any_sync(kFull, e != e1);
 #pragma unroll 1
             for (int c0 = 0; c0 < a.in; c0 += 32) {
                 unsigned r[2][16];
@@ -384,7 +414,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
                 for (int q = 0; q < 8; ++q) {
                     float v[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[q / 4][4 * (q % 4) + j]) * u1 * u2 * unit;
+                    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[q / 4][4 * (q % 4) + j]) * unit;
+                    if (far) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] *= rest;
+                    }
                     *reinterpret_cast<float4 *>(stg + lane * kCkStagePitch + 4 * q) = make_float4(v[0], v[1], v[2], v[3]);
                 }
                 __syncwarp();
@@ -414,6 +448,8 @@ struct CkWeightsShared {
     uint64_t image, op_full, op_empty, p1_full, a_ready, p2_full;
     alignas(16) unsigned mask[4][kCkRows];
     alignas(16) int units[kCkRows];
+    alignas(16) float factor[8][64];       // of the rows of each epilogue warp, relative to the tile
+    alignas(16) uint8_t exponents[kCkRows * 6];
     float both[kCkRows];
     int z_unit;
     uint32_t tmem_base;
@@ -481,7 +517,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         const uint64_t w2h = umma_desc(smem_u32(w2)), w2l = umma_desc(smem_u32(w2 + kCkTile));
         const uint64_t zk = umma_desc(smem_u32(zt)), dyh = umma_desc(smem_u32(dyt)), dyl = umma_desc(smem_u32(dyt + kCkTile));
         const unsigned z0 = smem_u32(zt), dy0 = smem_u32(dyt);
-        auto products = [&](int t) -> bool {
+        // MMAs into one accumulator follow one another: changing it after each costs half as much again (zh W1^T and dh in turn 5,000 clocks
+        // instead of 3,400 at 163 inputs and 35 outputs).
+        auto before = [&](int t) -> bool {  // dh and zh W1^T of tile t
             if (t == 0 && !umma_wait(&sh.image, 0, &sh.abort)) return false;
             if (!umma_wait(&sh.op_full, t & 1, &sh.abort)) return false;
             tc_fence_after();
@@ -497,9 +535,12 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             for (int ks = 0; ks < ks1; ++ks) umma_f16(pre, w1h + k(ks), zk + k(ks), id, 1);
             umma_commit(&sh.p1_full);
             mbar_arrive(&sh.p1_full);
+            return true;
+        };
+        auto after = [&](int t) -> bool {  // the sums over its rows
             if (!umma_wait(&sh.a_ready, t & 1, &sh.abort)) return false;  // which also says that tile t - 1 has left its accumulators
             tc_fence_after();
-            const unsigned g1 = tmem + kCkW1Col, g2 = tmem + kCkW2Col;
+            const unsigned pre = tmem + kCkPreCol, dh = tmem + kCkDhCol, g1 = tmem + kCkW1Col, g2 = tmem + kCkW2Col;
             for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks + 8, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, ks != 0);
             for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, 1);
             for (int ks = 0; ks < 8; ++ks) {
@@ -516,8 +557,28 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         uint4 mask;
         constexpr int kUnits = 11;
         uint4 code[kUnits];
+        constexpr int kWords = 6;
+        unsigned exps[kWords];  // the whole tile's, four a word: each warp finds the largest for itself
         auto load = [&](int t) {
             const long long row0 = row_of(t) + first;
+            {
+                const long long tile0 = row_of(t);
+                const int bytes = (int)(a.rows - tile0 < kCkRows ? a.rows - tile0 : kCkRows) * groups;
+                const uint8_t *p = a.exponents + tile0 * groups;
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    const int q = 4 * (i * 32 + lane);
+                    unsigned w = 0;
+                    if (q + 4 <= bytes) {
+                        w = __ldg(reinterpret_cast<const unsigned *>(p + q));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 3; ++j)
+                            if (q + j < bytes) w |= (unsigned)__ldg(p + q + j) << (8 * j);
+                    }
+                    exps[i] = w;
+                }
+            }
             rows.load(a, row0, lane);
             mask = row0 + lane < a.rows ? __ldg(a.mask + row0 + lane) : make_uint4(0, 0, 0, 0);
 #pragma unroll
@@ -529,15 +590,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         if (ntile > 0) load(0);
 #pragma unroll 1
         for (int t = 0; t < ntile && ok; ++t) {
-            // the largest exponent of the tile, by each warp for itself
-            const long long tile0 = row_of(t);
-            const int there = a.rows - tile0 < kCkRows ? (int)(a.rows - tile0) : kCkRows;
-            int largest = 7;
-            for (int q = lane; q < there * groups; q += 32) {
-                const int e = __ldg(a.exponents + tile0 * groups + q);
-                if (e != 255) largest = max(largest, e);
-            }
-            largest = (int)warp_max((unsigned)largest);
+            unsigned most = 0x07070707u;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) most = __vmaxu4(most, exps[i] & ~__vcmpeq4(exps[i], 0xffffffffu));
+            most = __vmaxu4(most, most >> 16);
+            const int largest = (int)warp_max(max(most & 0xffu, most >> 8 & 0xffu));
             if (!(ok = umma_wait(&sh.op_empty, (t & 1) ^ 1, &sh.abort))) break;
             rows.store(dyt, dyt + kCkTile, sh.units, first, lane);
             sh.mask[0][first + lane] = mask.x;
@@ -545,11 +602,15 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             sh.mask[2][first + lane] = mask.z;
             sh.mask[3][first + lane] = mask.w;
             if (warp == kCkProducer0 && lane == 0) sh.z_unit = largest - 133 - 8;
+            // (every warp writes the same bytes, and reads its own)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) reinterpret_cast<unsigned *>(sh.exponents)[i * 32 + lane] = exps[i];
+            __syncwarp();
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
                 const int q = i * 32 + lane, row = q / units, u = q - row * units;
                 if (row >= 32) continue;
-                const int e = tile0 + first + row < a.rows ? __ldg(a.exponents + (tile0 + first + row) * groups + u / 2) : 7;
+                const int e = sh.exponents[(first + row) * groups + u / 2];
                 const int d = e - largest + 8;  // (e of a group that is not finite lies above)
                 const __half s = e == 255 ? __ushort_as_half(0x7e00) : d < -24 ? __ushort_as_half(0) : __float2half_rn(power_of_two(d));
                 uint4 lo, hi;
@@ -561,10 +622,14 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.op_full);
+            if (lane == 0) {
+                mbar_arrive(&sh.op_full);
+                if (issues) ok = before(t);
+            }
+            __syncwarp();
             if (t + 1 < ntile) load(t + 1);
             if (issues) {
-                if (lane == 0) ok = products(t);
+                if (lane == 0) ok = ok && after(t);
                 ok = __shfl_sync(kFull, (int)ok, 0) != 0;
             }
         }
@@ -593,57 +658,52 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
 #pragma unroll
             for (int q = 0; q < 4; ++q) unit = max(unit, sh.units[32 * q + lane]);
             unit = __reduce_max_sync(kFull, unit);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) sh.factor[warp][32 * q + lane] = power_of_two(sh.units[64 * half + 32 * q + lane] - unit);
+            __syncwarp();
             // units: zh 2^zu, W1 2^w1; h in units of 2^hu, which the largest sum (176 x 2 x 32512 in the accumulator's) and bias leave below 2^15
             const int zu = sh.z_unit, hu = max(zu + head.w1 + 24, head.b1 + 2) - 15;
             const float to_h = power_of_two(max(zu + head.w1 - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
-            float partial = 0.f;
+            float partial[4] = {};
+            const unsigned bit = 1u << lane;
 #pragma unroll 1
-            for (int c = 4 * half; c < 4 * half + 4; ++c) {
-                unsigned r[16], parts[16];
-                tmem_ld16(tlane + kCkDhCol + 16 * c, r);
+            for (int c = 0; c < 4; ++c) {
+                const int at = 64 * half + 16 * c;
+                unsigned rd[16], rp[16], parts[16];
+                tmem_ld16(tlane + kCkDhCol + at, rd);
+                tmem_ld16(tlane + kCkPreCol + at, rp);
                 tc_wait_ld();
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
-                    const uint4 m = *reinterpret_cast<const uint4 *>(&sh.mask[quarter][16 * c + j]);
-                    const int4 u = *reinterpret_cast<const int4 *>(&sh.units[16 * c + j]);
+                    const uint4 m = *reinterpret_cast<const uint4 *>(&sh.mask[quarter][at + j]);
+                    const float4 f = *reinterpret_cast<const float4 *>(&sh.factor[warp][16 * c + j]);
                     const unsigned mw[4] = {m.x, m.y, m.z, m.w};
-                    const int uw[4] = {u.x, u.y, u.z, u.w};
+                    const float fw[4] = {f.x, f.y, f.z, f.w};
                     float v[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        v[q] = mw[q] >> lane & 1u ? __uint_as_float(r[j + q]) * power_of_two(uw[q] - unit) : 0.f;
-                        partial += v[q];
+                        v[q] = mw[q] & bit ? __uint_as_float(rd[j + q]) * fw[q] : 0.f;
+                        rp[j + q] = __float_as_uint(mw[q] & bit ? __fmaf_rn(__uint_as_float(rp[j + q]), to_h, bias) * fw[q] : 0.f);
+                        partial[q] += v[q];
                     }
                     split_halves(v[0], v[1], parts[j / 2], parts[8 + j / 2]);
                     split_halves(v[2], v[3], parts[j / 2 + 1], parts[8 + j / 2 + 1]);
                 }
-                tmem_st16(tlane + kCkDhCol + 16 * c, parts);
-                tmem_ld16(tlane + kCkPreCol + 16 * c, r);
-                tc_wait_ld();
+                tmem_st16(tlane + kCkDhCol + at, parts);
 #pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const uint4 m = *reinterpret_cast<const uint4 *>(&sh.mask[quarter][16 * c + j]);
-                    const int4 u = *reinterpret_cast<const int4 *>(&sh.units[16 * c + j]);
-                    const unsigned mw[4] = {m.x, m.y, m.z, m.w};
-                    const int uw[4] = {u.x, u.y, u.z, u.w};
-                    float v[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        v[q] = mw[q] >> lane & 1u ? __fmaf_rn(__uint_as_float(r[j + q]), to_h, bias) * power_of_two(uw[q] - unit) : 0.f;
-                    split_halves(v[0], v[1], parts[j / 2], parts[8 + j / 2]);
-                    split_halves(v[2], v[3], parts[j / 2 + 1], parts[8 + j / 2 + 1]);
-                }
-                tmem_st16(tlane + kCkPreCol + 16 * c, parts);
+                for (int j = 0; j < 8; ++j) split_halves(__uint_as_float(rp[2 * j]), __uint_as_float(rp[2 * j + 1]), parts[j], parts[8 + j]);
+                tmem_st16(tlane + kCkPreCol + at, parts);
             }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.a_ready);
-            const float unit_dh = power_of_two(unit), unit_w2 = power_of_two(head.w2);
-            db += partial * unit_w2 * unit_dh;
+            // what the tile's sums are multiples of: products of powers of two, zero where they fall below the smallest number
+            auto scale = [](int e) { return power_of_two(max(min(e, 127), -126)) * power_of_two(max(min(e + 126, 0), -126)); };
+            db += (partial[0] + partial[1] + (partial[2] + partial[3])) * scale(unit + head.w2);
             if (!(ok = umma_wait(&sh.p2_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
             tc_fence_after();
-            const float unit_z = power_of_two(zu + 8) * 0.00390625f, unit_h = power_of_two(max(min(hu, 127), -126));
+            const float f1 = scale(unit + head.w2 + zu), f2 = scale(unit + hu);
 #pragma unroll
             for (int i = 0; i < kBlocks; ++i) {
                 const int b = 2 * i + half;
@@ -651,9 +711,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
                 unsigned r[16];
                 tmem_ld16(tlane + (b < nb1 ? kCkW1Col + 16 * b : kCkW2Col + 16 * (b - nb1)), r);
                 tc_wait_ld();
-                const float f = b < nb1 ? unit_w2 * unit_z : unit_h;
+                const float f = b < nb1 ? f1 : f2;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) sums[i][j] = __fadd_rn(sums[i][j], __uint_as_float(r[j]) * f * unit_dh);
+                for (int j = 0; j < 16; ++j) sums[i][j] = __fmaf_rn(__uint_as_float(r[j]), f, sums[i][j]);
             }
             tc_fence_before();
         }
@@ -731,7 +791,7 @@ int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, con
     if ((!dW1 || !db1 || !dW2) && (dW1 || db1 || dW2)) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: dW1, db1 and dW2 come together", me);
     if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)mask | (uintptr_t)dy) % 16)
         return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, mask, dy and scratch must be there, 16-byte aligned", me);
-    if ((uintptr_t)dz % 4) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: dz must be float aligned", me);
+    if (((uintptr_t)dz | (uintptr_t)exponents) % 4) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: dz and exponents must be 4-byte aligned", me);
     const int64_t need = npa_mlp_checkpoint_backward_scratch_bytes(rows, in_dim, out_dim);
     if (scratch_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: scratch has %lld bytes, %lld needed", me, (long long)scratch_bytes, (long long)need);
     if (!dz && !dW1) return NPA_OK;

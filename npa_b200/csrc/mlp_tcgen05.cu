@@ -420,10 +420,13 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) linear_umma_kernel(const __gr
         int k_c = 0;
         [[maybe_unused]] auto keep = [&](const float (&v)[8]) {
             const int k = k_c * kUmmaChunk + lane;
-            unsigned mine = 0;
+            unsigned mine = 0, largest[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) largest[j] = magnitude(v[j]);
+            warp_max8(largest);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const unsigned e = rows8_exponent(warp_max(magnitude(v[j])));
+                const unsigned e = rows8_exponent(largest[j]);
                 if (lane == j) mine = e;
                 if (k_row0 + j < M && k < K) args.codes[(k_row0 + j) * args.codes_pitch + k] = (int8_t)rows8_code(v[j], rows8_to_units(e));
             }

@@ -52,9 +52,13 @@ __global__ void __launch_bounds__(256) rows8_compress_lanes_kernel(const T *__re
             ++r;
         }
     }
+    unsigned largest[kRowsFlight];
+#pragma unroll
+    for (int i = 0; i < kRowsFlight; ++i) largest[i] = magnitude(v[i]);
+    warp_max8(largest);
 #pragma unroll
     for (int i = 0; i < kRowsFlight; ++i) {
-        const unsigned e = rows8_exponent(warp_max(magnitude(v[i])));
+        const unsigned e = rows8_exponent(largest[i]);
         const int k = g * kRowsGroup + lane;
         if (row < rows) {
             if (k < cols) codes[row * codes_pitch + k] = (int8_t)rows8_code(v[i], rows8_to_units(e));
