@@ -56,9 +56,16 @@ __global__ void __launch_bounds__(T > 128 ? T : 128) quantize_rows_kernel(const 
     uint8_t *out = codes + row * codes_pitch;
     const bool aligned = (reinterpret_cast<uintptr_t>(codes) | codes_pitch) % 8 == 0;
     auto put = [&](int k, const float (&w)[V]) {
-        int code[V];
+        float x[V];
+        unsigned code[V];
 #pragma unroll
-        for (int q = 0; q < V; ++q) code[q] = row_code(quantizable<UNSIGNED>(w[q]), scale, inverse);
+        for (int q = 0; q < V; ++q) x[q] = quantizable<UNSIGNED>(w[q]);
+        if (inverse == 0.f) {  // the row is not finite
+#pragma unroll
+            for (int q = 0; q < V; ++q) code[q] = 0;
+        } else {
+            row_codes<V>(x, scale, inverse, code);
+        }
         store_codes<V>(out + k, cols - k, aligned, code);
     };
 #pragma unroll
@@ -70,6 +77,45 @@ __global__ void __launch_bounds__(T > 128 ? T : 128) quantize_rows_kernel(const 
         put(k, w);
     }
     if (t == 0) scales[row] = scale;
+}
+
+// Rows of up to 32 kBlocks values whose addresses fit no vector: a warp takes eight of them, lane = column, so that its loads are lines
+// and the maxima share their shuffles.
+template <typename X, bool UNSIGNED, int kBlocks>
+__global__ void __launch_bounds__(128) quantize_lanes_kernel(const X *__restrict__ x, long long pitch, long long rows, int cols, uint8_t *__restrict__ codes,
+                                                             long long codes_pitch, float *__restrict__ scales) {
+    after_previous_kernel();
+    const int lane = threadIdx.x & 31;
+    const long long row0 = ((long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * 8;
+    if (row0 >= rows) return;
+    float v[8][kBlocks];
+    unsigned largest[8];
+    const int there = rows - row0 < 8 ? (int)(rows - row0) : 8;
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) v[r][b] = r < there && 32 * b + lane < cols ? quantizable<UNSIGNED>(as_float(x[(row0 + r) * pitch + 32 * b + lane])) : 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        largest[r] = 0;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) largest[r] = max(largest[r], magnitude(v[r][b]));
+    }
+    warp_max8(largest);
+    float mine = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        float inverse;
+        const float scale = row_scale(largest[r], UNSIGNED ? 255.f : 127.f, inverse);
+        if (lane == r) mine = scale;
+        if (r >= there) continue;
+        unsigned code[kBlocks];
+        row_codes<kBlocks>(v[r], scale, inverse, code);
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+            if (32 * b + lane < cols) codes[(row0 + r) * codes_pitch + 32 * b + lane] = inverse == 0.f ? (uint8_t)0 : (uint8_t)code[b];
+    }
+    if (lane < there) scales[row0 + lane] = mine;
 }
 
 template <typename T, typename Code>
@@ -316,9 +362,19 @@ static void launch_quantize_type(const void *x, long long pitch, long long rows,
         else if (cols <= 4096) NPA_QUANTIZE(128, 8);
         else NPA_QUANTIZE(256, 8);
     } else {
-        if (cols <= 128) NPA_QUANTIZE(32, 1);
-        else if (cols <= 512) NPA_QUANTIZE(128, 1);
-        else NPA_QUANTIZE(256, 1);
+        if (cols <= 512) {
+            void (*const kernel)(const X *, long long, long long, int, uint8_t *, long long, float *) =
+                cols <= 64 ? quantize_lanes_kernel<X, UNSIGNED, 2> : cols <= 128 ? quantize_lanes_kernel<X, UNSIGNED, 4>
+                : cols <= 192 ? quantize_lanes_kernel<X, UNSIGNED, 6> : cols <= 256 ? quantize_lanes_kernel<X, UNSIGNED, 8> : nullptr;
+            if (kernel) {
+                launch_early(kernel, (unsigned)((rows + 31) / 32), 128, 0, st, static_cast<const X *>(x), pitch, rows, cols, static_cast<uint8_t *>(codes), codes_pitch,
+                             scales);
+                return;
+            }
+            NPA_QUANTIZE(128, 1);
+        } else {
+            NPA_QUANTIZE(256, 1);
+        }
     }
 #undef NPA_QUANTIZE
 }
@@ -489,7 +545,11 @@ int npa_linear_int8(const void *x, int32_t x_type, int64_t x_pitch, const float 
 // Memory of the two layers of an MLP, each in its turn, and of what lies between them.
 struct MlpPlan {
     long long o_codes, o_scales, o_work, bytes;
+    bool fused;
     MlpPlan(const void *z, long long z_pitch, const void *w1, long long w1_pitch, const void *w2, long long w2_pitch, long long rows, int in, int hidden, int out) {
+        fused = mlp_int8_fused(static_cast<const float *>(z), z_pitch, w1, w1_pitch, w2, w2_pitch, rows, in, hidden, out);
+        bytes = 0;
+        if (fused) return;
         o_codes = round16(rows * (long long)hidden * 4);  // behind h
         o_scales = o_codes + rows * round16(hidden);
         o_work = o_scales + round16(rows * 4);
@@ -517,6 +577,11 @@ int npa_mlp_int8(const float *z, int64_t z_pitch, const void *w1, int64_t w1_pit
     if (plan.bytes && (!scratch || (uintptr_t)scratch % 16)) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: scratch must be there, 16-byte aligned", me);
     if (scratch_bytes < plan.bytes)
         return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: scratch has %lld bytes, %lld needed", me, (long long)scratch_bytes, plan.bytes);
+    if (((uintptr_t)z | (uintptr_t)y | (uintptr_t)w1_scales | (uintptr_t)b1 | (uintptr_t)w2_scales) % 4)
+        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be aligned to its type", me);
+    if (z_pitch < 0 || w1_pitch < 0 || w2_pitch < 0) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: pitches must not be negative", me);
+    if (plan.fused)
+        return launch_mlp_int8(me, z, w1, w1_pitch, w1_scales, b1, w2, w2_pitch, w2_scales, y, rows, in_dim, out_dim, (cudaStream_t)stream);
     char *p = static_cast<char *>(scratch), *codes = p + plan.o_codes, *work = p + plan.o_work;
     float *h = reinterpret_cast<float *>(p), *scales = reinterpret_cast<float *>(p + plan.o_scales);
     rc = npa_linear_int8(z, NPA_FLOAT32, z_pitch, nullptr, w1, w1_pitch, w1_scales, b1, NPA_FLOAT32, 1, h, NPA_FLOAT32, rows, in_dim, hidden, work,

@@ -56,6 +56,32 @@ __device__ __forceinline__ int row_code(float x, float scale, float inverse) {
     return (int)r;
 }
 
+// Codes of N values without the remainder: x * inverse rounded to a whole number by adding 1.5 * 2^23, whose lowest byte is the code.
+// That is within 3e-5 of the quotient (255 * 2^-23), so only a value that close to a border needs row_code: `true` where there is one.
+constexpr float kRoundWhole = 12582912.f;
+template <int N>
+__device__ __forceinline__ bool quick_codes(const float (&x)[N], float inverse, unsigned (&code)[N]) {
+    float off = 0.f;
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        const float f = __fmaf_rn(x[q], inverse, kRoundWhole);
+        code[q] = __float_as_uint(f);
+        off = fmaxf(off, fabsf(__fmaf_rn(x[q], inverse, kRoundWhole - f)));
+    }
+    return off > 0.5f - 4e-5f;
+}
+template <int N>
+__device__ __forceinline__ void row_codes(const float (&x)[N], float scale, float inverse, unsigned (&code)[N]) {
+    if (quick_codes(x, inverse, code)) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) code[q] = (unsigned)row_code(x[q], scale, inverse);
+    }
+}
+// The lowest bytes of four codes.
+__device__ __forceinline__ unsigned pack_codes(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
 template <int LANES = 32>
 __device__ __forceinline__ unsigned warp_max(unsigned v) {
 #pragma unroll
@@ -107,13 +133,14 @@ __device__ __forceinline__ void load_values(const T *__restrict__ p, int left, f
 }
 // V codes to p, of which `left` exist; `aligned`: p is a multiple of V.
 template <int V>
-__device__ __forceinline__ void store_codes(uint8_t *p, int left, bool aligned, const int (&code)[V]) {
-    if (V == 8 && left >= V && aligned) {
-        unsigned w[2] = {};
-#pragma unroll
-        for (int q = 0; q < V; ++q) w[q / 4] |= ((unsigned)code[q] & 0xffu) << (8 * (q % 4));
-        *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
-    } else {
+__device__ __forceinline__ void store_codes(uint8_t *p, int left, bool aligned, const unsigned (&code)[V]) {
+    if constexpr (V == 8) {
+        if (left >= V && aligned) {
+            *reinterpret_cast<uint2 *>(p) = make_uint2(pack_codes(code[0], code[1], code[2], code[3]), pack_codes(code[4], code[5], code[6], code[7]));
+            return;
+        }
+    }
+    {
 #pragma unroll
         for (int q = 0; q < V; ++q)
             if (q < left) p[q] = (uint8_t)code[q];
@@ -149,5 +176,11 @@ __device__ __forceinline__ float int8_value(int sum, float s, float t, bool has_
 
 // int8_tcgen05.cu: the product of codes on the tensor cores; x and w 16-byte aligned with pitches of multiples of 16, x signed.
 int launch_int8_tcgen05(const char *me, const Int8Args &a, cudaStream_t st);
+
+// int8_mlp.cu: both layers in one kernel, where the arrays lie as it wants them.
+bool mlp_int8_fused(const float *z, long long z_pitch, const void *w1, long long w1_pitch, const void *w2, long long w2_pitch, long long rows, int in, int hidden,
+                    int out);
+int launch_mlp_int8(const char *me, const float *z, const void *w1, long long w1_pitch, const float *t1, const float *b1, const void *w2, long long w2_pitch,
+                    const float *t2, float *y, long long rows, int in, int out, cudaStream_t st);
 
 }  // namespace npa

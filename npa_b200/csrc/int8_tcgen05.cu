@@ -12,21 +12,17 @@
 //     whole sectors, while the MMAs of the next tile fill the other accumulator.
 //
 // The width BN of a tile follows from the number of tiles (int8_width).  Waits are bounded as in umma.cuh.
-#include <cuda.h>
-
 #include <mutex>
 
 #include "int8.cuh"
-#include "umma.cuh"
+#include "int8_tma.cuh"
 
 namespace npa {
 
-constexpr int kI8Rows = 128, kI8Chunk = 128;  // rows of a tile, bytes of K in a stage
+constexpr int kI8Rows = 128;                  // of a tile
 constexpr int kI8WarpLoad = 0, kI8WarpMma = 1, kI8Epilogue0 = 4, kI8EpilogueWarps = 4;
 constexpr int kI8Threads = (kI8Epilogue0 + kI8EpilogueWarps) * 32;
 constexpr int kI8StagePitch = 32 * 4 + 16;    // bytes of a staged row of 32 values of up to 4 bytes: 16-byte stores of eight rows cover all banks
-
-enum { INT8_STATUS_LOAD = 128, INT8_STATUS_MMA = 256, INT8_STATUS_EPILOGUE = 512 };
 
 template <int BN>
 struct Int8Shape {
@@ -53,22 +49,6 @@ struct Int8TileArgs {
     int out_dim, chunks, tiles_m, tiles_n, band, m_inner;
     unsigned *status;
 };
-
-unsigned *umma_status_word();  // mlp_tcgen05.cu
-
-__device__ inline void umma_i8(unsigned d_tmem, uint64_t a_desc, uint64_t b_desc, unsigned idesc, int accumulate) {
-    asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// A box of a two-dimensional array into this CTA's shared memory; x in elements along the rows.
-__device__ inline void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)), "l"(map),
-                 "r"(x), "r"(y), "r"(smem_u32(bar))
-                 : "memory");
-}
 
 // Tile t as (row tile, column tile): the dimension with fewer tiles runs first, in bands of `band`, so that the tiles in flight
 // share their operands in L2.
@@ -143,8 +123,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) int8_umma_kernel(const __grid_c
         __syncwarp();
     } else if (warp == kI8WarpMma) {
         if (lane == 0) {
-            // M = 128, N = BN, signed 8-bit x signed 8-bit -> 32-bit integers, both operands K-major
-            const unsigned idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(BN >> 3) << 17) | ((unsigned)(kI8Rows >> 4) << 24);
+            const unsigned idesc = i8_idesc(BN);
             const uint64_t desc0 = umma_desc(smem_u32(base));
             int s = 0, it = 0;
             unsigned ph = 0;
@@ -274,8 +253,7 @@ static EncodeTiled encode_tiled() {
     return fn;
 }
 
-// Rows of bytes as TMA reads them: boxes of 128 bytes of `box_rows` rows, 128-byte swizzle, zeros outside.
-static int byte_rows_map(const char *me, CUtensorMap *map, const void *p, long long pitch, long long rows, int cols, int box_rows) {
+int byte_rows_map(const char *me, CUtensorMap *map, const void *p, long long pitch, long long rows, int cols, int box_rows) {
     const EncodeTiled encode = encode_tiled();
     if (!encode) return fail(NPA_ERR_CUDA, "%s: the driver has no cuTensorMapEncodeTiled", me);
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};

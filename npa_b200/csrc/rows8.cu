@@ -22,9 +22,9 @@ __global__ void __launch_bounds__(256) rows8_compress_kernel(const T *__restrict
     if (row >= rows) return;
     const unsigned e = rows8_exponent(largest);
     const float to_units = rows8_to_units(e);
-    int code[8];
+    unsigned code[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) code[q] = rows8_code(v[q], to_units);
+    for (int q = 0; q < 8; ++q) code[q] = (unsigned)rows8_code(v[q], to_units);
     if (left > 0) store_codes<8>(reinterpret_cast<uint8_t *>(codes) + row * codes_pitch + k, left, (reinterpret_cast<uintptr_t>(codes) | codes_pitch) % 8 == 0, code);
     if (part % 4 == 0) exps[row * groups + part / 4] = (uint8_t)e;
 }
