@@ -101,13 +101,12 @@ __global__ void __launch_bounds__(128) quantize_lanes_kernel(const X *__restrict
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) largest[r] = max(largest[r], magnitude(v[r][b]));
     }
-    warp_max8(largest);
-    float mine = 0.f;
+    float back;
+    const float own = row_scale(gather_max8(largest), UNSIGNED ? 255.f : 127.f, back);  // four lanes a row
+    if (lane % 4 == 0 && lane / 4 < there) scales[row0 + lane / 4] = own;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-        float inverse;
-        const float scale = row_scale(largest[r], UNSIGNED ? 255.f : 127.f, inverse);
-        if (lane == r) mine = scale;
+        const float scale = __shfl_sync(kFull, own, 4 * r), inverse = __shfl_sync(kFull, back, 4 * r);
         if (r >= there) continue;
         unsigned code[kBlocks];
         row_codes<kBlocks>(v[r], scale, inverse, code);
@@ -115,7 +114,6 @@ __global__ void __launch_bounds__(128) quantize_lanes_kernel(const X *__restrict
         for (int b = 0; b < kBlocks; ++b)
             if (32 * b + lane < cols) codes[(row0 + r) * codes_pitch + 32 * b + lane] = inverse == 0.f ? (uint8_t)0 : (uint8_t)code[b];
     }
-    if (lane < there) scales[row0 + lane] = mine;
 }
 
 template <typename T, typename Code>

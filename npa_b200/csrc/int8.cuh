@@ -56,23 +56,24 @@ __device__ __forceinline__ int row_code(float x, float scale, float inverse) {
     return (int)r;
 }
 
-// Codes of N values without the remainder: x * inverse rounded to a whole number by adding 1.5 * 2^23, whose lowest byte is the code.
-// That is within 3e-5 of the quotient (255 * 2^-23), so only a value that close to a border needs row_code: `true` where there is one.
+// Codes of N values: x * inverse rounded to a whole number by adding 1.5 * 2^23, whose lowest byte is the code.  It is within 3e-5 of the
+// quotient (255 * 2^-23), so it is the right one unless that lies so near a border; the largest remainder says whether there is such
+// a value among them, or one half way between two codes: then row_code looks at each (`true`, one value in 10^5).
 constexpr float kRoundWhole = 12582912.f;
 template <int N>
-__device__ __forceinline__ bool quick_codes(const float (&x)[N], float inverse, unsigned (&code)[N]) {
-    float off = 0.f;
+__device__ __forceinline__ bool quick_codes(const float (&x)[N], float scale, float inverse, unsigned (&code)[N]) {
+    float rest = 0.f;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
         const float f = __fmaf_rn(x[q], inverse, kRoundWhole);
         code[q] = __float_as_uint(f);
-        off = fmaxf(off, fabsf(__fmaf_rn(x[q], inverse, kRoundWhole - f)));
+        rest = fmaxf(rest, fabsf(__fmaf_rn(kRoundWhole - f, scale, x[q])));
     }
-    return off > 0.5f - 4e-5f;
+    return rest >= 0.5f * scale;
 }
 template <int N>
 __device__ __forceinline__ void row_codes(const float (&x)[N], float scale, float inverse, unsigned (&code)[N]) {
-    if (quick_codes(x, inverse, code)) {
+    if (quick_codes(x, scale, inverse, code)) {
 #pragma unroll
         for (int q = 0; q < N; ++q) code[q] = (unsigned)row_code(x[q], scale, inverse);
     }
@@ -88,25 +89,40 @@ __device__ __forceinline__ unsigned warp_max(unsigned v) {
     for (int d = 1; d < LANES; d *= 2) v = max(v, __shfl_xor_sync(kFull, v, d));
     return v;
 }
-// Eight maxima over the lanes of a group of LANES at once, each to all of its lanes: the lanes share the values out while they halve,
-// 8 or 9 shuffles for the maxima and 8 to hand them back instead of 32 or 40.
-template <int LANES = 32>
-__device__ __forceinline__ void warp_max8(unsigned (&v)[8]) {
+// The larger magnitude; NaN if either is (fmaxf would drop it).
+__device__ __forceinline__ float larger(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return max(a, b); }
+// Eight maxima over the lanes of a group of LANES at once: the lanes share the values out while they halve, 8 or 9 shuffles instead of
+// 32 or 40.  That of value r comes to lanes r LANES / 8 and up of the group.
+template <int LANES = 32, typename V>
+__device__ __forceinline__ V gather_max8(V (&v)[8]) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int n = 4, d = LANES / 2; n >= 1; n /= 2, d /= 2) {
         const bool up = lane & d;
 #pragma unroll
         for (int i = 0; i < n; ++i) {
-            const unsigned keep = up ? v[i + n] : v[i], send = up ? v[i] : v[i + n];
-            v[i] = max(keep, __shfl_xor_sync(kFull, send, d));
+            const V keep = up ? v[i + n] : v[i], send = up ? v[i] : v[i + n];
+            v[i] = larger(keep, __shfl_xor_sync(kFull, send, d));
         }
     }
-    unsigned m = v[0];
+    V m = v[0];
 #pragma unroll
-    for (int d = LANES / 16; d >= 1; d /= 2) m = max(m, __shfl_xor_sync(kFull, m, d));
+    for (int d = LANES / 16; d >= 1; d /= 2) m = larger(m, __shfl_xor_sync(kFull, m, d));
+    return m;
+}
+template <int LANES = 32>
+__device__ __forceinline__ int max8_lane(int r) { return (threadIdx.x & 31 & ~(LANES - 1)) + r * (LANES / 8); }
+// And each to all lanes of its group.
+template <int LANES = 32>
+__device__ __forceinline__ void warp_max8(unsigned (&v)[8]) {
+    const unsigned m = gather_max8<LANES>(v);
 #pragma unroll
-    for (int r = 0; r < 8; ++r) v[r] = __shfl_sync(kFull, m, (lane & ~(LANES - 1)) + r * (LANES / 8));
+    for (int r = 0; r < 8; ++r) v[r] = __shfl_sync(kFull, m, max8_lane<LANES>(r));
 }
 
 // V values at p, of which `left` exist.

@@ -51,33 +51,35 @@ struct MlpInt8Args {
 // Byte of code (row, k), k < 128, in a swizzled tile.
 __device__ __forceinline__ int code_place(int row, int k) { return row * 128 + ((((k >> 4) ^ row) & 7) << 4) + (k & 15); }
 
-// Codes of eight rows of up to 32 kBlocks columns; `get(row, column)` reads a value.
-template <int kBlocks, typename Get>
-__device__ __forceinline__ void convert_rows(Get get, uint8_t *codes, float *scales, int first, int lane) {
-    float v[8][kBlocks];
-    unsigned largest[8];
+// Codes of eight rows of `in` <= 32 kBlocks values that follow one another at p; `codes`: the first of them in a swizzled tile, `scales`
+// its scale.  A lane works out the scale of one row (four lanes the same) and hands it round.
+template <int kBlocks>
+__device__ __forceinline__ void convert_rows(const float *p, int in, uint8_t *codes, float *scales, int lane) {
+    float v[8][kBlocks], largest[8];
+    const bool last = 32 * (kBlocks - 1) + lane < in;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-        largest[r] = 0;
+        const float *row = p + r * in + lane;
+        largest[r] = 0.f;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
-            v[r][b] = get(r, 32 * b + lane);
-            largest[r] = max(largest[r], magnitude(v[r][b]));
+            v[r][b] = b + 1 < kBlocks || last ? row[32 * b] : 0.f;
+            largest[r] = larger(largest[r], fabsf(v[r][b]));
         }
     }
-    warp_max8(largest);
-    float mine = 0.f;
+    float inverse;
+    const float scale = row_scale(magnitude(gather_max8(largest)), 127.f, inverse);
+    if (lane % 4 == 0) scales[lane / 4] = scale;
+    // place of (row r, column 32 b + lane): units of 16 codes change places by the row's lowest three bits, the lane's half by the first
+    const int place[2] = {((lane >> 4) << 4) + (lane & 15), (((lane >> 4) ^ 1) << 4) + (lane & 15)};
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-        float inverse;
-        const float scale = row_scale(largest[r], 127.f, inverse);
-        if (lane == r) mine = scale;
+        const float s = __shfl_sync(kFull, scale, 4 * r), i = __shfl_sync(kFull, inverse, 4 * r);
         unsigned code[kBlocks];
-        row_codes<kBlocks>(v[r], scale, inverse, code);
+        row_codes<kBlocks>(v[r], s, i, code);
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) codes[(b / 4) * kMlpTile + code_place(first + r, 32 * (b % 4) + lane)] = (uint8_t)code[b];
+        for (int b = 0; b < kBlocks; ++b) codes[(b / 4) * kMlpTile + r * 128 + (((2 * (b % 4)) ^ (r & 6)) << 4) + place[r & 1]] = (uint8_t)code[b];
     }
-    if (lane < 8) scales[first + lane] = mine;
 }
 
 template <int kBlocks>
@@ -226,14 +228,13 @@ __global__ void __launch_bounds__(kMlpThreads, 1) mlp_int8_kernel(const __grid_c
                 if (!(ok = umma_wait(&sh.raw_full[s], (q / a.slots) & 1, &sh.abort))) break;
                 const long long row0 = row_of(t) + part * kMlpSlotRows;
                 const int first = part * kMlpSlotRows + mine;
-                if (whole(row0)) {
-                    const float *p = reinterpret_cast<const float *>(raw + s * a.slot_bytes) + mine * a.in;
-                    convert_rows<kBlocks>([&](int r, int k) { return k < a.in ? p[r * a.in + k] : 0.f; }, codes, sh.scale[t & 3], first, lane);
-                } else {
-                    const float *p = a.z + (row0 + mine) * a.in;
-                    convert_rows<kBlocks>([&](int r, int k) { return k < a.in && row0 + mine + r < a.rows ? __ldg(p + r * a.in + k) : 0.f; }, codes, sh.scale[t & 3],
-                                          first, lane);
+                float *p = reinterpret_cast<float *>(raw + s * a.slot_bytes) + mine * a.in;
+                if (!whole(row0)) {  // this warp's rows of the last slot, as far as they exist
+                    const long long from = (row0 + mine) * a.in, end = a.rows * a.in;
+                    for (int k = lane; k < 8 * a.in; k += 32) p[k] = from + k < end ? __ldg(a.z + from + k) : 0.f;
+                    __syncwarp();
                 }
+                convert_rows<kBlocks>(p, a.in, codes + first * 128, &sh.scale[t & 3][first], lane);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) {
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(kMlpThreads, 1) mlp_int8_kernel(const __grid_c
             tc_fence_after();
             const float s = sh.scale[t & 3][row];
             float v[4][16];
-            unsigned largest = 0;
+            float most = 0.f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int c0 = 64 * half + 16 * c;
@@ -301,12 +302,15 @@ __global__ void __launch_bounds__(kMlpThreads, 1) mlp_int8_kernel(const __grid_c
                     const float tw[4] = {t1.x, t1.y, t1.z, t1.w}, bw[4] = {b1.x, b1.y, b1.z, b1.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        v[c][j + i] = int8_value((int)r[j + i], s, tw[i], true, bw[i], true);
-                        largest = max(largest, magnitude(v[c][j + i]));
+                        // (sums of 256 products of 127 x 127 are below 2^22: added to 1.5 * 2^23 in its last bits, they become numbers)
+                        const float sum = __int_as_float((int)r[j + i] + __float_as_int(kRoundWhole)) - kRoundWhole;
+                        v[c][j + i] = larger(__fadd_rn(__fmul_rn(sum, __fmul_rn(s, tw[i])), bw[i]), 0.f);
+                        most = larger(most, v[c][j + i]);
                     }
                 }
             }
             tc_fence_before();
+            unsigned largest = magnitude(most);
             sh.largest[b][e][lane] = largest;
             __syncwarp();
             if (lane == 0) {
