@@ -83,10 +83,12 @@ __global__ void __launch_bounds__(512) mlp_checkpoint_image_kernel(const __grid_
     __syncthreads();
     unsigned m[3] = {};
     // every block looks at all weights: they are few, and a launch in between would cost more
+    // (loads of a fixed number, so that all are in flight at once)
     if (a.s1i == 1 && a.s1o == a.in && (uintptr_t)a.W1 % 16 == 0) {
-#pragma unroll 12
-        for (int q = threadIdx.x; q < 32 * a.in; q += 512) {
-            const float4 v = __ldg(reinterpret_cast<const float4 *>(a.W1) + q);
+#pragma unroll
+        for (int i = 0; i < 32 * kCkMaxIn / 512; ++i) {
+            const int q = threadIdx.x + 512 * i;
+            const float4 v = q < 32 * a.in ? __ldg(reinterpret_cast<const float4 *>(a.W1) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
             m[0] = max(m[0], max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w))));
         }
     } else {
@@ -96,8 +98,11 @@ __global__ void __launch_bounds__(512) mlp_checkpoint_image_kernel(const __grid_
             m[0] = max(m[0], magnitude(__ldg(a.W1 + j * a.s1o + k * a.s1i)));
         }
     }
-#pragma unroll 12
-    for (int q = threadIdx.x; q < 128 * a.out; q += 512) m[1] = max(m[1], magnitude(__ldg(a.W2 + (q >> 7) * a.s2o + (q & 127) * a.s2i)));
+#pragma unroll
+    for (int i = 0; i < 128 * kCkMaxOut / 512; ++i) {
+        const int q = threadIdx.x + 512 * i;
+        m[1] = max(m[1], q < 128 * a.out ? magnitude(__ldg(a.W2 + (q >> 7) * a.s2o + (q & 127) * a.s2i)) : 0u);
+    }
     if (threadIdx.x < 128) m[2] = magnitude(__ldg(a.b1 + threadIdx.x));
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
@@ -741,6 +746,323 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
     }
 }
 
+// ---- forward -----------------------------------------------------------------------------------------------------------
+//     y = relu(z W1^T + b1) W2^T, leaving codes and exponents of z and the bits of the ReLU
+//
+// Tiles of 128 rows again, lane = row from the first product on.  Sixteen producer warps hold eight rows each, two columns a lane: the
+// maxima of the groups give the exponents, those of the rows their units; codes leave, heads and tails go to a ring of two slots of 64
+// columns.  The products with a tail have an accumulator of their own (an addition to a sum cuts off what lies below its last bit: 11
+// additions at 163 inputs instead of 33), which four epilogue warps add; h goes back in heads and tails in place, in units that no row
+// can exceed: with z in units of its row, W1 of its matrix and the largest bias known, a bound is at hand, and 2^-25 below it is float16's
+// smallest tail.  The second layer's sums take the place of the products with tails.
+constexpr int kFwProducers = 16, kFwEpilogue0 = 16, kFwWarpMma = 20, kFwThreads = 21 * 32;
+constexpr int kFwSlot = 2 * kCkTile, kFwSlots = 2;
+struct CkForwardShared {
+    uint64_t image, slot_full[kFwSlots], slot_empty[kFwSlots], h_full[2], h_ready[2], y_full[2], y_read[2], y_written, y_copied;
+    alignas(16) float b1[128];
+    int units[4][kCkRows];
+    uint32_t tmem_base;
+    int abort;
+};
+struct CkForwardArgs {
+    const float *z, *b1;
+    const uint8_t *image;
+    float *y;
+    int8_t *codes;
+    uint8_t *exponents;
+    uint2 *mask;  // [rows][2]
+    long long rows;
+    int in, out, pitch, chunks, tiles;
+    unsigned *status;
+};
+static int ck_forward_smem(int chunks, int out) { return 1024 + (2 * chunks + 2) * kCkTile + kFwSlots * kFwSlot + kCkRows * out * 4 + 16; }
+
+template <int kChunks>
+__global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(const __grid_constant__ CkForwardArgs a) {
+    after_previous_kernel();
+    extern __shared__ uint8_t ck_raw[];
+    __shared__ CkForwardShared sh;
+    uint8_t *base = ck_raw + ((1024u - (smem_u32(ck_raw) & 1023u)) & 1023u);
+    uint8_t *w2 = base + 2 * kChunks * kCkTile, *ring = w2 + 2 * kCkTile;
+    float *ytile = reinterpret_cast<float *>(ring + kFwSlots * kFwSlot);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(&sh.image, 1);
+        for (int q = 0; q < kFwSlots; ++q) {
+            mbar_init(&sh.slot_full[q], kFwProducers);
+            mbar_init(&sh.slot_empty[q], 1);
+        }
+        for (int q = 0; q < 2; ++q) {
+            mbar_init(&sh.h_full[q], 2);  // the products, and the MMA lane itself: what it has seen of the units the epilogue sees
+            mbar_init(&sh.h_ready[q], 4);
+            mbar_init(&sh.y_full[q], 1);
+            mbar_init(&sh.y_read[q], 4);
+        }
+        mbar_init(&sh.y_written, 4);
+        mbar_init(&sh.y_copied, 4);
+        sh.abort = 0;
+        mbar_fence_init();
+    }
+    if (threadIdx.x < 128) sh.b1[threadIdx.x] = __ldg(a.b1 + threadIdx.x);
+    if (warp == kFwWarpMma) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = sh.tmem_base;  // h of two tiles at 0 and 128, what goes with tails (then y) at 256 and 384
+    const int ntile = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+    auto row_of = [&](int it) { return ((long long)blockIdx.x + (long long)it * gridDim.x) * kCkRows; };
+    bool ok = true;
+
+    if (warp == kFwWarpMma) {
+        if (lane == 0) {
+            const int tiles = 2 * kChunks + 2;
+            mbar_arrive_expect(&sh.image, (unsigned)(tiles * kCkTile));
+            for (int q = 0; q < tiles; ++q) bulk_copy_g2s(base + q * kCkTile, a.image + kCkHeader + (long long)q * kCkTile, kCkTile, &sh.image);
+            const unsigned id1 = f16_idesc(128, false), id2 = f16_idesc((a.out + 15) / 16 * 16, true);
+            const uint64_t w1h = umma_desc(smem_u32(base)), w1l = umma_desc(smem_u32(base + kChunks * kCkTile));
+            const unsigned w2h = smem_u32(w2), w2l = smem_u32(w2 + kCkTile);
+            const int steps = (a.in + 15) / 16;
+            auto second = [&](int t) -> bool {
+                const int b = t & 1;
+                if (!umma_wait(&sh.h_ready[b], (t >> 1) & 1, &sh.abort)) return false;
+                tc_fence_after();
+                const unsigned d = tmem + 256 + 128 * b, ah = tmem + 128 * b;
+                for (int ks = 0; ks < 8; ++ks) {
+                    umma_f16_ts(d, ah + 16 * ks + 8, umma_desc_rows(w2h + 2048 * ks, kCkTile), id2, ks != 0);
+                    umma_f16_ts(d, ah + 16 * ks, umma_desc_rows(w2l + 2048 * ks, kCkTile), id2, 1);
+                }
+                for (int ks = 0; ks < 8; ++ks) umma_f16_ts(d, ah + 16 * ks, umma_desc_rows(w2h + 2048 * ks, kCkTile), id2, 1);
+                umma_commit(&sh.y_full[b]);
+                return true;
+            };
+            ok = umma_wait(&sh.image, 0, &sh.abort);
+            int s = 0;
+            unsigned ph = 0;
+#pragma unroll 1
+            for (int t = 0; t < ntile && ok; ++t) {
+                const int b = t & 1;
+                if (!(ok = umma_wait(&sh.y_read[b], ((t >> 1) & 1) ^ 1, &sh.abort))) break;  // y of tile t - 2: nothing of it is left
+                tc_fence_after();
+                const unsigned d = tmem + 128 * b, small = tmem + 256 + 128 * b;
+#pragma unroll 1
+                for (int c = 0; c < kChunks; ++c) {
+                    if (!(ok = umma_wait(&sh.slot_full[s], ph, &sh.abort))) break;
+                    tc_fence_after();
+                    const uint64_t zh = umma_desc(smem_u32(ring + s * kFwSlot)), zl = umma_desc(smem_u32(ring + s * kFwSlot + kCkTile));
+                    const uint64_t wh = w1h + (uint64_t)(c * (kCkTile >> 4)), wl = w1l + (uint64_t)(c * (kCkTile >> 4));
+                    const int here = min(4, steps - 4 * c);
+                    for (int ks = 0; ks < here; ++ks) {
+                        umma_f16(small, zl + 2 * ks, wh + 2 * ks, id1, (c | ks) != 0);
+                        umma_f16(small, zh + 2 * ks, wl + 2 * ks, id1, 1);
+                    }
+                    for (int ks = 0; ks < here; ++ks) umma_f16(d, zh + 2 * ks, wh + 2 * ks, id1, (c | ks) != 0);
+                    umma_commit(&sh.slot_empty[s]);
+                    if (++s == kFwSlots) {
+                        s = 0;
+                        ph ^= 1;
+                    }
+                }
+                if (!ok) break;
+                umma_commit(&sh.h_full[b]);
+                mbar_arrive(&sh.h_full[b]);
+                if (t > 0) ok = second(t - 1);
+            }
+            if (ok && ntile > 0) ok = second(ntile - 1);
+            if (!ok) {
+                atomicOr(a.status, CK_STATUS_MMA);
+                __nanosleep(20000);  // copies in flight land before the CTA leaves
+            }
+        }
+        __syncwarp();
+    } else if (warp < kFwProducers) {
+        const int first = warp * 8, groups = (a.in + 31) / 32;
+        // place of (row r, columns 2 lane, 2 lane + 1) in a slot: units of eight columns change places by the row's lowest three bits
+        const int word = (lane & 3) * 4;
+        int s = 0;
+        unsigned ph = 1;
+#pragma unroll 1
+        for (int t = 0; t < ntile && ok; ++t) {
+            const long long row0 = row_of(t) + first;
+            float2 v[8][kChunks];
+            unsigned row_most[8];
+            {
+                const int k = 64 * (kChunks - 1) + 2 * lane;
+                const bool one = k < a.in, two = k + 1 < a.in;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    // (a row that does not exist is read as the last one: nothing of it leaves)
+                    const float *p = a.z + (row0 + r < a.rows ? row0 + r : a.rows - 1) * a.in + 2 * lane;
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c) {
+                        v[r][c].x = c + 1 < kChunks || one ? __ldg(p + 64 * c) : 0.f;
+                        v[r][c].y = c + 1 < kChunks || two ? __ldg(p + 64 * c + 1) : 0.f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 8; ++r) row_most[r] = 0;
+            unsigned own = 0;  // row `lane / 4`'s largest finite magnitude, as far as seen
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                unsigned m[8];
+                bool finite = true;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) m[r] = max(magnitude(v[r][c].x), magnitude(v[r][c].y));
+                const unsigned most = gather_max8<16>(m);  // of row (lane & 15) / 2 and the 32 columns of this half of the warp
+                finite = most < 0x7f800000u;
+                const unsigned e = rows8_exponent(most);
+                const float to_units = rows8_to_units(e);
+                const int r8 = (lane & 15) >> 1, g = 2 * c + (lane >> 4);
+                if ((lane & 1) == 0 && g < groups && row0 + r8 < a.rows) a.exponents[(row0 + r8) * groups + g] = (uint8_t)e;
+                unsigned f = finite ? most : 0u;
+                if (__any_sync(kFull, !finite)) {  // what is finite of such groups, for the unit of the row
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) m[r] = max(finite_magnitude(v[r][c].x), finite_magnitude(v[r][c].y));
+                    f = gather_max8<16>(m);
+                }
+                own = max(own, max(f, __shfl_xor_sync(kFull, f, 16)));
+                const int k = 64 * c + 2 * lane;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const float u = __shfl_sync(kFull, to_units, max8_lane<16>(r));
+                    // (at most 127.5 units but in the last binade, which ends at 128; a group that is not finite has codes of zero)
+                    const float x = fminf(fmaxf(v[r][c].x * u, -127.f), 127.f), y = fminf(fmaxf(v[r][c].y * u, -127.f), 127.f);
+                    const unsigned code = u == 0.f ? 0u : __byte_perm(__float_as_uint(x + kRoundWhole), __float_as_uint(y + kRoundWhole), 0x0040);
+                    if (row0 + r < a.rows && k < a.pitch) *reinterpret_cast<uint16_t *>(a.codes + (row0 + r) * a.pitch + k) = (uint16_t)code;
+                }
+            }
+            const unsigned field = row_unit(own);
+            if (lane < 16 && (lane & 1) == 0) sh.units[t & 3][first + (lane >> 1)] = (int)field - 127;
+            const float scale = from_row_unit(field);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const float u = __shfl_sync(kFull, scale, 2 * r);
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    unsigned head, tail;
+                    split_halves(v[r][c].x * u, v[r][c].y * u, head, tail);
+                    v[r][c] = make_float2(__uint_as_float(head), __uint_as_float(tail));
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                if (!(ok = umma_wait(&sh.slot_empty[s], ph, &sh.abort))) break;
+                uint8_t *to = ring + s * kFwSlot + first * 128 + word;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const int at = r * 128 + (((lane >> 2) ^ r) << 4);
+                    *reinterpret_cast<float *>(to + at) = v[r][c].x;
+                    *reinterpret_cast<float *>(to + kCkTile + at) = v[r][c].y;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.slot_full[s]);
+                if (++s == kFwSlots) {
+                    s = 0;
+                    ph ^= 1;
+                }
+            }
+        }
+        if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_PRODUCER);
+    } else {
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
+        const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
+        // h is below 2^(zr + w1 + 10) by its products (176 of numbers below 2 x 2) and 2^(b1 + 1) by its bias: twice 2^14 of its units
+        auto unit_of = [&](int t) { return max(sh.units[t & 3][row] + head.w1 + 10, head.b1 + 1) - 14; };
+        auto leave = [&](int t) -> bool {  // y of tile t
+            const int b = t & 1;
+            const long long row0 = row_of(t);
+            const int e = unit_of(t) + head.w2, e1 = max(min(e, 127), -126);
+            const float unit = power_of_two(e1), rest = power_of_two(max(e - e1, -126));
+            if (!umma_wait(&sh.y_copied, (t & 1) ^ 1, &sh.abort)) return false;
+            if (!umma_wait(&sh.y_full[b], (t >> 1) & 1, &sh.abort)) return false;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c0 = 0; c0 < a.out; c0 += 16) {
+                unsigned r[16];
+                tmem_ld16(tlane + 256 + 128 * b + c0, r);
+                tc_wait_ld();
+                float *to = ytile + row * a.out + c0;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (c0 + j < a.out) to[j] = __uint_as_float(r[j]) * unit * rest;
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sh.y_read[b]);
+                mbar_arrive(&sh.y_written);
+            }
+            if (!umma_wait(&sh.y_written, t & 1, &sh.abort)) return false;
+            const int here = a.rows - row0 < kCkRows ? (int)(a.rows - row0) : kCkRows, total = here * a.out;
+            float *out = a.y + row0 * a.out;  // (128 rows of any width are a multiple of 16 bytes)
+            const int quads = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 ? total / 4 : 0;
+            for (int q = row; q < quads; q += 128) reinterpret_cast<float4 *>(out)[q] = reinterpret_cast<const float4 *>(ytile)[q];
+            for (int q = 4 * quads + row; q < total; q += 128) out[q] = ytile[q];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.y_copied);
+            return true;
+        };
+#pragma unroll 1
+        for (int t = 0; t < ntile; ++t) {
+            const int b = t & 1;
+            if (!(ok = umma_wait(&sh.h_full[b], (t >> 1) & 1, &sh.abort))) break;
+            tc_fence_after();
+            const int hu = unit_of(t);
+            const float f1 = power_of_two(max(sh.units[t & 3][row] + head.w1 - hu, -126)), f2 = power_of_two(min(max(-hu, -126), 127));
+            unsigned bits[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) bits[w] = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    const int c0 = 32 * w + 16 * half;
+                    unsigned r[16], q[16], parts[16], word = 0;
+                    tmem_ld16(tlane + 128 * b + c0, r);
+                    tmem_ld16(tlane + 256 + 128 * b + c0, q);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const float4 bias = *reinterpret_cast<const float4 *>(&sh.b1[c0 + j]);
+                        const float bw[4] = {bias.x, bias.y, bias.z, bias.w};
+                        float v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            v[i] = fmaxf(__fmaf_rn(__uint_as_float(r[j + i]) + __uint_as_float(q[j + i]), f1, bw[i] * f2), 0.f);
+                            word |= v[i] > 0.f ? 1u << (j + i) : 0u;
+                        }
+                        split_halves(v[0], v[1], parts[j / 2], parts[8 + j / 2]);
+                        split_halves(v[2], v[3], parts[j / 2 + 1], parts[8 + j / 2 + 1]);
+                    }
+                    bits[w] |= word << (16 * half);
+                    tmem_st16(tlane + 128 * b + c0, parts);
+                }
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.h_ready[b]);
+            const long long at = row_of(t) + row;
+            if (at < a.rows) reinterpret_cast<uint4 *>(a.mask)[at] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+            if (t > 0 && !(ok = leave(t - 1))) break;
+        }
+        if (ok && ntile > 0) ok = leave(ntile - 1);
+        if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_EPILOGUE);
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kFwWarpMma) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------
 static int64_t ck_image_bytes(int in_dim) { return kCkHeader + (int64_t)(2 * ((in_dim + 63) / 64) + 2) * kCkTile; }
 static GradReduce ck_reduce(int64_t rows, int in_dim, int out_dim) {
@@ -774,6 +1096,39 @@ int check_mlp8(const char *me, int64_t rows, int32_t in_dim, int32_t out_dim) {
 using namespace npa;
 
 extern "C" {
+
+int64_t npa_mlp_checkpoint_forward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim) {
+    return rows <= 0 || in_dim <= 0 || out_dim <= 0 ? 0 : ck_image_bytes(in_dim);
+}
+
+int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1, const float *W2, float *y, int64_t rows, int32_t in_dim, int32_t out_dim,
+                               int64_t w1_stride_out, int64_t w1_stride_in, int64_t w2_stride_out, int64_t w2_stride_in, void *codes, uint8_t *exponents,
+                               uint32_t *mask, void *scratch, int64_t scratch_bytes, void *stream) {
+    const char *me = "npa_mlp_checkpoint_forward";
+    int rc = check_mlp8(me, rows, in_dim, out_dim);
+    if (rc != NPA_OK) return rc;
+    if (!z || !W1 || !b1 || !W2 || !y || !codes || !exponents || !mask) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be non-NULL", me);
+    if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)mask) % 16)
+        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, mask and scratch must be there, 16-byte aligned", me);
+    if (((uintptr_t)z | (uintptr_t)W1 | (uintptr_t)b1 | (uintptr_t)W2 | (uintptr_t)y) % 4) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be float aligned", me);
+    const int64_t need = npa_mlp_checkpoint_forward_scratch_bytes(rows, in_dim, out_dim);
+    if (scratch_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: scratch has %lld bytes, %lld needed", me, (long long)scratch_bytes, (long long)need);
+    CkForwardArgs a = {};
+    a.z = z; a.b1 = b1; a.image = static_cast<const uint8_t *>(scratch); a.y = y; a.codes = static_cast<int8_t *>(codes); a.exponents = exponents;
+    a.mask = reinterpret_cast<uint2 *>(mask); a.rows = rows; a.in = in_dim; a.out = out_dim; a.pitch = (int)rows8_pitch(in_dim);
+    a.chunks = (in_dim + 63) / 64; a.tiles = (int)((rows + kCkRows - 1) / kCkRows);
+    if (!(a.status = umma_status_word())) return fail(NPA_ERR_CUDA, "%s: no status word", me);
+    const cudaStream_t st = (cudaStream_t)stream;
+    const CkImageArgs image{W1, b1, W2, w1_stride_out, w1_stride_in, w2_stride_out, w2_stride_in, in_dim, out_dim, a.chunks, static_cast<uint8_t *>(scratch)};
+    launch_early(mlp_checkpoint_image_kernel, 8 * (a.chunks + 1), 512, 0, st, image);
+    if ((rc = check_launch("mlp_checkpoint_image_kernel")) != NPA_OK) return rc;
+    const auto kernel = a.chunks == 1 ? mlp_checkpoint_forward_kernel<1> : a.chunks == 2 ? mlp_checkpoint_forward_kernel<2> : mlp_checkpoint_forward_kernel<3>;
+    const int smem = ck_forward_smem(a.chunks, out_dim);
+    int unused = 0;  // raises the kernel's limit of shared memory on this device
+    if ((rc = persistent_ctas(kernel, kFwThreads, (size_t)smem, &unused)) != NPA_OK) return rc;
+    launch_early(kernel, a.tiles < 148 ? a.tiles : 148, kFwThreads, (size_t)smem, st, a);
+    return check_launch("mlp_checkpoint_forward_kernel");
+}
 
 int64_t npa_mlp_checkpoint_backward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim) {
     if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return 0;

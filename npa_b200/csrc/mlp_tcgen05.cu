@@ -38,7 +38,6 @@
 #include <mutex>
 
 #include "perceive_backward.cuh"
-#include "rows8.cuh"
 #include "step_update.cuh"
 #include "umma.cuh"
 #include "weight_image.cuh"
@@ -99,11 +98,6 @@ struct UmmaArgs {
     StepArgs step;
     Geom g;
     StepRows parts;  // kUmmaParts: where the rows go instead of C
-    // kUmmaKept: the rows of A in 8 bits and the bits of the activated first layer, for a backward pass
-    int8_t *codes;
-    uint8_t *exponents;
-    uint16_t *mask;  // [M, 8]
-    int codes_pitch;
 };
 constexpr int kUmmaStepQuads = 4;  // float4 of the states per epilogue thread and tile: up to 32 features
 
@@ -114,7 +108,7 @@ __global__ void weight_image_kernel(const __grid_constant__ ImageJobs jobs) {
     write_image_element(jobs, blockIdx.x * blockDim.x + threadIdx.x);
 }
 
-enum : int { kUmmaOneLayer = 0, kUmmaTwoLayers = 1, kUmmaStep = 2, kUmmaParts2 = 3, kUmmaParts3 = 4, kUmmaKept = 5, kUmmaModes = 6 };
+enum : int { kUmmaOneLayer = 0, kUmmaTwoLayers = 1, kUmmaStep = 2, kUmmaParts2 = 3, kUmmaParts3 = 4, kUmmaModes = 5 };
 constexpr int kUmmaPartPitch = 12;  // floats per staged row of 8 features: float4 writes of eight lanes cover all banks
 __host__ __device__ constexpr int umma_epilogue_floats(int mode) {
     return mode == kUmmaParts2 || mode == kUmmaParts3 ? kUmmaEpilogueWarps * 32 * kUmmaPartPitch * (mode == kUmmaParts2 ? 4 : 5) : kUmmaEpiFloats;
@@ -252,7 +246,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) linear_umma_kernel(const __gr
     const int K = args.K, N = args.N, Np = args.Np, nchunks = args.nchunks, last_ksteps = args.last_ksteps;
     const int stages = args.stages, stage_bytes = args.stage_bytes;
     const bool relu = args.relu != 0;
-    constexpr bool fuse = MODE == kUmmaTwoLayers || MODE == kUmmaStep || MODE == kUmmaKept;  // two-layer mode
+    constexpr bool fuse = MODE == kUmmaTwoLayers || MODE == kUmmaStep;  // two-layer mode
     constexpr int kParts = MODE == kUmmaParts2 ? 2 : MODE == kUmmaParts3 ? 3 : 0;
     const int N2 = args.N2, N2p = args.N2p;
     const int acc_stride = fuse ? 128 : kUmmaAccStride;
@@ -415,27 +409,6 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) linear_umma_kernel(const __gr
                 l_row0 += (long long)gridDim.x * kUmmaRows;
             }
         };
-        // a chunk is a group of 8-bit rows: eight rows of it, lane = column
-        long long k_row0 = (long long)blockIdx.x * kUmmaRows + pw * 8;
-        int k_c = 0;
-        [[maybe_unused]] auto keep = [&](const float (&v)[8]) {
-            const int k = k_c * kUmmaChunk + lane;
-            unsigned mine = 0, largest[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) largest[j] = magnitude(v[j]);
-            warp_max8(largest);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const unsigned e = rows8_exponent(largest[j]);
-                if (lane == j) mine = e;
-                if (k_row0 + j < M && k < K) args.codes[(k_row0 + j) * args.codes_pitch + k] = (int8_t)rows8_code(v[j], rows8_to_units(e));
-            }
-            if (lane < 8 && k_row0 + lane < M) args.exponents[(k_row0 + lane) * nchunks + k_c] = (uint8_t)mine;
-            if (++k_c == nchunks) {
-                k_c = 0;
-                k_row0 += (long long)gridDim.x * kUmmaRows;
-            }
-        };
         int s = 0;
         unsigned ph = 1;
         auto store = [&](const float (&v)[8]) -> bool {
@@ -446,9 +419,8 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) linear_umma_kernel(const __gr
                 const int at = umma_swizzled(pw * 8 + j, lane);
                 const float head = __uint_as_float(tf32_head_bits(v[j]));
                 hi[at] = head;
-                lo[at] = MODE == kUmmaKept ? tf32_nearest(v[j] - head) : v[j] - head;
+                lo[at] = v[j] - head;
             }
-            if constexpr (MODE == kUmmaKept) keep(v);
             fence_proxy_async();  // the MMA reads these through the async proxy
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh->full[s]);
@@ -571,14 +543,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) linear_umma_kernel(const __gr
                             float v = __uint_as_float(r[j]) + bj[j];
                             if (relu) v = fmaxf(v, 0.f);
                             r[j] = __float_as_uint(v);
-                            const float rest = v - __uint_as_float(tf32_head_bits(v));
-                            tail[j] = __float_as_uint(MODE == kUmmaKept ? tf32_nearest(rest) : rest);
-                        }
-                        if constexpr (MODE == kUmmaKept) {
-                            unsigned bits = 0;
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) bits |= (__uint_as_float(r[j]) > 0.f ? 1u : 0u) << j;
-                            if (lane < nrows) args.mask[(row0 + lane) * 8 + b] = (uint16_t)bits;
+                            tail[j] = __float_as_uint(v - __uint_as_float(tf32_head_bits(v)));
                         }
                         tmem_st16(taddr0 + c0, r);                 // the MMA reads the head of these by truncation
                         tmem_st16(tlane + kUmmaHloCol + c0, tail);
@@ -728,7 +693,6 @@ static void (*umma_kernel(int mode))(UmmaArgs) {
         case kUmmaTwoLayers: return linear_umma_kernel<kUmmaTwoLayers>;
         case kUmmaParts2: return linear_umma_kernel<kUmmaParts2>;
         case kUmmaParts3: return linear_umma_kernel<kUmmaParts3>;
-        case kUmmaKept: return linear_umma_kernel<kUmmaKept>;
         default: return linear_umma_kernel<kUmmaOneLayer>;
     }
 }
@@ -771,7 +735,7 @@ static int umma_round16(int v) { return (v + 15) / 16 * 16; }
 static int umma_chunks(int k) { return (k + kUmmaChunk - 1) / kUmmaChunk; }
 
 static ImageJob image_job(const float *W, int64_t stride_out, int64_t stride_in, int in_dim, int out_dim, void *img) {
-    return ImageJob{W, stride_out, stride_in, in_dim, out_dim, umma_round16(out_dim), umma_chunks(in_dim), static_cast<float *>(img), 0, 0, 0};
+    return ImageJob{W, stride_out, stride_in, in_dim, out_dim, umma_round16(out_dim), umma_chunks(in_dim), static_cast<float *>(img)};
 }
 static int launch_images(const ImageJobs &jobs, cudaStream_t st) {
     launch_early(weight_image_kernel, (jobs.total() + 255) / 256, 256, 0, st, jobs);
@@ -965,16 +929,9 @@ int npa_bin_particles_step_images(const npa_grid *grid, int32_t channels, const 
     return bin_particles_and_images(grid, channels, x, s, permutation, x_out, s_out, jobs, (cudaStream_t)stream);
 }
 
-// What a forward pass leaves for a backward one that makes the hidden layer again.
-struct Kept {
-    int8_t *codes;
-    uint8_t *exponents;
-    uint16_t *mask;
-};
-
 // step != NULL: with the Euler update of D-dimensional positions on the geometry g.
 static int mlp_forward(const char *me, const float *z, const float *b1, float *h, float *y, int64_t rows, int32_t in_dim, int32_t out_dim,
-                       const void *scratch, int64_t scratch_bytes, const StepArgs *step, const Geom *g, cudaStream_t st, const Kept *kept = nullptr) {
+                       const void *scratch, int64_t scratch_bytes, const StepArgs *step, const Geom *g, cudaStream_t st) {
     if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: rows, in_dim and out_dim must be positive", me);
     if (in_dim > 1024 || out_dim > 64)
         return fail(NPA_ERR_UNSUPPORTED, "%s: supports in_dim <= 1024 and out_dim <= 64 (hidden width 128), got %d and %d", me, in_dim, out_dim);
@@ -999,10 +956,7 @@ static int mlp_forward(const char *me, const float *z, const float *b1, float *h
     if (a.stages > kUmmaMaxStages) a.stages = kUmmaMaxStages;
     if (a.stages < 2) return fail(NPA_ERR_UNSUPPORTED, "%s: no room for two stages", me);
     const size_t smem = (size_t)fixed + (size_t)a.stages * a.stage_bytes;
-    const int mode = step ? kUmmaStep : kept ? kUmmaKept : kUmmaTwoLayers;
-    if (kept) {
-        a.codes = kept->codes; a.exponents = kept->exponents; a.mask = kept->mask; a.codes_pitch = (int)rows8_pitch(in_dim);
-    }
+    const int mode = step ? kUmmaStep : kUmmaTwoLayers;
     if (step) {
         a.D = g->dim;
         a.step = *step;
@@ -1014,30 +968,6 @@ static int mlp_forward(const char *me, const float *z, const float *b1, float *h
     const int ctas = (int)(tiles < 148 ? tiles : 148);
     launch_early(umma_kernel(mode), ctas, kUmmaThreads, smem, st, a);
     return check_launch("linear_umma_kernel (two layers)");
-}
-
-int64_t npa_mlp_checkpoint_forward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim) {
-    return rows <= 0 ? 0 : npa_mlp_forward_tcgen05_scratch_bytes(in_dim, out_dim);
-}
-
-int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1, const float *W2, float *y, int64_t rows, int32_t in_dim, int32_t out_dim,
-                               int64_t w1_stride_out, int64_t w1_stride_in, int64_t w2_stride_out, int64_t w2_stride_in, void *codes, uint8_t *exponents,
-                               uint32_t *mask, void *scratch, int64_t scratch_bytes, void *stream) {
-    const char *me = "npa_mlp_checkpoint_forward";
-    int rc = check_mlp8(me, rows, in_dim, out_dim);
-    if (rc != NPA_OK) return rc;
-    if (!z || !W1 || !b1 || !W2 || !y || !codes || !exponents || !mask) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be non-NULL", me);
-    if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)mask) % 16)
-        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, mask and scratch must be there, 16-byte aligned", me);
-    const int64_t need = npa_mlp_checkpoint_forward_scratch_bytes(rows, in_dim, out_dim);
-    if (scratch_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: scratch has %lld bytes, %lld needed", me, (long long)scratch_bytes, (long long)need);
-    ImageJobs jobs;
-    rc = mlp_images(me, W1, W2, in_dim, out_dim, w1_stride_out, w1_stride_in, w2_stride_out, w2_stride_in, scratch, scratch_bytes, nullptr, 0, &jobs);
-    if (rc != NPA_OK) return rc;
-    for (int q = 0; q < jobs.count; ++q) jobs.job[q].nearest = 1;
-    if ((rc = launch_images(jobs, (cudaStream_t)stream)) != NPA_OK) return rc;
-    const Kept kept{static_cast<int8_t *>(codes), exponents, reinterpret_cast<uint16_t *>(mask)};
-    return mlp_forward(me, z, b1, nullptr, y, rows, in_dim, out_dim, scratch, scratch_bytes, nullptr, nullptr, (cudaStream_t)stream, &kept);
 }
 
 int npa_mlp_forward_tcgen05_prepared(const float *z, const float *b1, float *h, float *y, int64_t rows, int32_t in_dim, int32_t out_dim,

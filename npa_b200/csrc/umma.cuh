@@ -104,14 +104,6 @@ __host__ __device__ inline int umma_swizzled(int row, int k) { return row * 32 +
 
 __device__ inline unsigned tf32_head_bits(float x) { return __float_as_uint(x) & 0xffffe000u; }
 
-// Rounded to TF32.  A tail that the MMA cuts off instead is too small by 2^-23 of its number in the mean, always in the same direction:
-// the products of two layers come out 1e-6 too small.
-__device__ inline float tf32_nearest(float x) {
-    unsigned r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return __uint_as_float(r);
-}
-
 // Shared-memory operand descriptor of an MN-major TF32 tile.  32-bit operands that are contiguous along
 // M / N have one layout: the 128-byte swizzle on 32-byte units.  An atom is 4 k-rows x 128 bytes (32
 // floats of the M or N index, contiguous); inside it the 32-byte unit index is XORed with the k-row

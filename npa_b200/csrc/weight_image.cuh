@@ -17,7 +17,6 @@ struct ImageJob {
     int K, N, Np, nchunks;
     float *img;
     int features, dim;  // > 0: rows n in the order of StepColumns (below)
-    int nearest;        // tails rounded to TF32; otherwise the MMA cuts them off as it reads them
     __host__ __device__ int total() const { return nchunks * Np * kImageChunk; }
 };
 // The columns of z in the order in which the gradient of a step wants them: the features themselves, their blur, then axis by axis the
@@ -57,7 +56,7 @@ __device__ inline void write_image_element(const ImageJobs &jobs, int at) {
             float *chunk = j.img + (size_t)c * 2 * Np * kImageChunk;
             const int to = umma_swizzled(n, kk);
             chunk[to] = head;
-            chunk[Np * kImageChunk + to] = j.nearest ? tf32_nearest(v - head) : v - head;
+            chunk[Np * kImageChunk + to] = v - head;
             return;
         }
         at -= total;
