@@ -676,8 +676,8 @@ int npa_rows8_restore(const void *codes, int64_t codes_pitch, const uint8_t *exp
 
 /* The adaptation MLP (hidden width 128, in <= 176, out <= 48) whose backward reads z in 8 bits.  The forward leaves
  * codes [rows, in rounded up to 16], exponents, and mask [rows, 4] with the bits of h > 0 (unit 32 w + i is bit i of word
- * w); the backward makes the hidden layer again from them.  dz may be NULL, and dW1, db1 and dW2 together.  codes, mask,
- * dy and scratch 16-byte aligned; waits are bounded as in npa_linear_tcgen05, whose status has bits 1024, 2048, 4096 for
+ * w); the backward makes the hidden layer again from them.  dz may be NULL, and dW1, db1 and dW2 together.  codes, exponents,
+ * mask, dy and scratch 16-byte aligned; waits are bounded as in npa_linear_tcgen05, whose status has bits 1024, 2048, 4096 for
  * the MMA lane, producers and epilogue of the backward. */
 int64_t npa_mlp_checkpoint_forward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim);
 int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1, const float *W2, float *y, int64_t rows,

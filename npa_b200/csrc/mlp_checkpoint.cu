@@ -904,19 +904,22 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
             }
 #pragma unroll
             for (int r = 0; r < 8; ++r) row_most[r] = 0;
-            unsigned own = 0;  // row `lane / 4`'s largest finite magnitude, as far as seen
+            // codes are put together in this warp's rows of the slot that the first chunk is going to: five rows where its heads will be,
+            // three where its tails (in two bytes a lane they would go to memory in pieces of sectors, which cost 13,000 clocks a tile)
+            if (!(ok = umma_wait(&sh.slot_empty[s], ph, &sh.abort))) break;
+            uint8_t *const low = ring + s * kFwSlot + first * 128, *const high = low + kCkTile;
+            unsigned own = 0;  // the largest finite magnitude of row (lane & 15) / 2, as far as seen
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
                 unsigned m[8];
-                bool finite = true;
 #pragma unroll
                 for (int r = 0; r < 8; ++r) m[r] = max(magnitude(v[r][c].x), magnitude(v[r][c].y));
                 const unsigned most = gather_max8<16>(m);  // of row (lane & 15) / 2 and the 32 columns of this half of the warp
-                finite = most < 0x7f800000u;
+                const bool finite = most < 0x7f800000u;
                 const unsigned e = rows8_exponent(most);
                 const float to_units = rows8_to_units(e);
                 const int r8 = (lane & 15) >> 1, g = 2 * c + (lane >> 4);
-                if ((lane & 1) == 0 && g < groups && row0 + r8 < a.rows) a.exponents[(row0 + r8) * groups + g] = (uint8_t)e;
+                if ((lane & 1) == 0 && g < groups) high[768 + r8 * groups + g] = (uint8_t)e;
                 unsigned f = finite ? most : 0u;
                 if (__any_sync(kFull, !finite)) {  // what is finite of such groups, for the unit of the row
 #pragma unroll
@@ -931,9 +934,23 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                     // (at most 127.5 units but in the last binade, which ends at 128; a group that is not finite has codes of zero)
                     const float x = fminf(fmaxf(v[r][c].x * u, -127.f), 127.f), y = fminf(fmaxf(v[r][c].y * u, -127.f), 127.f);
                     const unsigned code = u == 0.f ? 0u : __byte_perm(__float_as_uint(x + kRoundWhole), __float_as_uint(y + kRoundWhole), 0x0040);
-                    if (row0 + r < a.rows && k < a.pitch) *reinterpret_cast<uint16_t *>(a.codes + (row0 + r) * a.pitch + k) = (uint16_t)code;
+                    if (k < a.pitch) *reinterpret_cast<uint16_t *>((r < 5 ? low + r * a.pitch : high + (r - 5) * a.pitch) + k) = (uint16_t)code;
                 }
             }
+            __syncwarp();
+            {
+                const int in_low = 5 * a.pitch / 16, total = 8 * a.pitch / 16;
+                const long long left = (a.rows - row0) * a.pitch / 16;  // (may be <= 0)
+                for (int q = lane; q < total && q < left; q += 32)
+                    reinterpret_cast<uint4 *>(a.codes + row0 * a.pitch)[q] = *reinterpret_cast<const uint4 *>(q < in_low ? low + 16 * q : high + 16 * (q - in_low));
+                if (row0 + 8 <= a.rows) {
+                    if (lane < groups) reinterpret_cast<uint2 *>(a.exponents + row0 * groups)[lane] = *reinterpret_cast<const uint2 *>(high + 768 + 8 * lane);
+                } else {
+                    for (int q = lane; q < 8 * groups; q += 32)
+                        if (row0 + q / groups < a.rows) a.exponents[row0 * groups + q] = high[768 + q];
+                }
+            }
+            __syncwarp();
             const unsigned field = row_unit(own);
             if (lane < 16 && (lane & 1) == 0) sh.units[t & 3][first + (lane >> 1)] = (int)field - 127;
             const float scale = from_row_unit(field);
@@ -949,7 +966,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
             }
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
-                if (!(ok = umma_wait(&sh.slot_empty[s], ph, &sh.abort))) break;
+                if (c > 0 && !(ok = umma_wait(&sh.slot_empty[s], ph, &sh.abort))) break;
                 uint8_t *to = ring + s * kFwSlot + first * 128 + word;
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
@@ -1108,8 +1125,8 @@ int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1,
     int rc = check_mlp8(me, rows, in_dim, out_dim);
     if (rc != NPA_OK) return rc;
     if (!z || !W1 || !b1 || !W2 || !y || !codes || !exponents || !mask) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be non-NULL", me);
-    if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)mask) % 16)
-        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, mask and scratch must be there, 16-byte aligned", me);
+    if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)mask | (uintptr_t)exponents) % 16)
+        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, exponents, mask and scratch must be there, 16-byte aligned", me);
     if (((uintptr_t)z | (uintptr_t)W1 | (uintptr_t)b1 | (uintptr_t)W2 | (uintptr_t)y) % 4) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be float aligned", me);
     const int64_t need = npa_mlp_checkpoint_forward_scratch_bytes(rows, in_dim, out_dim);
     if (scratch_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: scratch has %lld bytes, %lld needed", me, (long long)scratch_bytes, (long long)need);
