@@ -675,20 +675,20 @@ int npa_rows8_restore(const void *codes, int64_t codes_pitch, const uint8_t *exp
                       void *out, int32_t type, void *stream);
 
 /* The adaptation MLP (hidden width 128, in <= 176, out <= 48) whose backward reads z in 8 bits.  The forward leaves
- * codes [rows, in rounded up to 16], exponents, and mask [rows, 4] with the bits of h > 0 (unit 32 w + i is bit i of word
- * w); the backward makes the hidden layer again from them.  dz may be NULL, and dW1, db1 and dW2 together.  codes, exponents,
- * mask, dy and scratch 16-byte aligned; waits are bounded as in npa_linear_tcgen05, whose status has bits 1024, 2048, 4096 for
- * the MMA lane, producers and epilogue of the backward. */
-int64_t npa_mlp_checkpoint_forward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim);
+ * codes [rows, in rounded up to 16], exponents, mask [rows, 4] with the bits of h > 0 (unit 32 w + i is bit i of word w),
+ * and an image of the weights (npa_mlp_checkpoint_image_bytes() bytes) as the tensor cores read them, which is the
+ * backward's as well; the backward makes the hidden layer again.  dz may be NULL, and dW1, db1 and dW2 together.  codes,
+ * exponents, mask, image, dy and scratch 16-byte aligned; waits are bounded as in npa_linear_tcgen05, whose status has
+ * bits 1024, 2048, 4096 for the MMA lane, producers and epilogue of these kernels. */
+int64_t npa_mlp_checkpoint_image_bytes(int32_t in_dim);
 int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1, const float *W2, float *y, int64_t rows,
                                int32_t in_dim, int32_t out_dim, int64_t w1_stride_out, int64_t w1_stride_in,
                                int64_t w2_stride_out, int64_t w2_stride_in, void *codes, uint8_t *exponents, uint32_t *mask,
-                               void *scratch, int64_t scratch_bytes, void *stream);
+                               void *image, int64_t image_bytes, void *stream);
 int64_t npa_mlp_checkpoint_backward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim);
-int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, const uint32_t *mask, const float *W1,
-                                const float *b1, const float *W2, const float *dy, float *dz, float *dW1, float *db1,
-                                float *dW2, int64_t rows, int32_t in_dim, int32_t out_dim, int64_t w1_stride_out,
-                                int64_t w1_stride_in, int64_t w2_stride_out, int64_t w2_stride_in, void *scratch,
+int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, const uint32_t *mask, const void *image,
+                                int64_t image_bytes, const float *b1, const float *dy, float *dz, float *dW1, float *db1,
+                                float *dW2, int64_t rows, int32_t in_dim, int32_t out_dim, void *scratch,
                                 int64_t scratch_bytes, void *stream);
 
 /* Self-test of those bounded waits: a two-warp kernel in which warp 0 waits `limit_us` (1..1,000,000)

@@ -136,10 +136,10 @@ SIGNATURES = {
     "npa_mlp_int8": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _P, _I64, _I32, _I32, _I32, _P, _I64, _P]),
     "npa_rows8_compress": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _P, _I64, _P, _P]),
     "npa_rows8_restore": (ctypes.c_int, [_P, _I64, _P, _I64, _I32, _P, _I32, _P]),
-    "npa_mlp_checkpoint_forward_scratch_bytes": (_I64, [_I64, _I32, _I32]),
+    "npa_mlp_checkpoint_image_bytes": (_I64, [_I32]),
     "npa_mlp_checkpoint_forward": (ctypes.c_int, [_P] * 5 + [_I64, _I32, _I32] + [_I64] * 4 + [_P] * 4 + [_I64, _P]),
     "npa_mlp_checkpoint_backward_scratch_bytes": (_I64, [_I64, _I32, _I32]),
-    "npa_mlp_checkpoint_backward": (ctypes.c_int, [_P] * 11 + [_I64, _I32, _I32] + [_I64] * 4 + [_P, _I64, _P]),
+    "npa_mlp_checkpoint_backward": (ctypes.c_int, [_P] * 4 + [_I64] + [_P] * 6 + [_I64, _I32, _I32, _P, _I64, _P]),
     "npa_linear_tcgen05_status": (ctypes.c_int, [_P, _I32]),
     "npa_linear_tcgen05_wait_selftest": (ctypes.c_int, [_I32, _P, _P]),
     "npa_step_update_backward": (ctypes.c_int, [_P] * 3 + [_I32, ctypes.c_float, ctypes.c_float, _P, _P, _P, _P]),

@@ -25,6 +25,7 @@
 //
 // Waits are bounded as in umma.cuh; they report through npa_linear_tcgen05_status (bits 1024, 2048, 4096: MMA lane, producers, epilogue).
 #include <mutex>
+#include <type_traits>
 
 #include "mlp_grad_reduce.cuh"
 #include "rows8.cuh"
@@ -928,14 +929,20 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                 }
                 own = max(own, max(f, __shfl_xor_sync(kFull, f, 16)));
                 const int k = 64 * c + 2 * lane;
+                auto put = [&](auto clamp) {
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const float u = __shfl_sync(kFull, to_units, max8_lane<16>(r));
-                    // (at most 127.5 units but in the last binade, which ends at 128; a group that is not finite has codes of zero)
-                    const float x = fminf(fmaxf(v[r][c].x * u, -127.f), 127.f), y = fminf(fmaxf(v[r][c].y * u, -127.f), 127.f);
-                    const unsigned code = u == 0.f ? 0u : __byte_perm(__float_as_uint(x + kRoundWhole), __float_as_uint(y + kRoundWhole), 0x0040);
-                    if (k < a.pitch) *reinterpret_cast<uint16_t *>((r < 5 ? low + r * a.pitch : high + (r - 5) * a.pitch) + k) = (uint16_t)code;
-                }
+                    for (int r = 0; r < 8; ++r) {
+                        const float u = __shfl_sync(kFull, to_units, max8_lane<16>(r));
+                        unsigned x = __float_as_uint(__fmaf_rn(v[r][c].x, u, kRoundWhole)), y = __float_as_uint(__fmaf_rn(v[r][c].y, u, kRoundWhole));
+                        if constexpr (decltype(clamp)::value) {
+                            x = (unsigned)rows8_code(v[r][c].x, u);
+                            y = (unsigned)rows8_code(v[r][c].y, u);
+                        }
+                        if (k < a.pitch) *reinterpret_cast<uint16_t *>((r < 5 ? low + r * a.pitch : high + (r - 5) * a.pitch) + k) = (uint16_t)__byte_perm(x, y, 0x0040);
+                    }
+                };
+                if (__any_sync(kFull, e >= 254u)) put(std::true_type());  // up to 128 units in the last binade, or groups that are not finite
+                else put(std::false_type());
             }
             __syncwarp();
             {
@@ -1114,30 +1121,28 @@ using namespace npa;
 
 extern "C" {
 
-int64_t npa_mlp_checkpoint_forward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim) {
-    return rows <= 0 || in_dim <= 0 || out_dim <= 0 ? 0 : ck_image_bytes(in_dim);
-}
+int64_t npa_mlp_checkpoint_image_bytes(int32_t in_dim) { return in_dim <= 0 ? 0 : ck_image_bytes(in_dim); }
 
 int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1, const float *W2, float *y, int64_t rows, int32_t in_dim, int32_t out_dim,
                                int64_t w1_stride_out, int64_t w1_stride_in, int64_t w2_stride_out, int64_t w2_stride_in, void *codes, uint8_t *exponents,
-                               uint32_t *mask, void *scratch, int64_t scratch_bytes, void *stream) {
+                               uint32_t *mask, void *image, int64_t image_bytes, void *stream) {
     const char *me = "npa_mlp_checkpoint_forward";
     int rc = check_mlp8(me, rows, in_dim, out_dim);
     if (rc != NPA_OK) return rc;
     if (!z || !W1 || !b1 || !W2 || !y || !codes || !exponents || !mask) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be non-NULL", me);
-    if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)mask | (uintptr_t)exponents) % 16)
-        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, exponents, mask and scratch must be there, 16-byte aligned", me);
+    if (!image || ((uintptr_t)image | (uintptr_t)codes | (uintptr_t)mask | (uintptr_t)exponents) % 16)
+        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, exponents, mask and image must be there, 16-byte aligned", me);
     if (((uintptr_t)z | (uintptr_t)W1 | (uintptr_t)b1 | (uintptr_t)W2 | (uintptr_t)y) % 4) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be float aligned", me);
-    const int64_t need = npa_mlp_checkpoint_forward_scratch_bytes(rows, in_dim, out_dim);
-    if (scratch_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: scratch has %lld bytes, %lld needed", me, (long long)scratch_bytes, (long long)need);
+    const int64_t need = ck_image_bytes(in_dim);
+    if (image_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: image has %lld bytes, %lld needed", me, (long long)image_bytes, (long long)need);
     CkForwardArgs a = {};
-    a.z = z; a.b1 = b1; a.image = static_cast<const uint8_t *>(scratch); a.y = y; a.codes = static_cast<int8_t *>(codes); a.exponents = exponents;
+    a.z = z; a.b1 = b1; a.image = static_cast<const uint8_t *>(image); a.y = y; a.codes = static_cast<int8_t *>(codes); a.exponents = exponents;
     a.mask = reinterpret_cast<uint2 *>(mask); a.rows = rows; a.in = in_dim; a.out = out_dim; a.pitch = (int)rows8_pitch(in_dim);
     a.chunks = (in_dim + 63) / 64; a.tiles = (int)((rows + kCkRows - 1) / kCkRows);
     if (!(a.status = umma_status_word())) return fail(NPA_ERR_CUDA, "%s: no status word", me);
     const cudaStream_t st = (cudaStream_t)stream;
-    const CkImageArgs image{W1, b1, W2, w1_stride_out, w1_stride_in, w2_stride_out, w2_stride_in, in_dim, out_dim, a.chunks, static_cast<uint8_t *>(scratch)};
-    launch_early(mlp_checkpoint_image_kernel, 8 * (a.chunks + 1), 512, 0, st, image);
+    const CkImageArgs make{W1, b1, W2, w1_stride_out, w1_stride_in, w2_stride_out, w2_stride_in, in_dim, out_dim, a.chunks, static_cast<uint8_t *>(image)};
+    launch_early(mlp_checkpoint_image_kernel, 8 * (a.chunks + 1), 512, 0, st, make);
     if ((rc = check_launch("mlp_checkpoint_image_kernel")) != NPA_OK) return rc;
     const auto kernel = a.chunks == 1 ? mlp_checkpoint_forward_kernel<1> : a.chunks == 2 ? mlp_checkpoint_forward_kernel<2> : mlp_checkpoint_forward_kernel<3>;
     const int smem = ck_forward_smem(a.chunks, out_dim);
@@ -1149,21 +1154,22 @@ int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1,
 
 int64_t npa_mlp_checkpoint_backward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim) {
     if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return 0;
-    return ck_image_bytes(in_dim) + 4 * ck_partial_floats(ck_reduce(rows, in_dim, out_dim));
+    return 4 * ck_partial_floats(ck_reduce(rows, in_dim, out_dim));
 }
 
-int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, const uint32_t *mask, const float *W1, const float *b1, const float *W2,
-                                const float *dy, float *dz, float *dW1, float *db1, float *dW2, int64_t rows, int32_t in_dim, int32_t out_dim,
-                                int64_t w1_stride_out, int64_t w1_stride_in, int64_t w2_stride_out, int64_t w2_stride_in, void *scratch,
+int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, const uint32_t *mask, const void *image, int64_t image_bytes, const float *b1,
+                                const float *dy, float *dz, float *dW1, float *db1, float *dW2, int64_t rows, int32_t in_dim, int32_t out_dim, void *scratch,
                                 int64_t scratch_bytes, void *stream) {
     const char *me = "npa_mlp_checkpoint_backward";
     int rc = check_mlp8(me, rows, in_dim, out_dim);
     if (rc != NPA_OK) return rc;
-    if (!codes || !exponents || !mask || !W1 || !b1 || !W2 || !dy) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every input must be non-NULL", me);
+    if (!codes || !exponents || !mask || !image || !b1 || !dy) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every input must be non-NULL", me);
     if ((!dW1 || !db1 || !dW2) && (dW1 || db1 || dW2)) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: dW1, db1 and dW2 come together", me);
-    if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)mask | (uintptr_t)dy) % 16)
-        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, mask, dy and scratch must be there, 16-byte aligned", me);
-    if (((uintptr_t)dz | (uintptr_t)exponents) % 4) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: dz and exponents must be 4-byte aligned", me);
+    if (!scratch || ((uintptr_t)scratch | (uintptr_t)codes | (uintptr_t)exponents | (uintptr_t)mask | (uintptr_t)image | (uintptr_t)dy) % 16)
+        return fail(NPA_ERR_INVALID_ARGUMENT, "%s: codes, exponents, mask, image, dy and scratch must be there, 16-byte aligned", me);
+    if (((uintptr_t)dz | (uintptr_t)b1) % 4) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: dz and b1 must be float aligned", me);
+    if (image_bytes < ck_image_bytes(in_dim))
+        return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: image has %lld bytes, %lld needed", me, (long long)image_bytes, (long long)ck_image_bytes(in_dim));
     const int64_t need = npa_mlp_checkpoint_backward_scratch_bytes(rows, in_dim, out_dim);
     if (scratch_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: scratch has %lld bytes, %lld needed", me, (long long)scratch_bytes, (long long)need);
     if (!dz && !dW1) return NPA_OK;
@@ -1171,13 +1177,10 @@ int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, con
     GradReduce r = ck_reduce(rows, in_dim, out_dim);
     CkArgs a = {};
     a.codes = static_cast<const int8_t *>(codes); a.exponents = exponents; a.mask = reinterpret_cast<const uint4 *>(mask); a.dy = dy; a.b1 = b1;
-    a.image = static_cast<const uint8_t *>(scratch); a.dz = dz; a.partial = reinterpret_cast<float *>(static_cast<char *>(scratch) + ck_image_bytes(in_dim));
+    a.image = static_cast<const uint8_t *>(image); a.dz = dz; a.partial = static_cast<float *>(scratch);
     a.rows = rows; a.in = in_dim; a.out = out_dim; a.pitch = (int)rows8_pitch(in_dim); a.chunks = (in_dim + 63) / 64; a.N1p = r.N1p; a.N2p = r.N2p;
     a.tiles = (int)((rows + kCkRows - 1) / kCkRows);
     if (!(a.status = umma_status_word())) return fail(NPA_ERR_CUDA, "%s: no status word", me);
-    const CkImageArgs image{W1, b1, W2, w1_stride_out, w1_stride_in, w2_stride_out, w2_stride_in, in_dim, out_dim, a.chunks, static_cast<uint8_t *>(scratch)};
-    launch_early(mlp_checkpoint_image_kernel, 8 * (a.chunks + 1), 512, 0, st, image);
-    if ((rc = check_launch("mlp_checkpoint_image_kernel")) != NPA_OK) return rc;
     const bool two = out_dim > 32;
     if (dz && (rc = ck_launch(two ? mlp_checkpoint_dz_kernel<true> : mlp_checkpoint_dz_kernel<false>, "mlp_checkpoint_dz_kernel", a, ck_dz_smem(a.chunks), r.ctas, st)) !=
                   NPA_OK)

@@ -936,43 +936,64 @@ Tensor restore_rows(const Tensor &codes, const Tensor &exponents, at::ScalarType
     return out;
 }
 
+// What a forward with a checkpoint keeps, in one block: offsets in bytes.
+struct CheckpointPlaces {
+    int64_t exps, mask, image, image_bytes, bytes;
+    CheckpointPlaces(int64_t m, int64_t k) {
+        auto after = [](int64_t at, int64_t size) { return (at + size + 255) & ~(int64_t)255; };
+        exps = after(0, m * code_pitch(k));
+        mask = after(exps, m * row_groups(k));
+        image = after(mask, m * kHidden / 8);
+        image_bytes = npa_mlp_checkpoint_image_bytes((int)k);
+        bytes = image + image_bytes;
+    }
+};
+
 // The adaptation MLP with its input kept in 8 bits and its hidden layer as the bits of the ReLU.
 struct MlpCheckpointNode : Node {
-    SavedVariable w1_, b1_, w2_, codes_, exps_, mask_;
+    SavedVariable w1_, b1_, w2_, kept_;
+    int64_t rows;
     std::vector<int64_t> z_shape;
     variable_list apply(variable_list &&g) override {
-        const Tensor w1 = w1_.unpack(), b1 = b1_.unpack(), w2 = w2_.unpack(), codes = codes_.unpack(), exps = exps_.unpack(), mask = mask_.unpack();
+        const Tensor w1 = w1_.unpack(), b1 = b1_.unpack(), w2 = w2_.unpack(), kept = kept_.unpack();  // raise when the graph was released
         const bool nz = should_compute_output(0), n1 = should_compute_output(1), nb = should_compute_output(2), n2 = should_compute_output(3);
         const bool weights = n1 || nb || n2;
         if (!g[0].defined() || !(nz || weights)) return variable_list(4);
         c10::cuda::CUDAGuard guard(w1.device());
         const Tensor dy = solid(g[0]);
-        const int64_t k = w1.size(1), o = w2.size(0), m = codes.size(0);
+        const int64_t k = w1.size(1), o = w2.size(0);
         Tensor gz = nz ? floats(w1, z_shape) : Tensor(), gw1, gb1, gw2;
         if (weights) {
             gw1 = blank(w1);
             gb1 = blank(b1);
             gw2 = blank(w2);
         }
-        if (m == 0) {
+        if (rows == 0) {
             if (weights) gw1.zero_(), gb1.zero_(), gw2.zero_();
         } else {
-            const int64_t bytes = npa_mlp_checkpoint_backward_scratch_bytes(m, (int)k, (int)o);
+            const CheckpointPlaces p(rows, k);
+            // (a hook may have had it elsewhere: the places are only good in a block of the same size)
+            TORCH_CHECK(kept.numel() == p.bytes && kept.scalar_type() == at::kByte && kept.device() == w1.device() && kept.is_contiguous(),
+                        "a saved-tensor hook returned another tensor than the MLP had saved");
+            const Tensor held = (uintptr_t)kept.const_data_ptr() % 16 ? kept.clone() : kept;
+            const uint8_t *t = held.const_data_ptr<uint8_t>();
+            const int64_t bytes = npa_mlp_checkpoint_backward_scratch_bytes(rows, (int)k, (int)o);
             Tensor scratch = fresh(w1, {bytes}, at::kByte);
-            check_status(npa_mlp_checkpoint_backward(codes.const_data_ptr(), exps.const_data_ptr<uint8_t>(), reinterpret_cast<const uint32_t *>(iptr(mask)), fptr(w1),
-                                                     fptr(b1), fptr(w2), fptr(dy), fmut(gz), fmut(gw1), fmut(gb1), fmut(gw2), m, (int)k, (int)o, w1.stride(0),
-                                                     w1.stride(1), w2.stride(0), w2.stride(1), scratch.mutable_data_ptr(), bytes, stream_of(w1)));
+            check_status(npa_mlp_checkpoint_backward(t, t + p.exps, reinterpret_cast<const uint32_t *>(t + p.mask), t + p.image, p.image_bytes, fptr(b1), fptr(dy),
+                                                     fmut(gz), fmut(gw1), fmut(gb1), fmut(gw2), rows, (int)k, (int)o, scratch.mutable_data_ptr(), bytes,
+                                                     stream_of(w1)));
         }
         return {gz, n1 ? gw1 : Tensor(), nb ? gb1 : Tensor(), n2 ? gw2 : Tensor()};
     }
     void release_variables() override {
-        w1_.reset_data(); b1_.reset_data(); w2_.reset_data(); codes_.reset_data(); exps_.reset_data(); mask_.reset_data();
+        w1_.reset_data(); b1_.reset_data(); w2_.reset_data(); kept_.reset_data();
     }
 };
 
 // The caller has checked types, devices and widths (mlp.supported); z is contiguous.
 Tensor mlp_checkpoint(const Tensor &z, const Tensor &w1, const Tensor &b1, const Tensor &w2) {
-    if (!recording(z, w1, b1, w2) && z.numel()) return mlp(z, w1, b1, w2);
+    const bool record = recording(z, w1, b1, w2);
+    if (!record && z.numel()) return mlp(z, w1, b1, w2);
     refuse_tangents("the adaptation MLP", z, w1, b1, w2);
     c10::cuda::CUDAGuard guard(z.device());
     const int64_t k = w1.size(1), o = w2.size(0);
@@ -980,18 +1001,17 @@ Tensor mlp_checkpoint(const Tensor &z, const Tensor &w1, const Tensor &b1, const
     const int64_t m = z.numel() / k;
     std::vector<int64_t> shape = z.sizes().vec();
     shape.back() = o;
-    Tensor y = floats(z, shape), codes = code_rows(z, m, k, at::kChar), exps = fresh(z, {m, row_groups(k)}, at::kByte), mask = ints(z, {m, kHidden / 32});
+    const CheckpointPlaces p(m, k);
+    Tensor y = floats(z, shape), kept = fresh(z, {m ? p.bytes : 0}, at::kByte);
     if (m) {
-        const int64_t bytes = npa_mlp_checkpoint_forward_scratch_bytes(m, (int)k, (int)o);
-        Tensor scratch = fresh(z, {bytes}, at::kByte);
+        uint8_t *t = kept.mutable_data_ptr<uint8_t>();
         check_status(npa_mlp_checkpoint_forward(fptr(z), fptr(w1), fptr(b1), fptr(w2), fmut(y), m, (int)k, (int)o, w1.stride(0), w1.stride(1), w2.stride(0),
-                                                w2.stride(1), codes.mutable_data_ptr(), exps.mutable_data_ptr<uint8_t>(), reinterpret_cast<uint32_t *>(imut(mask)),
-                                                scratch.mutable_data_ptr(), bytes, stream_of(z)));
+                                                w2.stride(1), t, t + p.exps, reinterpret_cast<uint32_t *>(t + p.mask), t + p.image, p.image_bytes, stream_of(z)));
     }
-    if (recording(z, w1, b1, w2)) {
+    if (record) {
         auto n = node_for<MlpCheckpointNode>(z, w1, b1, w2);
-        n->w1_ = saved(w1); n->b1_ = saved(b1); n->w2_ = saved(w2);
-        n->codes_ = saved(codes); n->exps_ = saved(exps); n->mask_ = saved(mask); n->z_shape = z.sizes().vec();
+        n->w1_ = saved(w1); n->b1_ = saved(b1); n->w2_ = saved(w2); n->kept_ = saved(kept);
+        n->rows = m; n->z_shape = z.sizes().vec();
         torch::autograd::set_history(y, n);
     }
     return y;

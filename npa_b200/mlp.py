@@ -132,7 +132,8 @@ def apply_mlp(module, z, checkpoint=False):
     """``module(z)``; with the fused weight-gradient backward when ``supported(module)``.
 
     ``checkpoint=True`` keeps for the backward, instead of ``z`` and the hidden layer in 32 bits (``4 (in + 128)`` bytes a
-    row), ``z`` in 8 bits (``rows8``) and the bits of the ReLU (``in + in / 32 + 16`` bytes): values and the gradients of
+    row), ``z`` in 8 bits (``rows8``) and the bits of the ReLU (``in + in / 32 + 16`` bytes a row, and for each call 65 to
+    131 KB of weights as the tensor cores read them): values and the gradients of
     ``z`` and of the bias are those of the plain call, the gradients of the two weight matrices see ``z`` rounded to 8 bits.
     It needs a ``supported`` module on the default engine, and is refused (``ValueError``) otherwise;
     without a gradient to record the call is the plain one."""
@@ -140,9 +141,11 @@ def apply_mlp(module, z, checkpoint=False):
         if not on_tensor_memory(module):
             raise ValueError("checkpoint=True needs Sequential(Linear(in, 128), ReLU, Linear(128, out, bias=False)) in float32 on a CUDA device "
                              f"with in <= {MAX_IN} and out <= {MAX_OUT}, on the default engine")
-        if not (z.device == module[0].weight.device and z.dtype == torch.float32):
-            raise TypeError(f"z: expected a float32 tensor on {module[0].weight.device}, got {z.dtype} on {z.device}")
-        return N.ops.mlp_checkpoint(z.contiguous(), module[0].weight, module[0].bias, module[2].weight)
+        first, _, last = module
+        w1 = first.weight
+        if z.device != w1.device or z.dtype != torch.float32:
+            raise TypeError(f"z: expected a float32 tensor on {w1.device}, got {z.dtype} on {z.device}")
+        return N.ops.mlp_checkpoint(z.contiguous(), w1, first.bias, last.weight)
     if not (supported(module) and z.is_cuda and z.dtype == torch.float32):
         return module(z)
     if TENSOR_ENGINE == "tcgen05" and FUSED_FORWARD and FUSED_HIDDEN_GRAD:

@@ -42,13 +42,14 @@ def test_bad_arguments_of_the_c_abi():
         (uns, "out <= 48", lib.npa_mlp_checkpoint_forward(ok, ok, ok, ok, ok, 1, 8, 49, 8, 1, 128, 1, ok, ok, ok, ok, 1 << 24, None)),
         (small, "needed", lib.npa_mlp_checkpoint_forward(ok, ok, ok, ok, ok, 1, 8, 4, 8, 1, 128, 1, ok, ok, ok, ok, 16, None)),
         (inv, "aligned", lib.npa_mlp_checkpoint_forward(ok, ok, ok, ok, ok, 1, 8, 4, 8, 1, 128, 1, odd, ok, ok, ok, 1 << 24, None)),
-        (inv, "non-NULL", lib.npa_mlp_checkpoint_backward(ok, ok, None, ok, ok, ok, ok, ok, ok, ok, ok, 1, 8, 4, 8, 1, 128, 1, ok, 1 << 24, None)),
-        (inv, "together", lib.npa_mlp_checkpoint_backward(ok, ok, ok, ok, ok, ok, ok, ok, None, ok, ok, 1, 8, 4, 8, 1, 128, 1, ok, 1 << 24, None)),
-        (small, "needed", lib.npa_mlp_checkpoint_backward(ok, ok, ok, ok, ok, ok, ok, ok, ok, ok, ok, 1, 8, 4, 8, 1, 128, 1, ok, 64, None)),
+        (inv, "non-NULL", lib.npa_mlp_checkpoint_backward(ok, ok, None, ok, 1 << 24, ok, ok, ok, ok, ok, ok, 1, 8, 4, ok, 1 << 24, None)),
+        (inv, "together", lib.npa_mlp_checkpoint_backward(ok, ok, ok, ok, 1 << 24, ok, ok, ok, None, ok, ok, 1, 8, 4, ok, 1 << 24, None)),
+        (small, "needed", lib.npa_mlp_checkpoint_backward(ok, ok, ok, ok, 1 << 24, ok, ok, ok, ok, ok, ok, 1, 8, 4, ok, 64, None)),
+        (small, "needed", lib.npa_mlp_checkpoint_backward(ok, ok, ok, ok, 64, ok, ok, ok, ok, ok, ok, 1, 8, 4, ok, 1 << 24, None)),
     ]
     # (each message is the last error of its own call only when read at once)
     assert [rc for _, _, rc in calls] == [want for want, _, _ in calls]
-    rc = lib.npa_mlp_checkpoint_backward(ok, ok, ok, ok, ok, ok, ok, ok, None, ok, ok, 1, 8, 4, 8, 1, 128, 1, ok, 1 << 24, None)
+    rc = lib.npa_mlp_checkpoint_backward(ok, ok, ok, ok, 1 << 24, ok, ok, ok, None, ok, ok, 1, 8, 4, ok, 1 << 24, None)
     assert rc == inv and "together" in n.last_error()
     room = lib.npa_linear_int8_scratch_bytes
     assert room(ok, I8, 16, ok, 16, 100, 8, 4) == 0 and room(ok, F32, 8, ok, 16, 100, 8, 4) >= 100 * 16 + 400  # codes and scales of the rows
