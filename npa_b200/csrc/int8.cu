@@ -18,7 +18,7 @@ constexpr int kInt8MaxIn = 65536;
 // codes; what is beyond is read twice, the second time from L1 or L2.
 constexpr int kQuantizeHeld = 4;
 
-template <typename X, bool UNSIGNED, int T, int V>
+template <typename X, bool UNSIGNED, int T, int V, int W>
 __global__ void __launch_bounds__(T > 128 ? T : 128) quantize_rows_kernel(const X *__restrict__ x, long long pitch, long long rows, int cols,
                                                                          uint8_t *__restrict__ codes, long long codes_pitch, float *__restrict__ scales) {
     after_previous_kernel();
@@ -31,14 +31,14 @@ __global__ void __launch_bounds__(T > 128 ? T : 128) quantize_rows_kernel(const 
     float v[kQuantizeHeld][V];
     unsigned largest = 0;
 #pragma unroll
-    for (int i = 0; i < kQuantizeHeld; ++i) load_values<X, V>(p + (i * T + t) * V, end - (i * T + t) * V, v[i]);
+    for (int i = 0; i < kQuantizeHeld; ++i) load_values<X, V, W>(p + (i * T + t) * V, end - (i * T + t) * V, v[i]);
 #pragma unroll
     for (int i = 0; i < kQuantizeHeld; ++i)
 #pragma unroll
         for (int q = 0; q < V; ++q) largest = max(largest, magnitude(quantizable<UNSIGNED>(v[i][q])));
     for (int k = (kQuantizeHeld * T + t) * V; k < end; k += T * V) {
         float w[V];
-        load_values<X, V>(p + k, end - k, w);
+        load_values<X, V, W>(p + k, end - k, w);
 #pragma unroll
         for (int q = 0; q < V; ++q) largest = max(largest, magnitude(quantizable<UNSIGNED>(w[q])));
     }
@@ -73,24 +73,26 @@ __global__ void __launch_bounds__(T > 128 ? T : 128) quantize_rows_kernel(const 
         if ((i * T + t) * V < cols) put((i * T + t) * V, v[i]);
     for (int k = (kQuantizeHeld * T + t) * V; k < cols; k += T * V) {
         float w[V];
-        load_values<X, V>(p + k, cols - k, w);
+        load_values<X, V, W>(p + k, cols - k, w);
         put(k, w);
     }
     if (t == 0) scales[row] = scale;
 }
 
 // Rows of up to 32 kBlocks values whose addresses fit no vector: a warp takes eight of them, lane = column, so that its loads are lines
-// and the maxima share their shuffles.
+// and the maxima share their shuffles.  Codes leave through shared memory in 16 bytes a lane where they may (`whole`).
 template <typename X, bool UNSIGNED, int kBlocks>
 __global__ void __launch_bounds__(128) quantize_lanes_kernel(const X *__restrict__ x, long long pitch, long long rows, int cols, uint8_t *__restrict__ codes,
                                                              long long codes_pitch, float *__restrict__ scales) {
     after_previous_kernel();
-    const int lane = threadIdx.x & 31;
-    const long long row0 = ((long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * 8;
+    __shared__ __align__(16) uint8_t staged[4][8][32 * kBlocks];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long row0 = ((long long)blockIdx.x * 4 + warp) * 8;
     if (row0 >= rows) return;
     float v[8][kBlocks];
     unsigned largest[8];
     const int there = rows - row0 < 8 ? (int)(rows - row0) : 8;
+    const bool whole = (reinterpret_cast<uintptr_t>(codes) | codes_pitch) % 16 == 0;
 #pragma unroll
     for (int r = 0; r < 8; ++r)
 #pragma unroll
@@ -107,12 +109,21 @@ __global__ void __launch_bounds__(128) quantize_lanes_kernel(const X *__restrict
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
         const float scale = __shfl_sync(kFull, own, 4 * r), inverse = __shfl_sync(kFull, back, 4 * r);
-        if (r >= there) continue;
         unsigned code[kBlocks];
         row_codes<kBlocks>(v[r], scale, inverse, code);
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-            if (32 * b + lane < cols) codes[(row0 + r) * codes_pitch + 32 * b + lane] = inverse == 0.f ? (uint8_t)0 : (uint8_t)code[b];
+        for (int b = 0; b < kBlocks; ++b) {
+            const uint8_t c = inverse == 0.f ? (uint8_t)0 : (uint8_t)code[b];
+            if (whole) staged[warp][r][32 * b + lane] = c;
+            else if (r < there && 32 * b + lane < cols) codes[(row0 + r) * codes_pitch + 32 * b + lane] = c;
+        }
+    }
+    if (!whole) return;
+    __syncwarp();
+    const int pieces = (cols + 15) / 16;
+    for (int q = lane; q < there * pieces; q += 32) {
+        const int r = q / pieces, k = 16 * (q - r * pieces);
+        *reinterpret_cast<uint4 *>(codes + (row0 + r) * codes_pitch + k) = *reinterpret_cast<const uint4 *>(&staged[warp][r][k]);
     }
 }
 
@@ -344,21 +355,26 @@ static void by_type(int type, F f) {
 static bool is_float(int type) { return type == NPA_FLOAT32 || type == NPA_FLOAT16 || type == NPA_BFLOAT16; }
 static bool is_code(int type) { return type == NPA_INT8 || type == NPA_UINT8; }
 
-template <typename X, bool UNSIGNED, int T, int V>
+template <typename X, bool UNSIGNED, int T, int V, int W>
 static void launch_quantize_shape(const void *x, long long pitch, long long rows, int cols, void *codes, long long codes_pitch, float *scales, cudaStream_t st) {
     constexpr int kRows = T >= 128 ? 1 : 128 / T;
-    launch_early(quantize_rows_kernel<X, UNSIGNED, T, V>, (unsigned)((rows + kRows - 1) / kRows), T > 128 ? T : 128, 0, st, static_cast<const X *>(x), pitch, rows, cols,
+    launch_early(quantize_rows_kernel<X, UNSIGNED, T, V, W>, (unsigned)((rows + kRows - 1) / kRows), T > 128 ? T : 128, 0, st, static_cast<const X *>(x), pitch, rows, cols,
                  static_cast<uint8_t *>(codes), codes_pitch, scales);
 }
 template <typename X, bool UNSIGNED>
 static void launch_quantize_type(const void *x, long long pitch, long long rows, int cols, void *codes, long long codes_pitch, float *scales, cudaStream_t st) {
-#define NPA_QUANTIZE(T, V) launch_quantize_shape<X, UNSIGNED, T, V>(x, pitch, rows, cols, codes, codes_pitch, scales, st)
-    if (((uintptr_t)x | (uintptr_t)(pitch * (long long)sizeof(X))) % 16 == 0) {
+#define NPA_QUANTIZE(T, V, W) launch_quantize_shape<X, UNSIGNED, T, V, W>(x, pitch, rows, cols, codes, codes_pitch, scales, st)
+    const uintptr_t lie = (uintptr_t)x | (uintptr_t)(pitch * (long long)sizeof(X));
+    if (lie % 16 == 0) {
         // threads for a row so that it fits the registers of each
-        if (cols <= 128) NPA_QUANTIZE(8, 8);
-        else if (cols <= 1024) NPA_QUANTIZE(32, 8);
-        else if (cols <= 4096) NPA_QUANTIZE(128, 8);
-        else NPA_QUANTIZE(256, 8);
+        if (cols <= 128) NPA_QUANTIZE(8, 8, 16);
+        else if (cols <= 1024) NPA_QUANTIZE(32, 8, 16);
+        else if (cols <= 4096) NPA_QUANTIZE(128, 8, 16);
+        else NPA_QUANTIZE(256, 8, 16);
+    } else if (lie % 8 == 0) {
+        if (cols <= 128) NPA_QUANTIZE(8, 8, 8);
+        else if (cols <= 1024) NPA_QUANTIZE(32, 8, 8);
+        else NPA_QUANTIZE(256, 8, 8);
     } else {
         if (cols <= 512) {
             void (*const kernel)(const X *, long long, long long, int, uint8_t *, long long, float *) =
@@ -369,9 +385,9 @@ static void launch_quantize_type(const void *x, long long pitch, long long rows,
                              scales);
                 return;
             }
-            NPA_QUANTIZE(128, 1);
+            NPA_QUANTIZE(128, 1, 16);
         } else {
-            NPA_QUANTIZE(256, 1);
+            NPA_QUANTIZE(256, 1, 16);
         }
     }
 #undef NPA_QUANTIZE

@@ -9,6 +9,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace npa {
@@ -125,20 +127,21 @@ __device__ __forceinline__ void warp_max8(unsigned (&v)[8]) {
     for (int r = 0; r < 8; ++r) v[r] = __shfl_sync(kFull, m, max8_lane<LANES>(r));
 }
 
-// V values at p, of which `left` exist.
-template <typename T, int V>
+// V values at p, of which `left` exist; in loads of W bytes.
+template <typename T, int V, int W = 16>
 __device__ __forceinline__ void load_values(const T *__restrict__ p, int left, float (&v)[V]) {
     if constexpr (V == 1) {
         v[0] = left > 0 ? as_float(p[0]) : 0.f;
     } else {
         if (left >= V) {
-            constexpr int kQuads = V * (int)sizeof(T) / 16;
+            using Word = std::conditional_t<W == 16, uint4, uint2>;
+            constexpr int kWords = V * (int)sizeof(T) / W;
             union {
-                uint4 quad[kQuads];
+                Word word[kWords];
                 T value[V];
             } u;
 #pragma unroll
-            for (int q = 0; q < kQuads; ++q) u.quad[q] = __ldg(reinterpret_cast<const uint4 *>(p) + q);
+            for (int q = 0; q < kWords; ++q) u.word[q] = __ldg(reinterpret_cast<const Word *>(p) + q);
 #pragma unroll
             for (int q = 0; q < V; ++q) v[q] = as_float(u.value[q]);
         } else {

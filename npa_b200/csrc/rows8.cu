@@ -3,17 +3,17 @@
 
 namespace npa {
 
-// Rows whose addresses are multiples of 16 bytes: a thread takes eight values, four neighbours a group.
-template <typename T>
+// Rows whose addresses are multiples of W = 16 or 8 bytes: a thread takes eight values, four neighbours a group.
+template <typename T, int W>
 __global__ void __launch_bounds__(256) rows8_compress_kernel(const T *__restrict__ x, long long pitch, long long rows, int cols, int8_t *__restrict__ codes,
                                                              long long codes_pitch, uint8_t *__restrict__ exps) {
     after_previous_kernel();
     const int groups = rows8_groups(cols), each = 4 * groups;
-    const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x, row = at / each;
+    const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x, row = (rows * each) >> 32 ? at / each : (long long)((unsigned)at / (unsigned)each);
     const int part = (int)(at - row * each), k = 8 * part;
     const int left = row < rows ? cols - k : 0;
     float v[8];
-    load_values<T, 8>(x + (left > 0 ? row * pitch + k : 0), left, v);
+    load_values<T, 8, W>(x + (left > 0 ? row * pitch + k : 0), left, v);
     unsigned largest = 0;
 #pragma unroll
     for (int q = 0; q < 8; ++q) largest = max(largest, magnitude(v[q]));
@@ -29,45 +29,64 @@ __global__ void __launch_bounds__(256) rows8_compress_kernel(const T *__restrict
     if (part % 4 == 0) exps[row * groups + part / 4] = (uint8_t)e;
 }
 
-// Other rows: a warp takes a group, lane = column, so that its loads are lines; eight groups in flight.
+// Other rows: a warp takes eight groups that follow one another, lane = column, so that its loads are lines and the maxima share their
+// shuffles.  The codes leave through shared memory in pieces of 16 bytes (`whole`: where rows of codes lie on such; bytes otherwise):
+// a store of 32 single bytes costs 12 clocks of an SM, whatever it hits (95 us for 8,191 rows of 4,100).
 constexpr int kRowsFlight = 8;
 template <typename T>
 __global__ void __launch_bounds__(256) rows8_compress_lanes_kernel(const T *__restrict__ x, long long pitch, long long rows, int cols,
-                                                                   int8_t *__restrict__ codes, long long codes_pitch, uint8_t *__restrict__ exps) {
+                                                                   int8_t *__restrict__ codes, long long codes_pitch, uint8_t *__restrict__ exps, int whole) {
     after_previous_kernel();
-    const int lane = threadIdx.x & 31, groups = rows8_groups(cols);
-    const long long first = ((long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kRowsFlight, units = rows * groups;
+    __shared__ __align__(16) uint8_t staged[8][kRowsFlight * kRowsGroup];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = rows8_groups(cols);
+    const long long first = ((long long)blockIdx.x * 8 + warp) * kRowsFlight, units = rows * groups;
     if (first >= units) return;
-    long long row = first / groups;
-    int g = (int)(first - row * groups);
+    const long long row0 = units >> 32 ? first / groups : (long long)((unsigned)first / (unsigned)groups);
+    const int g0 = (int)(first - row0 * groups);
     float v[kRowsFlight];
-    long long r = row;
-    int h = g;
-#pragma unroll
-    for (int i = 0; i < kRowsFlight; ++i) {
-        const int k = h * kRowsGroup + lane;
-        v[i] = r < rows && k < cols ? as_float(x[r * pitch + k]) : 0.f;
-        if (++h == groups) {
-            h = 0;
-            ++r;
-        }
-    }
     unsigned largest[kRowsFlight];
-#pragma unroll
-    for (int i = 0; i < kRowsFlight; ++i) largest[i] = magnitude(v[i]);
-    warp_max8(largest);
+    long long row = row0;
+    int g = g0;
 #pragma unroll
     for (int i = 0; i < kRowsFlight; ++i) {
-        const unsigned e = rows8_exponent(largest[i]);
         const int k = g * kRowsGroup + lane;
-        if (row < rows) {
-            if (k < cols) codes[row * codes_pitch + k] = (int8_t)rows8_code(v[i], rows8_to_units(e));
-            if (lane == 0) exps[row * groups + g] = (uint8_t)e;
-        }
+        v[i] = row < rows && k < cols ? as_float(x[row * pitch + k]) : 0.f;
+        largest[i] = magnitude(v[i]);
         if (++g == groups) {
             g = 0;
             ++row;
         }
+    }
+    const unsigned e = rows8_exponent(gather_max8(largest));  // of group lane / 4
+    const float to_units = rows8_to_units(e);
+    const int mine = lane >> 2;
+    if ((lane & 3) == 0 && first + mine < units) exps[first + mine] = (uint8_t)e;
+    uint8_t *to = staged[warp];
+    row = row0;
+    g = g0;
+#pragma unroll
+    for (int i = 0; i < kRowsFlight; ++i) {
+        const int code = rows8_code(v[i], __shfl_sync(kFull, to_units, 4 * i));
+        if (whole) {
+            to[i * kRowsGroup + lane] = (uint8_t)code;
+        } else {
+            const int k = g * kRowsGroup + lane;
+            if (row < rows && k < cols) codes[row * codes_pitch + k] = (int8_t)code;
+            if (++g == groups) {
+                g = 0;
+                ++row;
+            }
+        }
+    }
+    if (!whole) return;
+    __syncwarp();
+    // half a group a lane: 16 bytes, unless they lie behind the row's last column
+    const long long at = first + (lane >> 1);
+    if (lane < 2 * kRowsFlight && at < units) {
+        const int ahead = g0 + (lane >> 1);
+        const long long r = row0 + ahead / groups;
+        const int k = (ahead % groups) * kRowsGroup + 16 * (lane & 1);
+        if (k < cols) *reinterpret_cast<uint4 *>(codes + r * codes_pitch + k) = *reinterpret_cast<const uint4 *>(to + 16 * lane);
     }
 }
 
@@ -87,7 +106,7 @@ __global__ void __launch_bounds__(256) rows8_restore_kernel(const int8_t *__rest
     const long long first = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * V, total = rows * cols;
     if (first >= total) return;
     const int groups = rows8_groups(cols);
-    long long row = first / cols;
+    long long row = total >> 32 ? first / cols : (long long)((unsigned)first / (unsigned)cols);
     int k = (int)(first - row * cols);
     union {
         uint4 quad;
@@ -95,24 +114,22 @@ __global__ void __launch_bounds__(256) rows8_restore_kernel(const int8_t *__rest
     } u;
     const int8_t *c = codes + row * codes_pitch;
     const uint8_t *e = exps + row * groups;
-    if (k + V <= cols && k / kRowsGroup == (k + V - 1) / kRowsGroup) {  // within one group of one row
-        const float unit = rows8_unit(e[k / kRowsGroup]);
+    if (k + V <= cols) {  // within one row: one group, or two
+        const int g = k / kRowsGroup, left = (g + 1) * kRowsGroup - k;
+        const float one = rows8_unit(e[g]), two = left < V ? rows8_unit(e[g + 1]) : one;
         int code[V];
-        if ((reinterpret_cast<uintptr_t>(c + k)) % V == 0) {
-            if constexpr (V == 4) {
-                const char4 q = *reinterpret_cast<const char4 *>(c + k);
-                code[0] = q.x; code[1] = q.y; code[2] = q.z; code[3] = q.w;
-            } else {
-                const uint2 q = *reinterpret_cast<const uint2 *>(c + k);
+        if (reinterpret_cast<uintptr_t>(c + k) % 4 == 0) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) code[i] = (int)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i % 4)));
+            for (int w = 0; w < V / 4; ++w) {
+                const char4 q = *reinterpret_cast<const char4 *>(c + k + 4 * w);
+                code[4 * w] = q.x; code[4 * w + 1] = q.y; code[4 * w + 2] = q.z; code[4 * w + 3] = q.w;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) code[i] = c[k + i];
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) u.value[i] = restored<T>((float)code[i] * unit);
+        for (int i = 0; i < V; ++i) u.value[i] = restored<T>((float)code[i] * (i < left ? one : two));
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -167,10 +184,16 @@ int npa_rows8_compress(const void *x, int32_t type, int64_t x_pitch, int64_t row
     if (x_pitch < 0) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: x_pitch must not be negative", me);
     by_float_type(type, [&](auto t) {
         using T = decltype(t);
-        const bool vectors = ((uintptr_t)x | (uintptr_t)(x_pitch * (int64_t)sizeof(T))) % 16 == 0;
+        const uintptr_t lie = (uintptr_t)x | (uintptr_t)(x_pitch * (int64_t)sizeof(T));
+        const bool vectors = lie % 8 == 0;
         const long long units = rows * rows8_groups(cols), blocks = vectors ? (4 * units + 255) / 256 : (units + 8 * kRowsFlight - 1) / (8 * kRowsFlight);
-        launch_early(vectors ? rows8_compress_kernel<T> : rows8_compress_lanes_kernel<T>, (unsigned)blocks, 256, 0, (cudaStream_t)stream,
-                     static_cast<const T *>(x), x_pitch, rows, cols, static_cast<int8_t *>(codes), codes_pitch, exponents);
+        const int whole = ((uintptr_t)codes | (uintptr_t)codes_pitch) % 16 == 0;
+        if (vectors)
+            launch_early(lie % 16 == 0 ? rows8_compress_kernel<T, 16> : rows8_compress_kernel<T, 8>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, static_cast<const T *>(x), x_pitch, rows, cols,
+                         static_cast<int8_t *>(codes), codes_pitch, exponents);
+        else
+            launch_early(rows8_compress_lanes_kernel<T>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, static_cast<const T *>(x), x_pitch, rows, cols,
+                         static_cast<int8_t *>(codes), codes_pitch, exponents, whole);
     });
     return check_launch("rows8_compress_kernel");
 }
