@@ -140,10 +140,11 @@ __global__ void __launch_bounds__(256) dequantize_rows_kernel(const Code *__rest
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
 // Up to 16 rows (a token, a handful of particles): the weights are read once, from memory or L2, and that is the time.  Each block holds
-// the codes of all rows in shared memory (it quantises them itself: they are few and in L2, and a launch of its own would cost more),
+// the codes of all rows in shared memory (it quantises up to 8,192 values itself, from L2; of more, every block would do too much of the
+// same: a launch in front does it, linear_few_odd 13.0 -> 9 us),
 // a warp takes NC channels and a lane 16 bytes of each at a time, NC x 4 loads in flight; four dp4a per row and 16 bytes are free
 // beside them.  Where the channels alone would not fill the SMs, the warps of a block share a channel's length.
-constexpr int kFewRows = 16, kFewBytes = 96 * 1024, kFewWarps = 8;
+constexpr int kFewRows = 16, kFewBytes = 96 * 1024, kFewWarps = 8, kFewQuantized = 8192;
 
 template <bool UNSIGNED>
 __device__ __forceinline__ int dot4(unsigned x, unsigned w, int acc) {
@@ -167,9 +168,27 @@ __device__ __forceinline__ void few_rows_codes(const Int8Args &a, uint8_t *codes
     const int rows = (int)a.rows, K = a.in;
     if (a.x_type >= NPA_INT8) {
         const uint8_t *x = static_cast<const uint8_t *>(a.x);
-        for (int q = threadIdx.x; q < ROWS * pitch; q += kFewWarps * 32) {
-            const int r = q / pitch, k = q - r * pitch;
-            codes[q] = r < rows && k < K ? __ldg(x + r * a.x_pitch + k) : 0;
+        if ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)a.x_pitch) % 16 == 0 && a.x_pitch >= pitch) {  // (codes behind a row's end meet weights of zero)
+            const int pieces = pitch / 16;
+            for (int q = threadIdx.x; q < ROWS * pieces; q += kFewWarps * 32) {
+                const int r = q / pieces, k = 16 * (q - r * pieces);
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < rows && k + 16 <= K) {
+                    v = __ldg(reinterpret_cast<const uint4 *>(x + r * a.x_pitch + k));
+                } else if (r < rows) {
+                    unsigned w[4] = {};
+#pragma unroll
+                    for (int j = 0; j < 15; ++j)
+                        if (k + j < K) w[j / 4] |= (unsigned)__ldg(x + r * a.x_pitch + k + j) << (8 * (j % 4));
+                    v = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                *reinterpret_cast<uint4 *>(codes + r * pitch + k) = v;
+            }
+        } else {
+            for (int q = threadIdx.x; q < ROWS * pitch; q += kFewWarps * 32) {
+                const int r = q / pitch, k = q - r * pitch;
+                codes[q] = r < rows && k < K ? __ldg(x + r * a.x_pitch + k) : 0;
+            }
         }
         if (threadIdx.x < ROWS) scales[threadIdx.x] = threadIdx.x < rows ? __ldg(a.x_scales + threadIdx.x) : 0.f;
         return;
@@ -445,7 +464,7 @@ struct Int8Plan {
     long long o_scales, o_w, o_sums, bytes;
     Int8Plan(const void *x, int x_type, long long x_pitch, const void *w, long long w_pitch, long long rows, int in, int out_dim) {
         few = few_rows(rows, in);
-        quantize = !few && is_float(x_type);
+        quantize = is_float(x_type) && (!few || rows * in > kFewQuantized);
         repack_x = !few && is_code(x_type) && (x_type == NPA_UINT8 || !aligned_codes(x, x_pitch) || x_pitch < in);
         repack_w = !aligned_codes(w, w_pitch) || w_pitch < in;  // (rows that overlap: TMA wants none)
         sums = !few && x_type == NPA_UINT8;
@@ -537,7 +556,6 @@ int npa_linear_int8(const void *x, int32_t x_type, int64_t x_pitch, const float 
         if ((rc = launch_repack(w, w_pitch, out_dim, in_dim, 0, s + plan.o_w, st)) != NPA_OK) return rc;
         a.w = reinterpret_cast<const int8_t *>(s + plan.o_w); a.w_pitch = round16(in_dim);
     }
-    if (plan.few) return launch_few_rows(a, st);
     if (plan.quantize) {
         float *scales = reinterpret_cast<float *>(s + plan.o_scales);
         if ((rc = launch_quantize(x, x_type, x_pitch, rows, in_dim, false, s, round16(in_dim), scales, st)) != NPA_OK) return rc;
@@ -547,6 +565,7 @@ int npa_linear_int8(const void *x, int32_t x_type, int64_t x_pitch, const float 
     if (plan.quantize || plan.repack_x) {
         a.x = s; a.x_pitch = round16(in_dim); a.x_type = NPA_INT8;
     }
+    if (plan.few) return launch_few_rows(a, st);
     if (plan.sums) {
         int *sums = reinterpret_cast<int *>(s + plan.o_sums);
         launch_early(weight_sums_kernel, (out_dim + 7) / 8, 256, 0, st, a.w, a.w_pitch, out_dim, in_dim, sums);
