@@ -198,29 +198,42 @@ struct DyRows {
             v[i].y = there && two ? __ldg(p + i * kEach * a.out + 1) : 0.f;
         }
     }
-    // ... and stored as heads and tails in units of their rows, whose exponents go to `units`.
-    __device__ __forceinline__ void store(uint8_t *heads, uint8_t *tails, int *units, int first, int lane) const {
-        const int k = TWO ? 2 * lane : 2 * (lane & 15), r0 = first + (TWO ? 0 : lane >> 4);
+    __device__ __forceinline__ void put(uint8_t *heads, uint8_t *tails, int first, int i, float scale, int lane) const {
+        unsigned head, tail;
+        split_halves(v[i].x * scale, v[i].y * scale, head, tail);
+        const int place = half_place(first + (TWO ? 0 : lane >> 4) + i * kEach, TWO ? 2 * lane : 2 * (lane & 15));
+        if (!TWO || lane < 24) {
+            *reinterpret_cast<unsigned *>(heads + place) = head;
+            *reinterpret_cast<unsigned *>(tails + place) = tail;
+        }
+    }
+    // ... and stored as heads and tails in units of their rows, whose exponents go to `units`: a lane works out one row's (four or two
+    // lanes the same) and hands it round.
+    __device__ __forceinline__ void store_by_row(uint8_t *heads, uint8_t *tails, int *units, int first, int lane) const {
+        constexpr int kLanes = TWO ? 32 : 16;
 #pragma unroll
         for (int i0 = 0; i0 < kPasses; i0 += 8) {
             unsigned m[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) m[i] = max(finite_magnitude(v[i0 + i].x), finite_magnitude(v[i0 + i].y));
-            warp_max8<TWO ? 32 : 16>(m);
+            const unsigned field = row_unit(gather_max8<kLanes>(m));
+            const float scale = from_row_unit(field);
+            const int pass = i0 + (lane & (kLanes - 1)) / (kLanes / 8);
+            if (lane % (kLanes / 8) == 0) units[first + (TWO ? 0 : lane >> 4) + pass * kEach] = (int)field - 127;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned field = row_unit(m[i]);
-                const float s = from_row_unit(field);
-                unsigned head, tail;
-                split_halves(v[i0 + i].x * s, v[i0 + i].y * s, head, tail);
-                const int row = r0 + (i0 + i) * kEach, place = half_place(row, k);
-                if (!TWO || lane < 24) {
-                    *reinterpret_cast<unsigned *>(heads + place) = head;
-                    *reinterpret_cast<unsigned *>(tails + place) = tail;
-                }
-                if ((lane & (TWO ? 31 : 15)) == 0) units[row] = (int)field - 127;
-            }
+            for (int i = 0; i < 8; ++i) put(heads, tails, first, i0 + i, __shfl_sync(kFull, scale, max8_lane<kLanes>(i)), lane);
         }
+    }
+    // The largest finite magnitude of the warp's rows; and heads and tails in one unit.
+    __device__ __forceinline__ unsigned largest() const {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) m = max(m, max(finite_magnitude(v[i].x), finite_magnitude(v[i].y)));
+        return warp_max(m);
+    }
+    __device__ __forceinline__ void store(uint8_t *heads, uint8_t *tails, float scale, int first, int lane) const {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) put(heads, tails, first, i, scale, lane);
     }
 };
 
@@ -232,31 +245,25 @@ __device__ __forceinline__ void ck_copy_image(uint8_t *dst, const CkArgs &a, uin
 
 // ---- dz ----------------------------------------------------------------------------------------------------------------
 // Warp-specialised, one persistent CTA per SM, tiles of 128 rows: four producer warps (32 rows of dy each, a tile ahead in registers;
-// a lane of the first issues the MMAs), four warps that mask dh and take it apart in place (lane = row; head and tail of 16 columns fill the 16 columns
-// of the accumulator they came from), four that store dz.  dh has two accumulators, so that the next tile's is made meanwhile.
+// a lane of the first issues the MMAs), eight that mask dh and take it apart in place (lane = row; head and tail of 16 columns fill the
+// 16 columns of the accumulator they came from) and store dz of the tile before.  dh has two accumulators, so that the next tile's is made
+// meanwhile.
 struct CkDzShared {
-    uint64_t image, op_full[2], op_empty[2], dh_full[2], dh_ready[2], dz_full, dz_empty;
+    uint64_t image, op_full, op_empty, dh_full[2], dh_ready[2], dz_full, dz_empty, staged[4], copied[4];
     int units[kCkRowRing][kCkRows];
     uint32_t tmem_base;
     int abort;
 };
-constexpr int kCkStagePitch = 36;  // floats of a staged row of 32 columns
 constexpr int kCkDzCol = 256;
-static int ck_dz_smem(int chunks) { return 1024 + (2 * chunks + 2) * kCkTile + 4 * kCkTile + 4 * 32 * kCkStagePitch * 4; }
-
-// 32 staged rows of 32 columns to rows of `pitch` floats, V at a time.
-template <int V>
-__device__ __forceinline__ void store_block(const float *stg, float *out, long long pitch, int nrows, int ncols, int lane) {
-    constexpr int kLanes = 32 / V, kStep = 32 / kLanes;
-    const int c = (lane % kLanes) * V, r0 = lane / kLanes;
-    if (c >= ncols) return;
-#pragma unroll 8
-    for (int r = r0; r < nrows; r += kStep) {
-        if constexpr (V == 4) *reinterpret_cast<float4 *>(out + r * pitch + c) = *reinterpret_cast<const float4 *>(stg + r * kCkStagePitch + c);
-        else if constexpr (V == 2) *reinterpret_cast<float2 *>(out + r * pitch + c) = *reinterpret_cast<const float2 *>(stg + r * kCkStagePitch + c);
-        else out[r * pitch + c] = stg[r * kCkStagePitch + c];
-    }
+// A quarter's 32 rows of dz are put together as they lie in memory; two quarters share a buffer where four do not fit.
+__host__ __device__ constexpr int ck_dz_buffers(int in) { return in <= 128 ? 4 : 2; }
+static int ck_dz_smem(int chunks, int in) { return 1024 + (2 * chunks + 2) * kCkTile + 2 * kCkTile + ck_dz_buffers(in) * 128 * in; }
+__device__ inline void bulk_copy_s2g(void *dst, const void *src, unsigned bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
 }
+__device__ inline void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ inline void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ inline void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 template <bool TWO>
 __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const __grid_constant__ CkArgs a) {
@@ -264,19 +271,23 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
     extern __shared__ uint8_t ck_raw[];
     __shared__ CkDzShared sh;
     uint8_t *base = ck_raw + ((1024u - (smem_u32(ck_raw) & 1023u)) & 1023u);
-    uint8_t *w2 = base + 2 * a.chunks * kCkTile, *ops = w2 + 2 * kCkTile;  // ops: [2][head | tail]
-    float *staged = reinterpret_cast<float *>(ops + 4 * kCkTile);
+    uint8_t *w2 = base + 2 * a.chunks * kCkTile, *ops = w2 + 2 * kCkTile;  // ops: heads | tails
+    float *staged = reinterpret_cast<float *>(ops + 2 * kCkTile);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(&sh.image, 1);
+        mbar_init(&sh.op_full, kCkProducers);
+        mbar_init(&sh.op_empty, 1);
         for (int q = 0; q < 2; ++q) {
-            mbar_init(&sh.op_full[q], kCkProducers);
-            mbar_init(&sh.op_empty[q], 1);
             mbar_init(&sh.dh_full[q], 1);
-            mbar_init(&sh.dh_ready[q], 4);
+            mbar_init(&sh.dh_ready[q], 8);
+        }
+        for (int q = 0; q < 4; ++q) {
+            mbar_init(&sh.staged[q], 2);
+            mbar_init(&sh.copied[q], 1);
         }
         mbar_init(&sh.dz_full, 2);  // the products, and the MMA lane itself: what it has seen of the producers' writes the epilogue sees
-        mbar_init(&sh.dz_empty, 4);
+        mbar_init(&sh.dz_empty, 8);
         sh.abort = 0;
         mbar_fence_init();
     }
@@ -305,17 +316,17 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
         auto first = [&](int t) -> bool {
             const int b = t & 1;
             if (t == 0 && !umma_wait(&sh.image, 0, &sh.abort)) return false;
-            if (!umma_wait(&sh.op_full[b], (t >> 1) & 1, &sh.abort)) return false;
+            if (!umma_wait(&sh.op_full, t & 1, &sh.abort)) return false;
             if (t > 1 && !umma_wait(&sh.dz_full, t & 1, &sh.abort)) return false;  // this accumulator was the operand of tile t - 2
             tc_fence_after();
-            const uint64_t dh = umma_desc(smem_u32(ops + b * 2 * kCkTile)), dl = umma_desc(smem_u32(ops + b * 2 * kCkTile + kCkTile));
+            const uint64_t dh = umma_desc(smem_u32(ops)), dl = umma_desc(smem_u32(ops + kCkTile));
             const unsigned d = tmem + b * 128;
             for (int ks = 0; ks < ks1; ++ks) {  // the small products first: an addition cuts off what lies below the sum's last bit
                 umma_f16(d, dl + 2 * ks, w2h + 2 * ks, id1, ks != 0);
                 umma_f16(d, dh + 2 * ks, w2l + 2 * ks, id1, 1);
             }
             for (int ks = 0; ks < ks1; ++ks) umma_f16(d, dh + 2 * ks, w2h + 2 * ks, id1, 1);
-            umma_commit(&sh.op_empty[b]);
+            umma_commit(&sh.op_empty);
             umma_commit(&sh.dh_full[b]);
             return true;
         };
@@ -338,13 +349,12 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
         if (ntile > 0) rows.load(a, row_of(0) + mine, lane);
 #pragma unroll 1
         for (int t = 0; t < ntile && ok; ++t) {
-            const int b = t & 1;
-            if (!(ok = umma_wait(&sh.op_empty[b], ((t >> 1) & 1) ^ 1, &sh.abort))) break;
-            rows.store(ops + b * 2 * kCkTile, ops + b * 2 * kCkTile + kCkTile, sh.units[t % kCkRowRing], mine, lane);
+            if (!(ok = umma_wait(&sh.op_empty, (t & 1) ^ 1, &sh.abort))) break;
+            rows.store_by_row(ops, ops + kCkTile, sh.units[t % kCkRowRing], mine, lane);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(&sh.op_full[b]);
+                mbar_arrive(&sh.op_full);
                 if (issues) ok = first(t);
             }
             __syncwarp();
@@ -362,79 +372,94 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             __nanosleep(20000);  // copies in flight land before the CTA leaves
         }
         __syncwarp();
-    } else if (warp < 4) {
-        const unsigned tlane = tmem + ((unsigned)(warp * 32) << 16);
-#pragma unroll 1
-        for (int t = 0; t < ntile; ++t) {
-            const int b = t & 1;
-            const long long row = row_of(t) + warp * 32 + lane;
-            const uint4 m = row < a.rows ? __ldg(a.mask + row) : make_uint4(0, 0, 0, 0);
-            if (!(ok = umma_wait(&sh.dh_full[b], (t >> 1) & 1, &sh.abort))) break;
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const unsigned word = c < 2 ? m.x : c < 4 ? m.y : c < 6 ? m.z : m.w, bits = c & 1 ? word >> 16 : word;
-                unsigned r[16], parts[16];
-                tmem_ld16(tlane + b * 128 + 16 * c, r);
-                tc_wait_ld();
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    split_halves(bits >> (2 * j) & 1u ? __uint_as_float(r[2 * j]) : 0.f, bits >> (2 * j + 1) & 1u ? __uint_as_float(r[2 * j + 1]) : 0.f, parts[j],
-                                 parts[8 + j]);
-                tmem_st16(tlane + b * 128 + 16 * c, parts);
-            }
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.dh_ready[b]);
-        }
-        if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_EPILOGUE);
     } else {
-        const int quarter = warp & 3;
-        const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16) + kCkDzCol;
-        float *stg = staged + quarter * 32 * kCkStagePitch;
+        const int quarter = warp & 3, half = warp >> 2;  // rows 32 quarter + lane; hidden units 64 half and up, every second 16 columns of dz
+        const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
         const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
-        const int vec = a.in % 4 == 0 && (uintptr_t)a.dz % 16 == 0 ? 4 : a.in % 2 == 0 && (uintptr_t)a.dz % 8 == 0 ? 2 : 1;
-#pragma unroll 1
-        for (int t = 0; t < ntile; ++t) {
+        const int buffers = ck_dz_buffers(a.in), turns = 4 / buffers, mine = quarter % buffers;  // (two quarters take turns)
+        float *stg = staged + mine * 32 * a.in;
+        const bool aligned = (uintptr_t)a.dz % 16 == 0;
+        auto bits_of = [&](int t) {
+            const long long row = row_of(t) + quarter * 32 + lane;
+            return row < a.rows ? __ldg(reinterpret_cast<const uint2 *>(a.mask) + 2 * row + half) : make_uint2(0, 0);
+        };
+        auto leave = [&](int t) -> bool {  // dz of tile t
             const long long row0 = row_of(t) + quarter * 32;
             const int nrows = a.rows - row0 < 32 ? (int)(a.rows - row0) : 32;  // may be <= 0
-            if (!(ok = umma_wait(&sh.dz_full, t & 1, &sh.abort))) break;
+            if (!umma_wait(&sh.dz_full, t & 1, &sh.abort)) return false;
             tc_fence_after();
             // the row's unit times those of the weights: one power of two unless it is out of range
             const int e = sh.units[t % kCkRowRing][quarter * 32 + lane] + head.w1 + head.w2, e1 = max(min(e, 127), -126);
             const float unit = power_of_two(e1), rest = power_of_two(max(e - e1, -126));
             const bool far = __any_sync(kFull, e != e1);
+            // the rows that were here before have left: turn `at` of this buffer, counted over the tiles
+            const int at = t * turns + quarter / buffers;
+            if (!umma_wait(&sh.copied[mine], (at & 1) ^ 1, &sh.abort)) return false;
+            float *row = stg + lane * a.in;
 #pragma unroll 1
-            for (int c0 = 0; c0 < a.in; c0 += 32) {
-                unsigned r[2][16];
-                tmem_ld16(tlane + c0, r[0]);
-                if (c0 + 16 < a.in) tmem_ld16(tlane + c0 + 16, r[1]);
+            for (int c0 = 16 * half; c0 < a.in; c0 += 32) {
+                unsigned r[16];
+                tmem_ld16(tlane + kCkDzCol + c0, r);
                 tc_wait_ld();
-                if (c0 + 32 >= a.in) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.dz_empty);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    float v = __uint_as_float(r[j]) * unit;
+                    if (far) v *= rest;
+                    if (c0 + j < a.in) row[c0 + j] = v;
                 }
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    float v[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[q / 4][4 * (q % 4) + j]) * unit;
-                    if (far) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) v[j] *= rest;
-                    }
-                    *reinterpret_cast<float4 *>(stg + lane * kCkStagePitch + 4 * q) = make_float4(v[0], v[1], v[2], v[3]);
-                }
-                __syncwarp();
-                float *out = a.dz + row0 * a.in + c0;
-                if (vec == 4) store_block<4>(stg, out, a.in, nrows, a.in - c0, lane);
-                else if (vec == 2) store_block<2>(stg, out, a.in, nrows, a.in - c0, lane);
-                else store_block<1>(stg, out, a.in, nrows, a.in - c0, lane);
-                __syncwarp();
             }
+            tc_fence_before();
+            fence_proxy_async();  // the copy reads these
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sh.dz_empty);
+                mbar_arrive(&sh.staged[mine]);
+            }
+            if (half == 0) {
+                if (!umma_wait(&sh.staged[mine], at & 1, &sh.abort)) return false;
+                if (nrows == 32 && aligned) {
+                    if (lane == 0) {
+                        bulk_copy_s2g(a.dz + row0 * a.in, stg, (unsigned)(128 * a.in));
+                        bulk_commit();
+                        bulk_wait_read();
+                    }
+                } else {
+                    for (int q = lane; q < nrows * a.in; q += 32) a.dz[row0 * a.in + q] = stg[q];
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.copied[mine]);
+            }
+            return true;
+        };
+        uint2 next = ntile > 0 ? bits_of(0) : make_uint2(0, 0);
+#pragma unroll 1
+        for (int t = 0; t < ntile; ++t) {
+            const int b = t & 1;
+            const uint2 m = next;
+            if (t + 1 < ntile) next = bits_of(t + 1);
+            if (!(ok = umma_wait(&sh.dh_full[b], (t >> 1) & 1, &sh.abort))) break;
+            tc_fence_after();
+            const unsigned d = tlane + b * 128 + 64 * half;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const unsigned word = c < 2 ? m.x : m.y, bits = c & 1 ? word >> 16 : word;
+                unsigned r[16], parts[16];
+                tmem_ld16(d + 16 * c, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    split_halves(bits >> (2 * j) & 1u ? __uint_as_float(r[2 * j]) : 0.f, bits >> (2 * j + 1) & 1u ? __uint_as_float(r[2 * j + 1]) : 0.f, parts[j],
+                                 parts[8 + j]);
+                tmem_st16(d + 16 * c, parts);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.dh_ready[b]);
+            if (t > 0 && !(ok = leave(t - 1))) break;
         }
+        if (ok && ntile > 0) ok = leave(ntile - 1);
+        if (lane == 0) bulk_wait();  // the rows are in memory before the block ends
         if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_EPILOGUE);
     }
 
@@ -451,10 +476,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
 // of the sums over the tile's rows.  The bits of 32 units and a row are one word, the same for a warp.  A tile's sums leave the
 // accumulators with the tile's unit and are added in 32 bits, in registers: up to 7 blocks of 16 columns a thread (kBlocks).
 struct CkWeightsShared {
-    uint64_t image, op_full, op_empty, p1_full, a_ready, p2_full;
+    uint64_t image, op_full, op_empty, dy_known, dh_full, pre_full, dh_ready, pre_ready, g1_full, g2_full;
     alignas(16) unsigned mask[4][kCkRows];
-    alignas(16) int units[kCkRows];
-    alignas(16) float factor[8][64];       // of the rows of each epilogue warp, relative to the tile
+    unsigned dy_most[2][kCkProducers];     // of two tiles: largest finite magnitude of each producer's rows
+    int dy_unit;
     alignas(16) uint8_t exponents[kCkRows * 6];
     float both[kCkRows];
     int z_unit;
@@ -495,9 +520,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         mbar_init(&sh.image, 1);
         mbar_init(&sh.op_full, kCkProducers);
         mbar_init(&sh.op_empty, 1);
-        mbar_init(&sh.p1_full, 2);  // the products, and the MMA lane itself: what it has seen of the producers' writes the epilogue sees
-        mbar_init(&sh.a_ready, 8);
-        mbar_init(&sh.p2_full, 1);
+        mbar_init(&sh.dy_known, kCkProducers);
+        mbar_init(&sh.dh_full, 2);  // the products, and the MMA lane itself: what it has seen of the producers' writes the epilogue sees
+        mbar_init(&sh.pre_full, 1);
+        mbar_init(&sh.dh_ready, 8);
+        mbar_init(&sh.pre_ready, 8);
+        mbar_init(&sh.g1_full, 1);
+        mbar_init(&sh.g2_full, 1);
         sh.abort = 0;
         mbar_fence_init();
     }
@@ -537,28 +566,33 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
                 umma_f16(dh, w2h + 2 * ks, dyl + 2 * ks, id, 1);
             }
             for (int ks = 0; ks < ks2; ++ks) umma_f16(dh, w2h + 2 * ks, dyh + 2 * ks, id, 1);
+            umma_commit(&sh.dh_full);
+            mbar_arrive(&sh.dh_full);
             for (int ks = 0; ks < ks1; ++ks) umma_f16(pre, w1l + k(ks), zk + k(ks), id, ks != 0);
             for (int ks = 0; ks < ks1; ++ks) umma_f16(pre, w1h + k(ks), zk + k(ks), id, 1);
-            umma_commit(&sh.p1_full);
-            mbar_arrive(&sh.p1_full);
+            umma_commit(&sh.pre_full);
             return true;
         };
         auto after = [&](int t) -> bool {  // the sums over its rows
-            if (!umma_wait(&sh.a_ready, t & 1, &sh.abort)) return false;  // which also says that tile t - 1 has left its accumulators
+            if (!umma_wait(&sh.dh_ready, t & 1, &sh.abort)) return false;  // which also says that tile t - 1 has left its accumulators
             tc_fence_after();
             const unsigned pre = tmem + kCkPreCol, dh = tmem + kCkDhCol, g1 = tmem + kCkW1Col, g2 = tmem + kCkW2Col;
             for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks + 8, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, ks != 0);
             for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, 1);
+            umma_commit(&sh.g1_full);
+            if (!umma_wait(&sh.pre_ready, t & 1, &sh.abort)) return false;
+            tc_fence_after();
             for (int ks = 0; ks < 8; ++ks) {
                 umma_f16_ts(g2, pre + 16 * ks + 8, umma_desc_rows(dy0 + 2048 * ks, kCkTile), id2, ks != 0);
                 umma_f16_ts(g2, pre + 16 * ks, umma_desc_rows(dy0 + kCkTile + 2048 * ks, kCkTile), id2, 1);
             }
             for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g2, pre + 16 * ks, umma_desc_rows(dy0 + 2048 * ks, kCkTile), id2, 1);
             umma_commit(&sh.op_empty);
-            umma_commit(&sh.p2_full);
+            umma_commit(&sh.g2_full);
             return true;
         };
         const int first = (warp - kCkProducer0) * 32, groups = (a.in + 31) / 32, units = a.pitch / 16;  // units of 16 codes in a row
+        const unsigned per_unit = 65535u / units + 1;  // q / units = q * per_unit >> 16 for q < 352
         DyRows<TWO> rows;
         uint4 mask;
         constexpr int kUnits = 11;
@@ -588,9 +622,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             rows.load(a, row0, lane);
             mask = row0 + lane < a.rows ? __ldg(a.mask + row0 + lane) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < kUnits; ++i) {  // unit u of a row to 32 / ... lanes: flat, so that lines are read whole
+            for (int i = 0; i < kUnits; ++i) {  // flat, so that lines are read whole
                 const int q = i * 32 + lane;
-                code[i] = q < 32 * units && row0 + q / units < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.codes + row0 * a.pitch) + q) : make_uint4(0, 0, 0, 0);
+                code[i] = q < 32 * units && row0 + (q * per_unit >> 16) < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.codes + row0 * a.pitch) + q) : make_uint4(0, 0, 0, 0);
             }
         };
         if (ntile > 0) load(0);
@@ -601,20 +635,34 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             for (int i = 0; i < kWords; ++i) most = __vmaxu4(most, exps[i] & ~__vcmpeq4(exps[i], 0xffffffffu));
             most = __vmaxu4(most, most >> 16);
             const int largest = (int)warp_max(max(most & 0xffu, most >> 8 & 0xffu));
+            // and the largest of dy, from the four of them (the sums over its rows want one unit, and dh is as good in it)
+            const unsigned mine = rows.largest();
+            if (lane == 0) {
+                sh.dy_most[t & 1][warp - kCkProducer0] = mine;
+                mbar_arrive(&sh.dy_known);
+            }
+            if (!(ok = umma_wait(&sh.dy_known, t & 1, &sh.abort))) break;
+            unsigned field = 0;
+#pragma unroll
+            for (int q = 0; q < kCkProducers; ++q) field = max(field, sh.dy_most[t & 1][q]);
+            field = row_unit(field);
             if (!(ok = umma_wait(&sh.op_empty, (t & 1) ^ 1, &sh.abort))) break;
-            rows.store(dyt, dyt + kCkTile, sh.units, first, lane);
+            rows.store(dyt, dyt + kCkTile, from_row_unit(field), first, lane);
             sh.mask[0][first + lane] = mask.x;
             sh.mask[1][first + lane] = mask.y;
             sh.mask[2][first + lane] = mask.z;
             sh.mask[3][first + lane] = mask.w;
-            if (warp == kCkProducer0 && lane == 0) sh.z_unit = largest - 133 - 8;
+            if (warp == kCkProducer0 && lane == 0) {
+                sh.z_unit = largest - 133 - 8;
+                sh.dy_unit = (int)field - 127;
+            }
             // (every warp writes the same bytes, and reads its own)
 #pragma unroll
             for (int i = 0; i < kWords; ++i) reinterpret_cast<unsigned *>(sh.exponents)[i * 32 + lane] = exps[i];
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                const int q = i * 32 + lane, row = q / units, u = q - row * units;
+                const int q = i * 32 + lane, row = q * per_unit >> 16, u = q - row * units;
                 if (row >= 32) continue;
                 const int e = sh.exponents[(first + row) * groups + u / 2];
                 const int d = e - largest + 8;  // (e of a group that is not finite lies above)
@@ -657,63 +705,63 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             for (int j = 0; j < 16; ++j) sums[b][j] = 0.f;
 #pragma unroll 1
         for (int t = 0; t < ntile; ++t) {
-            if (!(ok = umma_wait(&sh.p1_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
+            if (!(ok = umma_wait(&sh.dh_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
             tc_fence_after();
-            // rows' units relative to the largest of the tile: a warp makes those of its half
-            int unit = -126;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) unit = max(unit, sh.units[32 * q + lane]);
-            unit = __reduce_max_sync(kFull, unit);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) sh.factor[warp][32 * q + lane] = power_of_two(sh.units[64 * half + 32 * q + lane] - unit);
-            __syncwarp();
-            // units: zh 2^zu, W1 2^w1; h in units of 2^hu, which the largest sum (176 x 2 x 32512 in the accumulator's) and bias leave below 2^15
-            const int zu = sh.z_unit, hu = max(zu + head.w1 + 24, head.b1 + 2) - 15;
-            const float to_h = power_of_two(max(zu + head.w1 - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
-            float partial[4] = {};
             const unsigned bit = 1u << lane;
+            // masks rows 64 half .. + 63 of an accumulator (lane = hidden unit) and takes them apart
+            auto apart = [&](unsigned at, auto value) {
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                const int at = 64 * half + 16 * c;
-                unsigned rd[16], rp[16], parts[16];
-                tmem_ld16(tlane + kCkDhCol + at, rd);
-                tmem_ld16(tlane + kCkPreCol + at, rp);
-                tc_wait_ld();
+                for (int c = 0; c < 4; ++c) {
+                    const int row = 64 * half + 16 * c;
+                    unsigned r[16], parts[16];
+                    tmem_ld16(at + row, r);
+                    tc_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const uint4 m = *reinterpret_cast<const uint4 *>(&sh.mask[quarter][at + j]);
-                    const float4 f = *reinterpret_cast<const float4 *>(&sh.factor[warp][16 * c + j]);
-                    const unsigned mw[4] = {m.x, m.y, m.z, m.w};
-                    const float fw[4] = {f.x, f.y, f.z, f.w};
-                    float v[4];
+                    for (int j = 0; j < 16; j += 4) {
+                        const uint4 m = *reinterpret_cast<const uint4 *>(&sh.mask[quarter][row + j]);
+                        const unsigned mw[4] = {m.x, m.y, m.z, m.w};
+                        float v[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        v[q] = mw[q] & bit ? __uint_as_float(rd[j + q]) * fw[q] : 0.f;
-                        rp[j + q] = __float_as_uint(mw[q] & bit ? __fmaf_rn(__uint_as_float(rp[j + q]), to_h, bias) * fw[q] : 0.f);
-                        partial[q] += v[q];
+                        for (int q = 0; q < 4; ++q) v[q] = value(__uint_as_float(r[j + q]), (mw[q] & bit) != 0, q);
+                        split_halves(v[0], v[1], parts[j / 2], parts[8 + j / 2]);
+                        split_halves(v[2], v[3], parts[j / 2 + 1], parts[8 + j / 2 + 1]);
                     }
-                    split_halves(v[0], v[1], parts[j / 2], parts[8 + j / 2]);
-                    split_halves(v[2], v[3], parts[j / 2 + 1], parts[8 + j / 2 + 1]);
+                    tmem_st16(at + row, parts);
                 }
-                tmem_st16(tlane + kCkDhCol + at, parts);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) split_halves(__uint_as_float(rp[2 * j]), __uint_as_float(rp[2 * j + 1]), parts[j], parts[8 + j]);
-                tmem_st16(tlane + kCkPreCol + at, parts);
-            }
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.a_ready);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+            };
+            float partial[4] = {};
+            apart(tlane + kCkDhCol, [&](float v, bool alive, int q) {
+                v = alive ? v : 0.f;
+                partial[q] += v;
+                return v;
+            });
+            if (lane == 0) mbar_arrive(&sh.dh_ready);
+            // units: zh 2^zu, W1 2^w1; h in units of 2^hu, which the largest sum (176 x 2 x 32512 in the accumulator's) and bias leave below 2^15
+            const int unit = sh.dy_unit, zu = sh.z_unit, hu = max(zu + head.w1 + 24, head.b1 + 2) - 15;
+            const float to_h = power_of_two(max(zu + head.w1 - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
+            if (!(ok = umma_wait(&sh.pre_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
+            tc_fence_after();
+            apart(tlane + kCkPreCol, [&](float v, bool alive, int) { return alive ? __fmaf_rn(v, to_h, bias) : 0.f; });
+            if (lane == 0) mbar_arrive(&sh.pre_ready);
             // what the tile's sums are multiples of: products of powers of two, zero where they fall below the smallest number
             auto scale = [](int e) { return power_of_two(max(min(e, 127), -126)) * power_of_two(max(min(e + 126, 0), -126)); };
             db += (partial[0] + partial[1] + (partial[2] + partial[3])) * scale(unit + head.w2);
-            if (!(ok = umma_wait(&sh.p2_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
+            if (!(ok = umma_wait(&sh.g1_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
             tc_fence_after();
+            bool both = false;  // dW2's sums are there as well
             const float f1 = scale(unit + head.w2 + zu), f2 = scale(unit + hu);
 #pragma unroll
             for (int i = 0; i < kBlocks; ++i) {
                 const int b = 2 * i + half;
                 if (b >= nb) break;
+                if (b >= nb1 && !both) {
+                    if (!(ok = umma_wait(&sh.g2_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
+                    tc_fence_after();
+                    both = true;
+                }
                 unsigned r[16];
                 tmem_ld16(tlane + (b < nb1 ? kCkW1Col + 16 * b : kCkW2Col + 16 * (b - nb1)), r);
                 tc_wait_ld();
@@ -722,6 +770,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
                 for (int j = 0; j < 16; ++j) sums[i][j] = __fmaf_rn(__uint_as_float(r[j]), f, sums[i][j]);
             }
             tc_fence_before();
+            if (!ok) break;
         }
         if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_EPILOGUE);
         // db1 in column `in`: both halves of the rows through shared memory.  (A warp that gave up comes here as well: the barriers want all.)
@@ -1182,7 +1231,7 @@ int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, con
     a.tiles = (int)((rows + kCkRows - 1) / kCkRows);
     if (!(a.status = umma_status_word())) return fail(NPA_ERR_CUDA, "%s: no status word", me);
     const bool two = out_dim > 32;
-    if (dz && (rc = ck_launch(two ? mlp_checkpoint_dz_kernel<true> : mlp_checkpoint_dz_kernel<false>, "mlp_checkpoint_dz_kernel", a, ck_dz_smem(a.chunks), r.ctas, st)) !=
+    if (dz && (rc = ck_launch(two ? mlp_checkpoint_dz_kernel<true> : mlp_checkpoint_dz_kernel<false>, "mlp_checkpoint_dz_kernel", a, ck_dz_smem(a.chunks, in_dim), r.ctas, st)) !=
                   NPA_OK)
         return rc;
     if (!dW1) return NPA_OK;
