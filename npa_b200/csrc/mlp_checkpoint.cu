@@ -158,6 +158,13 @@ __device__ constexpr unsigned f16_idesc(int n, bool rows_b) {
     return (1u << 4) | (rows_b ? 1u << 16 : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(128 >> 4) << 24);
 }
 
+// What is worked out from `v` behind this is worked out again in every round of a loop: dozens of addresses kept over the tiles would
+// take the registers of what is under way, and a spilled register comes back from L2 (shared memory leaves no L1).
+__device__ __forceinline__ int worked_out_here(int v) {
+    asm volatile("" : "+r"(v));
+    return v;
+}
+
 struct CkArgs {
     const int8_t *codes;
     const uint8_t *exponents;
@@ -187,21 +194,21 @@ struct DyRows {
     static constexpr int kEach = TWO ? 1 : 2, kPasses = 32 / kEach;  // rows a pass
     float2 v[kPasses];
     __device__ __forceinline__ void load(const CkArgs &a, long long row0, int lane) {
-        const int k = TWO ? 2 * lane : 2 * (lane & 15), r0 = TWO ? 0 : lane >> 4;
+        const int k = TWO ? 2 * lane : 2 * (lane & 15), r0 = TWO ? 0 : lane >> 4, out = worked_out_here(a.out);
         const float *p = a.dy + (row0 + r0) * a.out + k;
         const int rows = a.rows - row0 < 32 ? (int)(a.rows - row0) : 32;
         const bool one = k < a.out, two = k + 1 < a.out;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
             const bool there = r0 + i * kEach < rows;
-            v[i].x = there && one ? __ldg(p + i * kEach * a.out) : 0.f;
-            v[i].y = there && two ? __ldg(p + i * kEach * a.out + 1) : 0.f;
+            v[i].x = there && one ? __ldg(p + i * kEach * out) : 0.f;
+            v[i].y = there && two ? __ldg(p + i * kEach * out + 1) : 0.f;
         }
     }
     __device__ __forceinline__ void put(uint8_t *heads, uint8_t *tails, int first, int i, float scale, int lane) const {
         unsigned head, tail;
         split_halves(v[i].x * scale, v[i].y * scale, head, tail);
-        const int place = half_place(first + (TWO ? 0 : lane >> 4) + i * kEach, TWO ? 2 * lane : 2 * (lane & 15));
+        const int place = half_place(first + (TWO ? 0 : lane >> 4) + i * kEach, TWO ? 2 * lane : 2 * (lane & 15));  // (`first` is a multiple of 32)
         if (!TWO || lane < 24) {
             *reinterpret_cast<unsigned *>(heads + place) = head;
             *reinterpret_cast<unsigned *>(tails + place) = tail;
@@ -396,18 +403,22 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             const int at = t * turns + quarter / buffers;
             if (!umma_wait(&sh.copied[mine], (at & 1) ^ 1, &sh.abort)) return false;
             float *row = stg + lane * a.in;
-#pragma unroll 1
-            for (int c0 = 16 * half; c0 < a.in; c0 += 32) {
+            auto block = [&](int c0, auto full) {
                 unsigned r[16];
                 tmem_ld16(tlane + kCkDzCol + c0, r);
                 tc_wait_ld();
+                if (far) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    float v = __uint_as_float(r[j]) * unit;
-                    if (far) v *= rest;
-                    if (c0 + j < a.in) row[c0 + j] = v;
+                    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * rest);
                 }
-            }
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (decltype(full)::value || c0 + j < a.in) row[c0 + j] = __uint_as_float(r[j]) * unit;
+            };
+            int c0 = 16 * half;
+#pragma unroll 1
+            for (; c0 + 16 <= a.in; c0 += 32) block(c0, std::true_type());
+            if (c0 < a.in) block(c0, std::false_type());
             tc_fence_before();
             fence_proxy_async();  // the copy reads these
             __syncwarp();
@@ -546,12 +557,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         // the first of the producers issues the MMAs as well (one lane): the operands have one buffer, so it would wait for them anyway
         const bool issues = warp == kCkProducer0;
         if (issues && lane == 0) ck_copy_image(base, a, &sh.image);
-        const int n1 = (a.in + 15) / 16 * 16, n2 = (a.out + 15) / 16 * 16, ks1 = n1 / 16, ks2 = n2 / 16;
-        const unsigned id = f16_idesc(128, false), id1 = f16_idesc(n1, true), id2 = f16_idesc(n2, true);
-        const uint64_t w1h = umma_desc(smem_u32(base)), w1l = umma_desc(smem_u32(base + a.chunks * kCkTile));
-        const uint64_t w2h = umma_desc(smem_u32(w2)), w2l = umma_desc(smem_u32(w2 + kCkTile));
-        const uint64_t zk = umma_desc(smem_u32(zt)), dyh = umma_desc(smem_u32(dyt)), dyl = umma_desc(smem_u32(dyt + kCkTile));
-        const unsigned z0 = smem_u32(zt), dy0 = smem_u32(dyt);
+        // (operands are described where they are used: kept over the loop they would cost the producers their registers, and a spilled
+        // register comes back from L2)
+        const int chunks = a.chunks;
         // MMAs into one accumulator follow one another: changing it after each costs half as much again (zh W1^T and dh in turn 5,000 clocks
         // instead of 3,400 at 163 inputs and 35 outputs).
         auto before = [&](int t) -> bool {  // dh and zh W1^T of tile t
@@ -559,6 +567,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             if (!umma_wait(&sh.op_full, t & 1, &sh.abort)) return false;
             tc_fence_after();
             // (the A operands of tile t - 1 lay where these go: the producers have waited for its products)
+            const int ks1 = (a.in + 15) / 16, ks2 = (a.out + 15) / 16;
+            const unsigned id = f16_idesc(128, false);
+            const uint64_t w1h = umma_desc(smem_u32(base)), w1l = umma_desc(smem_u32(base + chunks * kCkTile));
+            const uint64_t w2h = umma_desc(smem_u32(w2)), w2l = umma_desc(smem_u32(w2 + kCkTile));
+            const uint64_t zk = umma_desc(smem_u32(zt)), dyh = umma_desc(smem_u32(dyt)), dyl = umma_desc(smem_u32(dyt + kCkTile));
             auto k = [](int ks) { return (uint64_t)((ks >> 2) * (kCkTile >> 4) + 2 * (ks & 3)); };  // 16 columns further
             const unsigned pre = tmem + kCkPreCol, dh = tmem + kCkDhCol;
             for (int ks = 0; ks < ks2; ++ks) {
@@ -577,6 +590,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             if (!umma_wait(&sh.dh_ready, t & 1, &sh.abort)) return false;  // which also says that tile t - 1 has left its accumulators
             tc_fence_after();
             const unsigned pre = tmem + kCkPreCol, dh = tmem + kCkDhCol, g1 = tmem + kCkW1Col, g2 = tmem + kCkW2Col;
+            const unsigned id1 = f16_idesc((a.in + 15) / 16 * 16, true), id2 = f16_idesc((a.out + 15) / 16 * 16, true);
+            const unsigned z0 = smem_u32(zt), dy0 = smem_u32(dyt);
             for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks + 8, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, ks != 0);
             for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, 1);
             umma_commit(&sh.g1_full);
@@ -621,11 +636,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             }
             rows.load(a, row0, lane);
             mask = row0 + lane < a.rows ? __ldg(a.mask + row0 + lane) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < kUnits; ++i) {  // flat, so that lines are read whole
-                const int q = i * 32 + lane;
-                code[i] = q < 32 * units && row0 + (q * per_unit >> 16) < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.codes + row0 * a.pitch) + q) : make_uint4(0, 0, 0, 0);
-            }
         };
         if (ntile > 0) load(0);
 #pragma unroll 1
@@ -647,6 +657,15 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             for (int q = 0; q < kCkProducers; ++q) field = max(field, sh.dy_most[t & 1][q]);
             field = row_unit(field);
             if (!(ok = umma_wait(&sh.op_empty, (t & 1) ^ 1, &sh.abort))) break;
+            {  // (on their way while dy is stored; a tile ahead there is no room for them)
+                const long long row0 = row_of(t) + first;
+                const int lane0 = worked_out_here(lane);
+#pragma unroll
+                for (int i = 0; i < kUnits; ++i) {  // flat, so that lines are read whole
+                    const int q = i * 32 + lane0;
+                    code[i] = q < 32 * units && row0 + (q * per_unit >> 16) < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.codes + row0 * a.pitch) + q) : make_uint4(0, 0, 0, 0);
+                }
+            }
             rows.store(dyt, dyt + kCkTile, from_row_unit(field), first, lane);
             sh.mask[0][first + lane] = mask.x;
             sh.mask[1][first + lane] = mask.y;
@@ -660,9 +679,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
 #pragma unroll
             for (int i = 0; i < kWords; ++i) reinterpret_cast<unsigned *>(sh.exponents)[i * 32 + lane] = exps[i];
             __syncwarp();
+            const int lane0 = worked_out_here(lane);
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                const int q = i * 32 + lane, row = q * per_unit >> 16, u = q - row * units;
+                const int q = i * 32 + lane0, row = q * per_unit >> 16, u = q - row * units;
                 if (row >= 32) continue;
                 const int e = sh.exponents[(first + row) * groups + u / 2];
                 const int d = e - largest + 8;  // (e of a group that is not finite lies above)
@@ -805,7 +825,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
 // additions at 163 inputs instead of 33), which four epilogue warps add; h goes back in heads and tails in place, in units that no row
 // can exceed: with z in units of its row, W1 of its matrix and the largest bias known, a bound is at hand, and 2^-25 below it is float16's
 // smallest tail.  The second layer's sums take the place of the products with tails.
-constexpr int kFwProducers = 16, kFwEpilogue0 = 16, kFwWarpMma = 20, kFwThreads = 21 * 32;
+constexpr int kFwProducers = 16, kFwThreads = 20 * 32;  // (twenty warps: 96 registers a thread; one more would cost 16 of them)
 constexpr int kFwSlot = 2 * kCkTile, kFwSlots = 2;
 struct CkForwardShared {
     uint64_t image, slot_full[kFwSlots], slot_empty[kFwSlots], h_full[2], h_ready[2], y_full[2], y_read[2], y_written, y_copied;
@@ -854,7 +874,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
         mbar_fence_init();
     }
     if (threadIdx.x < 128) sh.b1[threadIdx.x] = __ldg(a.b1 + threadIdx.x);
-    if (warp == kFwWarpMma) {
+    if (warp == kFwProducers) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -866,68 +886,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
     auto row_of = [&](int it) { return ((long long)blockIdx.x + (long long)it * gridDim.x) * kCkRows; };
     bool ok = true;
 
-    if (warp == kFwWarpMma) {
-        if (lane == 0) {
-            const int tiles = 2 * kChunks + 2;
-            mbar_arrive_expect(&sh.image, (unsigned)(tiles * kCkTile));
-            for (int q = 0; q < tiles; ++q) bulk_copy_g2s(base + q * kCkTile, a.image + kCkHeader + (long long)q * kCkTile, kCkTile, &sh.image);
-            const unsigned id1 = f16_idesc(128, false), id2 = f16_idesc((a.out + 15) / 16 * 16, true);
-            const uint64_t w1h = umma_desc(smem_u32(base)), w1l = umma_desc(smem_u32(base + kChunks * kCkTile));
-            const unsigned w2h = smem_u32(w2), w2l = smem_u32(w2 + kCkTile);
-            const int steps = (a.in + 15) / 16;
-            auto second = [&](int t) -> bool {
-                const int b = t & 1;
-                if (!umma_wait(&sh.h_ready[b], (t >> 1) & 1, &sh.abort)) return false;
-                tc_fence_after();
-                const unsigned d = tmem + 256 + 128 * b, ah = tmem + 128 * b;
-                for (int ks = 0; ks < 8; ++ks) {
-                    umma_f16_ts(d, ah + 16 * ks + 8, umma_desc_rows(w2h + 2048 * ks, kCkTile), id2, ks != 0);
-                    umma_f16_ts(d, ah + 16 * ks, umma_desc_rows(w2l + 2048 * ks, kCkTile), id2, 1);
-                }
-                for (int ks = 0; ks < 8; ++ks) umma_f16_ts(d, ah + 16 * ks, umma_desc_rows(w2h + 2048 * ks, kCkTile), id2, 1);
-                umma_commit(&sh.y_full[b]);
-                return true;
-            };
-            ok = umma_wait(&sh.image, 0, &sh.abort);
-            int s = 0;
-            unsigned ph = 0;
-#pragma unroll 1
-            for (int t = 0; t < ntile && ok; ++t) {
-                const int b = t & 1;
-                if (!(ok = umma_wait(&sh.y_read[b], ((t >> 1) & 1) ^ 1, &sh.abort))) break;  // y of tile t - 2: nothing of it is left
-                tc_fence_after();
-                const unsigned d = tmem + 128 * b, small = tmem + 256 + 128 * b;
-#pragma unroll 1
-                for (int c = 0; c < kChunks; ++c) {
-                    if (!(ok = umma_wait(&sh.slot_full[s], ph, &sh.abort))) break;
-                    tc_fence_after();
-                    const uint64_t zh = umma_desc(smem_u32(ring + s * kFwSlot)), zl = umma_desc(smem_u32(ring + s * kFwSlot + kCkTile));
-                    const uint64_t wh = w1h + (uint64_t)(c * (kCkTile >> 4)), wl = w1l + (uint64_t)(c * (kCkTile >> 4));
-                    const int here = min(4, steps - 4 * c);
-                    for (int ks = 0; ks < here; ++ks) {
-                        umma_f16(small, zl + 2 * ks, wh + 2 * ks, id1, (c | ks) != 0);
-                        umma_f16(small, zh + 2 * ks, wl + 2 * ks, id1, 1);
-                    }
-                    for (int ks = 0; ks < here; ++ks) umma_f16(d, zh + 2 * ks, wh + 2 * ks, id1, (c | ks) != 0);
-                    umma_commit(&sh.slot_empty[s]);
-                    if (++s == kFwSlots) {
-                        s = 0;
-                        ph ^= 1;
-                    }
-                }
-                if (!ok) break;
-                umma_commit(&sh.h_full[b]);
-                mbar_arrive(&sh.h_full[b]);
-                if (t > 0) ok = second(t - 1);
-            }
-            if (ok && ntile > 0) ok = second(ntile - 1);
-            if (!ok) {
-                atomicOr(a.status, CK_STATUS_MMA);
-                __nanosleep(20000);  // copies in flight land before the CTA leaves
-            }
-        }
-        __syncwarp();
-    } else if (warp < kFwProducers) {
+    if (warp < kFwProducers) {
         const int first = warp * 8, groups = (a.in + 31) / 32;
         // place of (row r, columns 2 lane, 2 lane + 1) in a slot: units of eight columns change places by the row's lowest three bits
         const int word = (lane & 3) * 4;
@@ -939,12 +898,13 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
             float2 v[8][kChunks];
             unsigned row_most[8];
             {
-                const int k = 64 * (kChunks - 1) + 2 * lane;
+                const int k = 64 * (kChunks - 1) + 2 * lane, in = worked_out_here(a.in);
                 const bool one = k < a.in, two = k + 1 < a.in;
+                const float *p0 = a.z + (row0 < a.rows ? row0 : a.rows - 1) * a.in + 2 * lane;
+                const int last = (int)(a.rows - 1 - row0 < 7 ? max((int)(a.rows - 1 - row0), 0) : 7);
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
-                    // (a row that does not exist is read as the last one: nothing of it leaves)
-                    const float *p = a.z + (row0 + r < a.rows ? row0 + r : a.rows - 1) * a.in + 2 * lane;
+                    const float *p = p0 + min(r, last) * in;  // (a row that does not exist is read as the last one: nothing of it leaves)
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c) {
                         v[r][c].x = c + 1 < kChunks || one ? __ldg(p + 64 * c) : 0.f;
@@ -977,7 +937,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                     f = gather_max8<16>(m);
                 }
                 own = max(own, max(f, __shfl_xor_sync(kFull, f, 16)));
-                const int k = 64 * c + 2 * lane;
+                const int k = 64 * c + 2 * lane, pitch = worked_out_here(a.pitch);
                 auto put = [&](auto clamp) {
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
@@ -987,7 +947,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                             x = (unsigned)rows8_code(v[r][c].x, u);
                             y = (unsigned)rows8_code(v[r][c].y, u);
                         }
-                        if (k < a.pitch) *reinterpret_cast<uint16_t *>((r < 5 ? low + r * a.pitch : high + (r - 5) * a.pitch) + k) = (uint16_t)__byte_perm(x, y, 0x0040);
+                        if (k < pitch) *reinterpret_cast<uint16_t *>((r < 5 ? low + r * pitch : high + (r - 5) * pitch) + k) = (uint16_t)__byte_perm(x, y, 0x0040);
                     }
                 };
                 if (__any_sync(kFull, e >= 254u)) put(std::true_type());  // up to 128 units in the last binade, or groups that are not finite
@@ -1042,6 +1002,59 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
         if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_PRODUCER);
     } else {
         const int quarter = warp & 3, row = quarter * 32 + lane;
+        // a lane of the first warp issues the MMAs as well: while the producers fill the slots there is little else for it to do
+        const bool issues = quarter == 0;
+        if (issues && lane == 0) {
+            const int tiles = 2 * kChunks + 2;
+            mbar_arrive_expect(&sh.image, (unsigned)(tiles * kCkTile));
+            for (int q = 0; q < tiles; ++q) bulk_copy_g2s(base + q * kCkTile, a.image + kCkHeader + (long long)q * kCkTile, kCkTile, &sh.image);
+        }
+        auto first_layer = [&](int t) -> bool {
+            const int b = t & 1, steps = (a.in + 15) / 16;
+            const unsigned id1 = f16_idesc(128, false);
+            const uint64_t w1h = umma_desc(smem_u32(base)), w1l = umma_desc(smem_u32(base + kChunks * kCkTile));
+            if (t == 0 && !umma_wait(&sh.image, 0, &sh.abort)) return false;
+            if (!umma_wait(&sh.y_read[b], ((t >> 1) & 1) ^ 1, &sh.abort)) return false;  // y of tile t - 2: nothing of it is left
+            tc_fence_after();
+            const unsigned d = tmem + 128 * b, small = tmem + 256 + 128 * b;
+            int q = t * kChunks;
+#pragma unroll 1
+            for (int c = 0; c < kChunks; ++c, ++q) {
+                const int s = q % kFwSlots;
+                if (!umma_wait(&sh.slot_full[s], (q / kFwSlots) & 1, &sh.abort)) return false;
+                tc_fence_after();
+                const uint64_t zh = umma_desc(smem_u32(ring + s * kFwSlot)), zl = umma_desc(smem_u32(ring + s * kFwSlot + kCkTile));
+                const uint64_t wh = w1h + (uint64_t)(c * (kCkTile >> 4)), wl = w1l + (uint64_t)(c * (kCkTile >> 4));
+                const int here = min(4, steps - 4 * c);
+                for (int ks = 0; ks < here; ++ks) {
+                    umma_f16(small, zl + 2 * ks, wh + 2 * ks, id1, (c | ks) != 0);
+                    umma_f16(small, zh + 2 * ks, wl + 2 * ks, id1, 1);
+                }
+                for (int ks = 0; ks < here; ++ks) umma_f16(d, zh + 2 * ks, wh + 2 * ks, id1, (c | ks) != 0);
+                umma_commit(&sh.slot_empty[s]);
+            }
+            umma_commit(&sh.h_full[b]);
+            mbar_arrive(&sh.h_full[b]);
+            return true;
+        };
+        auto second_layer = [&](int t) -> bool {
+            const int b = t & 1;
+            const unsigned id2 = f16_idesc((a.out + 15) / 16 * 16, true), w2h = smem_u32(w2), w2l = smem_u32(w2 + kCkTile);
+            if (!umma_wait(&sh.h_ready[b], (t >> 1) & 1, &sh.abort)) return false;
+            tc_fence_after();
+            const unsigned d = tmem + 256 + 128 * b, ah = tmem + 128 * b;
+            for (int ks = 0; ks < 8; ++ks) {
+                umma_f16_ts(d, ah + 16 * ks + 8, umma_desc_rows(w2h + 2048 * ks, kCkTile), id2, ks != 0);
+                umma_f16_ts(d, ah + 16 * ks, umma_desc_rows(w2l + 2048 * ks, kCkTile), id2, 1);
+            }
+            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(d, ah + 16 * ks, umma_desc_rows(w2h + 2048 * ks, kCkTile), id2, 1);
+            umma_commit(&sh.y_full[b]);
+            return true;
+        };
+        auto issue = [&](bool did) {  // what lane 0 says goes for the warp
+            did = __shfl_sync(kFull, (int)did, 0) != 0;
+            return did;
+        };
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
         const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
         // h is below 2^(zr + w1 + 10) by its products (176 of numbers below 2 x 2) and 2^(b1 + 1) by its bias: twice 2^14 of its units
@@ -1083,6 +1096,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
 #pragma unroll 1
         for (int t = 0; t < ntile; ++t) {
             const int b = t & 1;
+            if (issues && !(ok = issue(lane != 0 || first_layer(t)))) break;
             if (!(ok = umma_wait(&sh.h_full[b], (t >> 1) & 1, &sh.abort))) break;
             tc_fence_after();
             const int hu = unit_of(t);
@@ -1120,17 +1134,19 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.h_ready[b]);
+            if (issues && !(ok = issue(lane != 0 || second_layer(t)))) break;
             const long long at = row_of(t) + row;
             if (at < a.rows) reinterpret_cast<uint4 *>(a.mask)[at] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
             if (t > 0 && !(ok = leave(t - 1))) break;
         }
         if (ok && ntile > 0) ok = leave(ntile - 1);
+        if (!ok && issues && lane == 0) __nanosleep(20000);  // copies in flight land before the CTA leaves
         if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_EPILOGUE);
     }
 
     tc_fence_before();
     __syncthreads();
-    if (warp == kFwWarpMma) {
+    if (warp == kFwProducers) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
