@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
 // of the sums over the tile's rows.  The bits of 32 units and a row are one word, the same for a warp.  A tile's sums leave the
 // accumulators with the tile's unit and are added in 32 bits, in registers: up to 7 blocks of 16 columns a thread (kBlocks).
 struct CkWeightsShared {
-    uint64_t image, op_full, op_empty, dy_known, dh_full, pre_full, dh_ready, pre_ready, g1_full, g2_full;
+    uint64_t image, op_full, z_empty, dy_empty, dy_known, dh_full, pre_full, dh_ready, pre_ready, g1_full, g2_full;
     alignas(16) unsigned mask[4][kCkRows];
     unsigned dy_most[2][kCkProducers];     // of two tiles: largest finite magnitude of each producer's rows
     int dy_unit;
@@ -530,7 +530,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
     if (threadIdx.x == 0) {
         mbar_init(&sh.image, 1);
         mbar_init(&sh.op_full, kCkProducers);
-        mbar_init(&sh.op_empty, 1);
+        mbar_init(&sh.z_empty, 1);
+        mbar_init(&sh.dy_empty, 1);
         mbar_init(&sh.dy_known, kCkProducers);
         mbar_init(&sh.dh_full, 2);  // the products, and the MMA lane itself: what it has seen of the producers' writes the epilogue sees
         mbar_init(&sh.pre_full, 1);
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
     bool ok = true;
 
     if (warp >= kCkProducer0) {
-        // the first of the producers issues the MMAs as well (one lane): the operands have one buffer, so it would wait for them anyway
+        // the first of the producers issues the products that make the A operands (one lane)
         const bool issues = warp == kCkProducer0;
         if (issues && lane == 0) ck_copy_image(base, a, &sh.image);
         // (operands are described where they are used: kept over the loop they would cost the producers their registers, and a spilled
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             if (t == 0 && !umma_wait(&sh.image, 0, &sh.abort)) return false;
             if (!umma_wait(&sh.op_full, t & 1, &sh.abort)) return false;
             tc_fence_after();
-            // (the A operands of tile t - 1 lay where these go: the producers have waited for its products)
+            // (the A operands of tile t - 1 lay where these go: the producers have waited for both of its sums)
             const int ks1 = (a.in + 15) / 16, ks2 = (a.out + 15) / 16;
             const unsigned id = f16_idesc(128, false);
             const uint64_t w1h = umma_desc(smem_u32(base)), w1l = umma_desc(smem_u32(base + chunks * kCkTile));
@@ -584,26 +585,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             for (int ks = 0; ks < ks1; ++ks) umma_f16(pre, w1l + k(ks), zk + k(ks), id, ks != 0);
             for (int ks = 0; ks < ks1; ++ks) umma_f16(pre, w1h + k(ks), zk + k(ks), id, 1);
             umma_commit(&sh.pre_full);
-            return true;
-        };
-        auto after = [&](int t) -> bool {  // the sums over its rows
-            if (!umma_wait(&sh.dh_ready, t & 1, &sh.abort)) return false;  // which also says that tile t - 1 has left its accumulators
-            tc_fence_after();
-            const unsigned pre = tmem + kCkPreCol, dh = tmem + kCkDhCol, g1 = tmem + kCkW1Col, g2 = tmem + kCkW2Col;
-            const unsigned id1 = f16_idesc((a.in + 15) / 16 * 16, true), id2 = f16_idesc((a.out + 15) / 16 * 16, true);
-            const unsigned z0 = smem_u32(zt), dy0 = smem_u32(dyt);
-            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks + 8, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, ks != 0);
-            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, 1);
-            umma_commit(&sh.g1_full);
-            if (!umma_wait(&sh.pre_ready, t & 1, &sh.abort)) return false;
-            tc_fence_after();
-            for (int ks = 0; ks < 8; ++ks) {
-                umma_f16_ts(g2, pre + 16 * ks + 8, umma_desc_rows(dy0 + 2048 * ks, kCkTile), id2, ks != 0);
-                umma_f16_ts(g2, pre + 16 * ks, umma_desc_rows(dy0 + kCkTile + 2048 * ks, kCkTile), id2, 1);
-            }
-            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g2, pre + 16 * ks, umma_desc_rows(dy0 + 2048 * ks, kCkTile), id2, 1);
-            umma_commit(&sh.op_empty);
-            umma_commit(&sh.g2_full);
             return true;
         };
         const int first = (warp - kCkProducer0) * 32, groups = (a.in + 31) / 32, units = a.pitch / 16;  // units of 16 codes in a row
@@ -636,6 +617,12 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             }
             rows.load(a, row0, lane);
             mask = row0 + lane < a.rows ? __ldg(a.mask + row0 + lane) : make_uint4(0, 0, 0, 0);
+            const int lane0 = worked_out_here(lane);
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {  // flat, so that lines are read whole
+                const int q = i * 32 + lane0;
+                code[i] = q < 32 * units && row0 + (q * per_unit >> 16) < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.codes + row0 * a.pitch) + q) : make_uint4(0, 0, 0, 0);
+            }
         };
         if (ntile > 0) load(0);
 #pragma unroll 1
@@ -645,36 +632,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             for (int i = 0; i < kWords; ++i) most = __vmaxu4(most, exps[i] & ~__vcmpeq4(exps[i], 0xffffffffu));
             most = __vmaxu4(most, most >> 16);
             const int largest = (int)warp_max(max(most & 0xffu, most >> 8 & 0xffu));
-            // and the largest of dy, from the four of them (the sums over its rows want one unit, and dh is as good in it)
-            const unsigned mine = rows.largest();
-            if (lane == 0) {
-                sh.dy_most[t & 1][warp - kCkProducer0] = mine;
-                mbar_arrive(&sh.dy_known);
-            }
-            if (!(ok = umma_wait(&sh.dy_known, t & 1, &sh.abort))) break;
-            unsigned field = 0;
-#pragma unroll
-            for (int q = 0; q < kCkProducers; ++q) field = max(field, sh.dy_most[t & 1][q]);
-            field = row_unit(field);
-            if (!(ok = umma_wait(&sh.op_empty, (t & 1) ^ 1, &sh.abort))) break;
-            {  // (on their way while dy is stored; a tile ahead there is no room for them)
-                const long long row0 = row_of(t) + first;
-                const int lane0 = worked_out_here(lane);
-#pragma unroll
-                for (int i = 0; i < kUnits; ++i) {  // flat, so that lines are read whole
-                    const int q = i * 32 + lane0;
-                    code[i] = q < 32 * units && row0 + (q * per_unit >> 16) < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.codes + row0 * a.pitch) + q) : make_uint4(0, 0, 0, 0);
-                }
-            }
-            rows.store(dyt, dyt + kCkTile, from_row_unit(field), first, lane);
-            sh.mask[0][first + lane] = mask.x;
-            sh.mask[1][first + lane] = mask.y;
-            sh.mask[2][first + lane] = mask.z;
-            sh.mask[3][first + lane] = mask.w;
-            if (warp == kCkProducer0 && lane == 0) {
-                sh.z_unit = largest - 133 - 8;
-                sh.dy_unit = (int)field - 127;
-            }
+            // zh, as soon as dW1's products of the tile before have read it (dW2's are still under way)
+            if (!(ok = umma_wait(&sh.z_empty, (t & 1) ^ 1, &sh.abort))) break;
+            if (t > 0 && !(ok = umma_wait(&sh.pre_full, (t - 1) & 1, &sh.abort))) break;  // and its own (another lane's, which no order binds to those)
             // (every warp writes the same bytes, and reads its own)
 #pragma unroll
             for (int i = 0; i < kWords; ++i) reinterpret_cast<unsigned *>(sh.exponents)[i * 32 + lane] = exps[i];
@@ -694,18 +654,35 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
                 *reinterpret_cast<uint4 *>(to + half_place(first + row, k)) = lo;
                 *reinterpret_cast<uint4 *>(to + half_place(first + row, k + 8)) = hi;
             }
+            // dy: the largest of the tile from the four of them (the sums over its rows want one unit, and dh is as good in it)
+            const unsigned mine = rows.largest();
+            if (lane == 0) {
+                sh.dy_most[t & 1][warp - kCkProducer0] = mine;
+                mbar_arrive(&sh.dy_known);
+            }
+            if (!(ok = umma_wait(&sh.dy_known, t & 1, &sh.abort))) break;
+            unsigned field = 0;
+#pragma unroll
+            for (int q = 0; q < kCkProducers; ++q) field = max(field, sh.dy_most[t & 1][q]);
+            field = row_unit(field);
+            if (!(ok = umma_wait(&sh.dy_empty, (t & 1) ^ 1, &sh.abort))) break;
+            rows.store(dyt, dyt + kCkTile, from_row_unit(field), first, lane);
+            sh.mask[0][first + lane] = mask.x;
+            sh.mask[1][first + lane] = mask.y;
+            sh.mask[2][first + lane] = mask.z;
+            sh.mask[3][first + lane] = mask.w;
+            if (warp == kCkProducer0 && lane == 0) {
+                sh.z_unit = largest - 133 - 8;
+                sh.dy_unit = (int)field - 127;
+            }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&sh.op_full);
                 if (issues) ok = before(t);
             }
-            __syncwarp();
+            ok = __shfl_sync(kFull, (int)ok, 0) != 0;
             if (t + 1 < ntile) load(t + 1);
-            if (issues) {
-                if (lane == 0) ok = ok && after(t);
-                ok = __shfl_sync(kFull, (int)ok, 0) != 0;
-            }
         }
         if (!ok && lane == 0) {
             atomicOr(a.status, issues ? CK_STATUS_MMA : CK_STATUS_PRODUCER);
@@ -716,6 +693,30 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         const int quarter = warp & 3, half = warp >> 2;  // hidden units 32 quarter + lane, rows 64 half .. + 63 of a tile
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
         const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
+        // a lane of the first warp issues the sums over the rows: it knows first that their operands are there
+        auto sums_of_w1 = [&](int t) -> bool {
+            if (!umma_wait(&sh.dh_ready, t & 1, &sh.abort)) return false;  // which also says that tile t - 1 has left its accumulators
+            tc_fence_after();
+            const unsigned dh = tmem + kCkDhCol, g1 = tmem + kCkW1Col, id1 = f16_idesc((a.in + 15) / 16 * 16, true), z0 = smem_u32(zt);
+            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks + 8, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, ks != 0);
+            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g1, dh + 16 * ks, umma_desc_rows(z0 + 2048 * ks, kCkTile), id1, 1);
+            umma_commit(&sh.z_empty);
+            umma_commit(&sh.g1_full);
+            return true;
+        };
+        auto sums_of_w2 = [&](int t) -> bool {
+            if (!umma_wait(&sh.pre_ready, t & 1, &sh.abort)) return false;
+            tc_fence_after();
+            const unsigned pre = tmem + kCkPreCol, g2 = tmem + kCkW2Col, id2 = f16_idesc((a.out + 15) / 16 * 16, true), dy0 = smem_u32(dyt);
+            for (int ks = 0; ks < 8; ++ks) {
+                umma_f16_ts(g2, pre + 16 * ks + 8, umma_desc_rows(dy0 + 2048 * ks, kCkTile), id2, ks != 0);
+                umma_f16_ts(g2, pre + 16 * ks, umma_desc_rows(dy0 + kCkTile + 2048 * ks, kCkTile), id2, 1);
+            }
+            for (int ks = 0; ks < 8; ++ks) umma_f16_ts(g2, pre + 16 * ks, umma_desc_rows(dy0 + 2048 * ks, kCkTile), id2, 1);
+            umma_commit(&sh.dy_empty);
+            umma_commit(&sh.g2_full);
+            return true;
+        };
         const float b1 = __ldg(a.b1 + quarter * 32 + lane);
         const int nb1 = (a.in + 15) / 16, nb = nb1 + (a.out + 15) / 16;
         float sums[kBlocks][16], db = 0.f;
@@ -758,14 +759,22 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
                 partial[q] += v;
                 return v;
             });
-            if (lane == 0) mbar_arrive(&sh.dh_ready);
+            if (lane == 0) {
+                mbar_arrive(&sh.dh_ready);
+                if (warp == 0) ok = sums_of_w1(t);
+            }
+            __syncwarp();
             // units: zh 2^zu, W1 2^w1; h in units of 2^hu, which the largest sum (176 x 2 x 32512 in the accumulator's) and bias leave below 2^15
             const int unit = sh.dy_unit, zu = sh.z_unit, hu = max(zu + head.w1 + 24, head.b1 + 2) - 15;
             const float to_h = power_of_two(max(zu + head.w1 - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
-            if (!(ok = umma_wait(&sh.pre_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
+            if (!umma_wait(&sh.pre_full, t & 1, &sh.abort, kUmmaWaitNs, 50)) ok = false;
             tc_fence_after();
             apart(tlane + kCkPreCol, [&](float v, bool alive, int) { return alive ? __fmaf_rn(v, to_h, bias) : 0.f; });
-            if (lane == 0) mbar_arrive(&sh.pre_ready);
+            if (lane == 0) {
+                mbar_arrive(&sh.pre_ready);
+                if (warp == 0) ok = ok && sums_of_w2(t);
+            }
+            if (!(ok = __shfl_sync(kFull, (int)ok, 0) != 0)) break;
             // what the tile's sums are multiples of: products of powers of two, zero where they fall below the smallest number
             auto scale = [](int e) { return power_of_two(max(min(e, 127), -126)) * power_of_two(max(min(e + 126, 0), -126)); };
             db += (partial[0] + partial[1] + (partial[2] + partial[3])) * scale(unit + head.w2);
