@@ -273,16 +273,27 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const __g
     __shared__ float scales[ROWS];
     __shared__ int sums[kFewWarps][NC * ROWS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pitch = (a.in + 15) / 16 * 16;
-    few_rows_codes<ROWS>(a, few_codes, pitch, scales);
-    __syncthreads();
     const int part = warp % share;  // `share` warps divide the length of their channels
     const int n0 = (blockIdx.x * (kFewWarps / share) + warp / share) * NC;
     int acc[NC][ROWS] = {};
     const int8_t *w[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) w[c] = a.w + (long long)min(n0 + c, a.out_dim - 1) * a.w_pitch;
+    const int step = 512 * share, full = n0 < a.out_dim ? a.in / 16 * 16 : 0;
+    int k = (part * 32 + lane) * 16;
+    // the first weights are on their way while the rows are quantised
+    uint4 wv[4][NC];
+    auto fetch = [&]() {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) wv[u][c] = __ldg(reinterpret_cast<const uint4 *>(w[c] + k + u * step));
+    };
+    bool ahead = k + 3 * step < full;
+    if (ahead) fetch();
+    few_rows_codes<ROWS>(a, few_codes, pitch, scales);
+    __syncthreads();
     if (n0 < a.out_dim) {
-        const int step = 512 * share, full = a.in / 16 * 16;
         auto add = [&](int k, const uint4(&wv)[NC]) {
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
@@ -296,21 +307,18 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const __g
                 }
             }
         };
-        int k = (part * 32 + lane) * 16;
-        for (; k + 3 * step < full; k += 4 * step) {
-            uint4 wv[4][NC];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int c = 0; c < NC; ++c) wv[u][c] = __ldg(reinterpret_cast<const uint4 *>(w[c] + k + u * step));
+        while (ahead) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) add(k + u * step, wv[u]);
+            k += 4 * step;
+            ahead = k + 3 * step < full;
+            if (ahead) fetch();
         }
         for (; k < a.in; k += step) {
-            uint4 wv[NC];
+            uint4 last[NC];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) wv[c] = load_weights(w[c] + k, a.in - k);
-            add(k, wv);
+            for (int c = 0; c < NC; ++c) last[c] = load_weights(w[c] + k, a.in - k);
+            add(k, last);
         }
     }
 #pragma unroll
