@@ -955,7 +955,7 @@ struct MlpCheckpointNode : Node {
     int64_t rows;
     std::vector<int64_t> z_shape;
     variable_list apply(variable_list &&g) override {
-        const Tensor w1 = w1_.unpack(), b1 = b1_.unpack(), w2 = w2_.unpack(), kept = kept_.unpack();  // raise when the graph was released
+        const Tensor w1 = w1_.unpack(), b1 = b1_.unpack().contiguous(), w2 = w2_.unpack(), kept = kept_.unpack();  // raise when the graph was released
         const bool nz = should_compute_output(0), n1 = should_compute_output(1), nb = should_compute_output(2), n2 = should_compute_output(3);
         const bool weights = n1 || nb || n2;
         if (!g[0].defined() || !(nz || weights)) return variable_list(4);
@@ -1005,7 +1005,8 @@ Tensor mlp_checkpoint(const Tensor &z, const Tensor &w1, const Tensor &b1, const
     Tensor y = floats(z, shape), kept = fresh(z, {m ? p.bytes : 0}, at::kByte);
     if (m) {
         uint8_t *t = kept.mutable_data_ptr<uint8_t>();
-        check_status(npa_mlp_checkpoint_forward(fptr(z), fptr(w1), fptr(b1), fptr(w2), fmut(y), m, (int)k, (int)o, w1.stride(0), w1.stride(1), w2.stride(0),
+        const Tensor b = b1.contiguous();
+        check_status(npa_mlp_checkpoint_forward(fptr(z), fptr(w1), fptr(b), fptr(w2), fmut(y), m, (int)k, (int)o, w1.stride(0), w1.stride(1), w2.stride(0),
                                                 w2.stride(1), t, t + p.exps, reinterpret_cast<uint32_t *>(t + p.mask), t + p.image, p.image_bytes, stream_of(z)));
     }
     if (record) {

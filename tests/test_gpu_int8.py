@@ -271,3 +271,35 @@ def test_a_step_with_an_integer_mlp():
         assert torch.isfinite(x).all() and torch.isfinite(s).all()
     with pytest.raises(RuntimeError, match="no backward"):
         step_euler(model, x, s.requires_grad_(True), grid)
+
+
+def test_first_call_inside_a_capture_and_traces():
+    """A shape that no call has used before is recorded in a graph; torch.jit.trace keeps the operators as nodes."""
+    from npa_b200.int8 import Int8MLP, linear_int8, quantize_rows
+    x, z = _rand(190, 48, seed=1), _rand(77, 40, seed=2)
+    w, t = quantize_rows(_rand(24, 48, seed=3))
+    quick = Int8MLP(torch.nn.Sequential(torch.nn.Linear(40, 128), torch.nn.ReLU(), torch.nn.Linear(128, 9, bias=False)).cuda())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g), torch.no_grad():
+        a, b = linear_int8(x, w, t, out_dtype=torch.float16), quick(z)
+    g.replay()
+    with torch.no_grad():
+        assert torch.equal(a, linear_int8(x, w, t, out_dtype=torch.float16)) and torch.equal(b, quick(z))
+        traced = torch.jit.trace(quick, z)
+        other = _rand(77, 40, seed=9)
+        assert torch.equal(traced(other), quick(other))
+
+
+@pytest.mark.parametrize("shift", range(9))
+def test_rows_of_every_alignment(shift):
+    """Rows that start on 2, 4, 8 or 16 bytes, of lengths around the kernels' blocks."""
+    from npa_b200.int8 import quantize_rows
+    from npa_b200.rows8 import compress_rows
+    for cols in (31, 64, 65, 127, 129, 192, 193, 255, 257, 511, 513, 1030, 4104, 8195):
+        for dtype in TYPES:
+            x = _rand(9, cols + 16, seed=cols, dtype=dtype)[:, shift:shift + cols]
+            codes, scales = quantize_rows(x)
+            want, want_scales = ref.quantized(x)
+            assert torch.equal(codes.cpu().long(), want) and torch.equal(scales.cpu(), want_scales)
+            assert torch.equal(compress_rows(x).restore(torch.float32).cpu(), ref.kept(x).float())

@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import rows8_reference as ref
 
@@ -364,3 +365,69 @@ def test_training_steps(dim, C, N):
     assert float((kept[2] - plain[2]).norm()) <= 1e-2 * float(plain[2].norm())
     for k in range(3, 6):
         assert float((kept[k] - formula[k]).norm()) <= 1e-2 * float(formula[k].norm()), k
+
+
+def test_saved_on_the_host_and_recomputed():
+    """Saved-tensor hooks see what the MLP keeps: moved to the host and back, dropped and recomputed, or refused when it comes back changed."""
+    from npa_b200.mlp import apply_mlp
+    module = _mlp(83, 19)
+    z, up = _rand(700, 83, seed=1), _rand(700, 19, seed=2)
+    want = _run(module, z, up)
+    with torch.autograd.graph.save_on_cpu():
+        zr = z.clone().requires_grad_(True)
+        y = apply_mlp(module, zr, checkpoint=True)
+    for a, b in zip(torch.autograd.grad(y, [zr, *module.parameters()], up), want[1:]):
+        assert torch.equal(a, b)
+    zr = z.clone().requires_grad_(True)
+    y = torch.utils.checkpoint.checkpoint(lambda t: apply_mlp(module, t, checkpoint=True), zr, use_reentrant=False)
+    for a, b in zip(torch.autograd.grad(y, [zr, *module.parameters()], up), want[1:]):
+        assert torch.equal(a, b)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:-1] if t.dtype == torch.uint8 else t):
+        y = apply_mlp(module, z, checkpoint=True)
+    with pytest.raises(RuntimeError, match="saved-tensor hook"):
+        torch.autograd.grad(y, list(module.parameters()), up)
+
+
+@pytest.mark.parametrize("k,o", [(66, 18), (163, 35)])
+def test_strided_parameters_and_upstream(k, o):
+    """Transposed weights, a bias with gaps, upstream gradients that are broadcast or lie transposed or off 16 bytes."""
+    from npa_b200 import _native as n
+    module = _mlp(k, o)
+    w1, b1, w2 = (p.detach() for p in module.parameters())
+    z, up = _rand(1000, k, seed=1), _rand(1000, o, seed=2)
+    want = _run(module, z, up)
+    w1t, w2t = w1.t().contiguous().t(), w2.t().contiguous().t()
+    gap = torch.zeros(256, device="cuda")[::2]
+    gap.copy_(b1)
+    odd = torch.empty(1000 * o + 1, device="cuda")[1:].view(1000, o)
+    odd.copy_(up)
+    leaves = [t.requires_grad_(True) for t in (z.clone(), w1t, gap, w2t)]
+    y = n.ops.mlp_checkpoint(*leaves)
+    for upstream in (up, up.t().contiguous().t(), odd):
+        got = [y.detach(), *torch.autograd.grad(y, leaves, upstream, retain_graph=True)]
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    one = torch.autograd.grad(y, leaves, up[:1].expand(1000, o), retain_graph=True)
+    for a, b in zip(one, _run(module, z, up[:1].expand(1000, o).contiguous())[1:]):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda t: n.ops.mlp_checkpoint(t, w1t, gap, w2t), (z,), (z,))
+
+
+def test_upstream_that_is_not_finite():
+    """An infinity in one row's upstream gradient stays in that row of dz and in the units alive there; masked units do not see it."""
+    module = _mlp(66, 18)
+    w1, b1, w2 = (p.detach() for p in module.parameters())
+    z = ref.clear_of_the_corner(_rand(400, 66, seed=1), w1, b1)[:300]
+    up = _rand(300, 18, seed=2) * 1e-6
+    want = _run(module, z, up)
+    alive = (z.double() @ w1.double().t() + b1.double() > 0)[5]
+    up[5, 2] = float("inf")
+    got = _run(module, z, up)
+    rest = torch.arange(300, device="cuda") != 5
+    assert torch.equal(got[1][rest], want[1][rest]) and not torch.isfinite(got[1][5]).all()
+    assert not torch.isfinite(got[3][alive]).any() and torch.isfinite(got[3][~alive]).all()
+    # the row's finite share of the dead units' gradient is zero, so what they had stays to the rounding of their sum
+    assert float((got[2][~alive] - want[2][~alive]).abs().max()) <= 4e-6 * float(want[2].abs().max())
+    others = torch.arange(18, device="cuda") != 2
+    assert torch.isfinite(got[4][others]).all() and not torch.isfinite(got[4][2]).all()
