@@ -28,14 +28,17 @@ __global__ void __launch_bounds__(T > 128 ? T : 128) quantize_rows_kernel(const 
     const bool here = row < rows;  // (the warp's other rows need its shuffles)
     const X *p = x + (here ? row : 0) * pitch;
     const int end = here ? cols : 0;
-    float v[kQuantizeHeld][V];
+    Values<X, V, W> held[kQuantizeHeld];  // (in their own type: half the registers for 16 bits, and twice the rows under way)
     unsigned largest = 0;
 #pragma unroll
-    for (int i = 0; i < kQuantizeHeld; ++i) load_values<X, V, W>(p + (i * T + t) * V, end - (i * T + t) * V, v[i]);
+    for (int i = 0; i < kQuantizeHeld; ++i) held[i].load(p + (i * T + t) * V, end - (i * T + t) * V);
 #pragma unroll
-    for (int i = 0; i < kQuantizeHeld; ++i)
+    for (int i = 0; i < kQuantizeHeld; ++i) {
+        float v[V];
+        held[i].get(v);
 #pragma unroll
-        for (int q = 0; q < V; ++q) largest = max(largest, magnitude(quantizable<UNSIGNED>(v[i][q])));
+        for (int q = 0; q < V; ++q) largest = max(largest, magnitude(quantizable<UNSIGNED>(v[q])));
+    }
     for (int k = (kQuantizeHeld * T + t) * V; k < end; k += T * V) {
         float w[V];
         load_values<X, V, W>(p + k, end - k, w);
@@ -70,7 +73,11 @@ __global__ void __launch_bounds__(T > 128 ? T : 128) quantize_rows_kernel(const 
     };
 #pragma unroll
     for (int i = 0; i < kQuantizeHeld; ++i)
-        if ((i * T + t) * V < cols) put((i * T + t) * V, v[i]);
+        if ((i * T + t) * V < cols) {
+            float v[V];
+            held[i].get(v);
+            put((i * T + t) * V, v);
+        }
     for (int k = (kQuantizeHeld * T + t) * V; k < cols; k += T * V) {
         float w[V];
         load_values<X, V, W>(p + k, cols - k, w);

@@ -73,11 +73,13 @@ __device__ __forceinline__ bool quick_codes(const float (&x)[N], float scale, fl
     }
     return rest >= 0.5f * scale;
 }
-template <int N>
+static __device__ __noinline__ unsigned row_code_out_of_line(float x, float scale, float inverse) { return (unsigned)row_code(x, scale, inverse); }
+// (FAR: where many copies of this would crowd the instructions that run, mlp_int8 13.1 us for 2,500 rows instead of 14.8; slower elsewhere.)
+template <int N, bool FAR = false>
 __device__ __forceinline__ void row_codes(const float (&x)[N], float scale, float inverse, unsigned (&code)[N]) {
     if (quick_codes(x, scale, inverse, code)) {
 #pragma unroll
-        for (int q = 0; q < N; ++q) code[q] = (unsigned)row_code(x[q], scale, inverse);
+        for (int q = 0; q < N; ++q) code[q] = FAR ? row_code_out_of_line(x[q], scale, inverse) : (unsigned)row_code(x[q], scale, inverse);
     }
 }
 // The lowest bytes of four codes.
@@ -129,26 +131,34 @@ __device__ __forceinline__ void warp_max8(unsigned (&v)[8]) {
 
 // V values at p, of which `left` exist; in loads of W bytes.
 template <typename T, int V, int W = 16>
-__device__ __forceinline__ void load_values(const T *__restrict__ p, int left, float (&v)[V]) {
-    if constexpr (V == 1) {
-        v[0] = left > 0 ? as_float(p[0]) : 0.f;
-    } else {
-        if (left >= V) {
-            using Word = std::conditional_t<W == 16, uint4, uint2>;
-            constexpr int kWords = V * (int)sizeof(T) / W;
-            union {
-                Word word[kWords];
-                T value[V];
-            } u;
+struct Values {
+    using Word = std::conditional_t<W == 16, uint4, uint2>;
+    union {
+        Word word[V == 1 ? 1 : V * (int)sizeof(T) / W];
+        T value[V];
+    };
+    __device__ __forceinline__ void load(const T *__restrict__ p, int left) {
+        if constexpr (V > 1) {
+            if (left >= V) {
 #pragma unroll
-            for (int q = 0; q < kWords; ++q) u.word[q] = __ldg(reinterpret_cast<const Word *>(p) + q);
-#pragma unroll
-            for (int q = 0; q < V; ++q) v[q] = as_float(u.value[q]);
-        } else {
-#pragma unroll
-            for (int q = 0; q < V; ++q) v[q] = q < left ? as_float(p[q]) : 0.f;
+                for (int q = 0; q < V * (int)sizeof(T) / W; ++q) word[q] = __ldg(reinterpret_cast<const Word *>(p) + q);
+                return;
+            }
         }
+#pragma unroll
+        for (int q = 0; q < V; ++q) value[q] = q < left ? p[q] : from_float<T>(0.f);
     }
+    __device__ __forceinline__ void get(float (&v)[V]) const {
+#pragma unroll
+        for (int q = 0; q < V; ++q) v[q] = as_float(value[q]);
+    }
+    __device__ __forceinline__ Values() {}
+};
+template <typename T, int V, int W = 16>
+__device__ __forceinline__ void load_values(const T *__restrict__ p, int left, float (&v)[V]) {
+    Values<T, V, W> r;
+    r.load(p, left);
+    r.get(v);
 }
 // V codes to p, of which `left` exist; `aligned`: p is a multiple of V.
 template <int V>

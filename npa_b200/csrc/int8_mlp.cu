@@ -76,7 +76,7 @@ __device__ __forceinline__ void convert_rows(const float *p, int in, uint8_t *co
     for (int r = 0; r < 8; ++r) {
         const float s = __shfl_sync(kFull, scale, 4 * r), i = __shfl_sync(kFull, inverse, 4 * r);
         unsigned code[kBlocks];
-        row_codes<kBlocks>(v[r], s, i, code);
+        row_codes<kBlocks, true>(v[r], s, i, code);
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) codes[(b / 4) * kMlpTile + r * 128 + (((2 * (b % 4)) ^ (r & 6)) << 4) + place[r & 1]] = (uint8_t)code[b];
     }
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kMlpThreads, 1) mlp_int8_kernel(const __grid_c
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 unsigned code[16], w[4];
-                row_codes<16>(v[c], u, inverse, code);
+                row_codes<16, true>(v[c], u, inverse, code);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[j] = pack_codes(code[4 * j], code[4 * j + 1], code[4 * j + 2], code[4 * j + 3]) ^ 0x80808080u;
                 *reinterpret_cast<uint4 *>(to + code_place(row, 64 * half + 16 * c)) = make_uint4(w[0], w[1], w[2], w[3]);
