@@ -23,8 +23,7 @@ __global__ void __launch_bounds__(256) rows8_compress_kernel(const T *__restrict
     const unsigned e = rows8_exponent(largest);
     const float to_units = rows8_to_units(e);
     unsigned code[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) code[q] = (unsigned)rows8_code(v[q], to_units);
+    rows8_codes<8>(v, e, to_units, code);
     if (left > 0) store_codes<8>(reinterpret_cast<uint8_t *>(codes) + row * codes_pitch + k, left, (reinterpret_cast<uintptr_t>(codes) | codes_pitch) % 8 == 0, code);
     if (part % 4 == 0) exps[row * groups + part / 4] = (uint8_t)e;
 }
@@ -64,9 +63,12 @@ __global__ void __launch_bounds__(256) rows8_compress_lanes_kernel(const T *__re
     uint8_t *to = staged[warp];
     row = row0;
     g = g0;
+    const bool far = __any_sync(kFull, e >= 254u);
 #pragma unroll
     for (int i = 0; i < kRowsFlight; ++i) {
-        const int code = rows8_code(v[i], __shfl_sync(kFull, to_units, 4 * i));
+        const float units_of = __shfl_sync(kFull, to_units, 4 * i);
+        int code = (int)__float_as_uint(__fmaf_rn(v[i], units_of, kRoundWhole));
+        if (far) code = rows8_code(v[i], units_of);
         if (whole) {
             to[i * kRowsGroup + lane] = (uint8_t)code;
         } else {
@@ -117,19 +119,24 @@ __global__ void __launch_bounds__(256) rows8_restore_kernel(const int8_t *__rest
     if (k + V <= cols) {  // within one row: one group, or two
         const int g = k / kRowsGroup, left = (g + 1) * kRowsGroup - k;
         const float one = rows8_unit(e[g]), two = left < V ? rows8_unit(e[g + 1]) : one;
-        int code[V];
+        unsigned word[V / 4];
         if (reinterpret_cast<uintptr_t>(c + k) % 4 == 0) {
 #pragma unroll
-            for (int w = 0; w < V / 4; ++w) {
-                const char4 q = *reinterpret_cast<const char4 *>(c + k + 4 * w);
-                code[4 * w] = q.x; code[4 * w + 1] = q.y; code[4 * w + 2] = q.z; code[4 * w + 3] = q.w;
-            }
+            for (int w = 0; w < V / 4; ++w) word[w] = *reinterpret_cast<const unsigned *>(c + k + 4 * w);
         } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) code[i] = c[k + i];
+            for (int w = 0; w < V / 4; ++w) {
+                const uint8_t *b = reinterpret_cast<const uint8_t *>(c + k + 4 * w);
+                word[w] = (unsigned)b[0] | (unsigned)b[1] << 8 | (unsigned)b[2] << 16 | (unsigned)b[3] << 24;
+            }
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) u.value[i] = restored<T>((float)code[i] * (i < left ? one : two));
+        for (int w = 0; w < V / 4; ++w) {
+            float v[4];
+            rows8_numbers(word[w], v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u.value[4 * w + i] = restored<T>(v[i] * (4 * w + i < left ? one : two));
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {

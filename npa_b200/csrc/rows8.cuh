@@ -28,6 +28,23 @@ __device__ __forceinline__ float rows8_unit(unsigned e) { return e == 255u ? __u
 __device__ __forceinline__ int rows8_code(float x, float to_units) {
     return to_units == 0.f ? 0 : max(-127, min(127, __float2int_rn(x * to_units)));
 }
+// Codes of N values of a group, in their lowest bytes: rounded by adding 1.5 * 2^23.  Only the last binade (up to 128 units) and groups
+// that are not finite need rows8_code.
+template <int N>
+__device__ __forceinline__ void rows8_codes(const float (&x)[N], unsigned e, float to_units, unsigned (&code)[N]) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) code[q] = __float_as_uint(__fmaf_rn(x[q], to_units, kRoundWhole));
+    if (e >= 254u) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) code[q] = (unsigned)rows8_code(x[q], to_units);
+    }
+}
+// Four codes as numbers: each byte, 128 added, becomes the last of 2^23's.
+__device__ __forceinline__ void rows8_numbers(unsigned codes, float (&v)[4]) {
+    const unsigned u = codes ^ 0x80808080u;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650 + q)) - 8388736.f;
+}
 
 // mlp_checkpoint.cu: the sizes that the MLP with a checkpoint takes.
 int check_mlp8(const char *me, int64_t rows, int32_t in_dim, int32_t out_dim);
