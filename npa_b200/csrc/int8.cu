@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "int8.cuh"
+#include "ops.cuh"
 
 namespace npa {
 
@@ -24,66 +25,80 @@ __global__ void __launch_bounds__(T > 128 ? T : 128) quantize_rows_kernel(const 
     after_previous_kernel();
     constexpr int kRows = T >= 128 ? 1 : 128 / T;
     const int t = threadIdx.x % T;
-    const long long row = (long long)blockIdx.x * kRows + threadIdx.x / T;
-    const bool here = row < rows;  // (the warp's other rows need its shuffles)
-    const X *p = x + (here ? row : 0) * pitch;
-    const int end = here ? cols : 0;
-    Values<X, V, W> held[kQuantizeHeld];  // (in their own type: half the registers for 16 bits, and twice the rows under way)
-    unsigned largest = 0;
-#pragma unroll
-    for (int i = 0; i < kQuantizeHeld; ++i) held[i].load(p + (i * T + t) * V, end - (i * T + t) * V);
-#pragma unroll
-    for (int i = 0; i < kQuantizeHeld; ++i) {
-        float v[V];
-        held[i].get(v);
-#pragma unroll
-        for (int q = 0; q < V; ++q) largest = max(largest, magnitude(quantizable<UNSIGNED>(v[q])));
-    }
-    for (int k = (kQuantizeHeld * T + t) * V; k < end; k += T * V) {
-        float w[V];
-        load_values<X, V, W>(p + k, end - k, w);
-#pragma unroll
-        for (int q = 0; q < V; ++q) largest = max(largest, magnitude(quantizable<UNSIGNED>(w[q])));
-    }
-    largest = warp_max<(T < 32 ? T : 32)>(largest);
-    if constexpr (T > 32) {
-        __shared__ unsigned most[T / 32];
-        if (t % 32 == 0) most[t / 32] = largest;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < T / 32; ++w) largest = max(largest, most[w]);
-    }
-    if (!here) return;
-    float inverse;
-    const float scale = row_scale(largest, UNSIGNED ? 255.f : 127.f, inverse);
-    uint8_t *out = codes + row * codes_pitch;
     const bool aligned = (reinterpret_cast<uintptr_t>(codes) | codes_pitch) % 8 == 0;
-    auto put = [&](int k, const float (&w)[V]) {
-        float x[V];
-        unsigned code[V];
+    // (in their own type: half the registers for 16 bits, and twice the rows under way)
+    Values<X, V, W> held[kQuantizeHeld], next[kQuantizeHeld];
+    auto load = [&](Values<X, V, W>(&to)[kQuantizeHeld], long long row) {
+        const X *p = x + (row < rows ? row : 0) * pitch;
+        const int end = row < rows ? cols : 0;
 #pragma unroll
-        for (int q = 0; q < V; ++q) x[q] = quantizable<UNSIGNED>(w[q]);
-        if (inverse == 0.f) {  // the row is not finite
-#pragma unroll
-            for (int q = 0; q < V; ++q) code[q] = 0;
-        } else {
-            row_codes<V>(x, scale, inverse, code);
-        }
-        store_codes<V>(out + k, cols - k, aligned, code);
+        for (int i = 0; i < kQuantizeHeld; ++i) to[i].load(p + (i * T + t) * V, end - (i * T + t) * V);
     };
+    long long row = (long long)blockIdx.x * kRows + threadIdx.x / T;
+    const long long step = (long long)gridDim.x * kRows;
+    load(held, row);
+    // (the block's rows end together: their threads share warps and barriers)
+    for (int turn = 0; row - threadIdx.x / T < rows; row += step, turn ^= 1) {
+        load(next, row + step);  // on its way meanwhile
+        const bool here = row < rows;
+        const X *p = x + (here ? row : 0) * pitch;
+        const int end = here ? cols : 0;
+        unsigned largest = 0;
 #pragma unroll
-    for (int i = 0; i < kQuantizeHeld; ++i)
-        if ((i * T + t) * V < cols) {
+        for (int i = 0; i < kQuantizeHeld; ++i) {
             float v[V];
             held[i].get(v);
-            put((i * T + t) * V, v);
+#pragma unroll
+            for (int q = 0; q < V; ++q) largest = max(largest, magnitude(quantizable<UNSIGNED>(v[q])));
         }
-    for (int k = (kQuantizeHeld * T + t) * V; k < cols; k += T * V) {
-        float w[V];
-        load_values<X, V, W>(p + k, cols - k, w);
-        put(k, w);
+        for (int k = (kQuantizeHeld * T + t) * V; k < end; k += T * V) {
+            float w[V];
+            load_values<X, V, W>(p + k, end - k, w);
+#pragma unroll
+            for (int q = 0; q < V; ++q) largest = max(largest, magnitude(quantizable<UNSIGNED>(w[q])));
+        }
+        largest = warp_max<(T < 32 ? T : 32)>(largest);
+        if constexpr (T > 32) {
+            __shared__ unsigned most[2][T / 32];
+            if (t % 32 == 0) most[turn][t / 32] = largest;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < T / 32; ++w) largest = max(largest, most[turn][w]);
+        }
+        if (here) {
+            float inverse;
+            const float scale = row_scale(largest, UNSIGNED ? 255.f : 127.f, inverse);
+            uint8_t *out = codes + row * codes_pitch;
+            auto put = [&](int k, const float (&w)[V]) {
+                float x[V];
+                unsigned code[V];
+#pragma unroll
+                for (int q = 0; q < V; ++q) x[q] = quantizable<UNSIGNED>(w[q]);
+                if (inverse == 0.f) {  // the row is not finite
+#pragma unroll
+                    for (int q = 0; q < V; ++q) code[q] = 0;
+                } else {
+                    row_codes<V>(x, scale, inverse, code);
+                }
+                store_codes<V>(out + k, cols - k, aligned, code);
+            };
+#pragma unroll
+            for (int i = 0; i < kQuantizeHeld; ++i)
+                if ((i * T + t) * V < cols) {
+                    float v[V];
+                    held[i].get(v);
+                    put((i * T + t) * V, v);
+                }
+            for (int k = (kQuantizeHeld * T + t) * V; k < cols; k += T * V) {
+                float w[V];
+                load_values<X, V, W>(p + k, cols - k, w);
+                put(k, w);
+            }
+            if (t == 0) scales[row] = scale;
+        }
+#pragma unroll
+        for (int i = 0; i < kQuantizeHeld; ++i) held[i] = next[i];
     }
-    if (t == 0) scales[row] = scale;
 }
 
 // Rows of up to 32 kBlocks values whose addresses fit no vector: a warp takes eight of them, lane = column, so that its loads are lines
@@ -391,9 +406,12 @@ static bool is_code(int type) { return type == NPA_INT8 || type == NPA_UINT8; }
 
 template <typename X, bool UNSIGNED, int T, int V, int W>
 static void launch_quantize_shape(const void *x, long long pitch, long long rows, int cols, void *codes, long long codes_pitch, float *scales, cudaStream_t st) {
-    constexpr int kRows = T >= 128 ? 1 : 128 / T;
-    launch_early(quantize_rows_kernel<X, UNSIGNED, T, V, W>, (unsigned)((rows + kRows - 1) / kRows), T > 128 ? T : 128, 0, st, static_cast<const X *>(x), pitch, rows, cols,
-                 static_cast<uint8_t *>(codes), codes_pitch, scales);
+    constexpr int kRows = T >= 128 ? 1 : 128 / T, kThreads = T > 128 ? T : 128;
+    const long long blocks = (rows + kRows - 1) / kRows;
+    int resident = 0;  // (where it cannot be asked for, the launch says why)
+    if (persistent_ctas(quantize_rows_kernel<X, UNSIGNED, T, V, W>, kThreads, 0, &resident) != NPA_OK) resident = 148;
+    launch_early(quantize_rows_kernel<X, UNSIGNED, T, V, W>, (unsigned)(blocks < resident ? blocks : resident), kThreads, 0, st, static_cast<const X *>(x), pitch, rows,
+                 cols, static_cast<uint8_t *>(codes), codes_pitch, scales);
 }
 template <typename X, bool UNSIGNED>
 static void launch_quantize_type(const void *x, long long pitch, long long rows, int cols, void *codes, long long codes_pitch, float *scales, cudaStream_t st) {

@@ -153,6 +153,11 @@ struct Values {
         for (int q = 0; q < V; ++q) v[q] = as_float(value[q]);
     }
     __device__ __forceinline__ Values() {}
+    __device__ __forceinline__ Values &operator=(const Values &from) {
+#pragma unroll
+        for (int q = 0; q < (int)(sizeof(word) / sizeof(Word)); ++q) word[q] = from.word[q];
+        return *this;
+    }
 };
 template <typename T, int V, int W = 16>
 __device__ __forceinline__ void load_values(const T *__restrict__ p, int left, float (&v)[V]) {
