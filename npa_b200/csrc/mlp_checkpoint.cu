@@ -394,8 +394,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
         const int quarter = warp & 3, half = warp >> 2;  // rows 32 quarter + lane; hidden units 64 half and up, every second 16 columns of dz
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
         const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
-        const int buffers = ck_dz_buffers(a.in), turns = 4 / buffers, mine = quarter % buffers;  // (two quarters take turns)
-        float *stg = staged + mine * 32 * a.in;
+        const int buffers = ck_dz_buffers(a.in);  // (with two of them quarters 0 and 2, 1 and 3 take turns)
+        float *stg = staged + quarter % buffers * 32 * a.in;
         const bool aligned = (uintptr_t)a.dz % 16 == 0;
         auto bits_of = [&](int t) {
             const long long row = row_of(t) + quarter * 32 + lane;
@@ -410,14 +410,21 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             const int e = sh.units[t % kCkRowRing][quarter * 32 + lane] + head.w1 + head.w2, e1 = max(min(e, 127), -126);
             const float unit = power_of_two(e1), rest = power_of_two(max(e - e1, -126));
             const bool far = __any_sync(kFull, e != e1);
-            // the rows that were here before have left: turn `at` of this buffer, counted over the tiles
-            const int at = t * turns + quarter / buffers;
-            if (!umma_wait(&sh.copied[mine], (at & 1) ^ 1, &sh.abort)) return false;
             float *row = stg + lane * a.in;
-            auto block = [&](int c0, auto full) {
-                unsigned r[16];
-                tmem_ld16(tlane + kCkDzCol + c0, r);
-                tc_wait_ld();
+            auto emptied = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.dz_empty);
+            };
+            // The rows that were here before have left: this quarter's, and those of the one that shares its buffer.  (A barrier each, one
+            // phase a tile: a wait tells a barrier's last two phases apart and no more.)
+            auto free_again = [&]() -> bool {
+                if (t > 0 && !umma_wait(&sh.copied[quarter], (t - 1) & 1, &sh.abort)) return false;
+                if (buffers == 4) return true;
+                if (quarter >= 2) return umma_wait(&sh.copied[quarter - 2], t & 1, &sh.abort);
+                return t == 0 || umma_wait(&sh.copied[quarter + 2], (t - 1) & 1, &sh.abort);
+            };
+            auto put = [&](unsigned(&r)[16], int c0, auto full) {
                 if (far) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * rest);
@@ -426,19 +433,23 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
                 for (int j = 0; j < 16; ++j)
                     if (decltype(full)::value || c0 + j < a.in) row[c0 + j] = __uint_as_float(r[j]) * unit;
             };
+            if (!free_again()) return false;
+            auto block = [&](int c0, auto full) {
+                unsigned r[16];
+                tmem_ld16(tlane + kCkDzCol + c0, r);
+                tc_wait_ld();
+                put(r, c0, full);
+            };
             int c0 = 16 * half;
 #pragma unroll 1
             for (; c0 + 16 <= a.in; c0 += 32) block(c0, std::true_type());
             if (c0 < a.in) block(c0, std::false_type());
-            tc_fence_before();
+            emptied();
             fence_proxy_async();  // the copy reads these
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&sh.dz_empty);
-                mbar_arrive(&sh.staged[mine]);
-            }
+            if (lane == 0) mbar_arrive(&sh.staged[quarter]);
             if (half == 0) {
-                if (!umma_wait(&sh.staged[mine], at & 1, &sh.abort)) return false;
+                if (!umma_wait(&sh.staged[quarter], t & 1, &sh.abort)) return false;
                 if (nrows == 32 && aligned) {
                     if (lane == 0) {
                         bulk_copy_s2g(a.dz + row0 * a.in, stg, (unsigned)(128 * a.in));
@@ -449,7 +460,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
                     for (int q = lane; q < nrows * a.in; q += 32) a.dz[row0 * a.in + q] = stg[q];
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.copied[mine]);
+                if (lane == 0) mbar_arrive(&sh.copied[quarter]);
             }
             return true;
         };
