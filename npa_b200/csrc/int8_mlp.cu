@@ -377,7 +377,8 @@ int launch_mlp_int8(const char *me, const float *z, const void *w1, long long w1
     a.blocks = (in + 31) / 32;
     const int fixed = 1024 + a.chunks * kMlpTile + a.n2 * 128 + a.zbufs * a.chunks * kMlpTile + 2 * kMlpTile + kMlpRows * out * 4 + 16;
     const int room = 232448 - (int)sizeof(MlpInt8Shared) - 1024 - fixed;
-    a.slots = room / a.slot_bytes < kMlpMaxSlots ? room / a.slot_bytes : kMlpMaxSlots;
+    // an even number of them: a slot then always serves the same four warps, which see each of its phases (a wait tells two apart, no more)
+    a.slots = (room / a.slot_bytes < kMlpMaxSlots ? room / a.slot_bytes : kMlpMaxSlots) & ~1;
     if (a.slots < 2) return fail(NPA_ERR_UNSUPPORTED, "%s: no room for two slots of rows", me);
     if (!(a.status = umma_status_word())) return fail(NPA_ERR_CUDA, "%s: no status word", me);
     CUtensorMap w1_map, w2_map;
