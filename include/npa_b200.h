@@ -639,7 +639,8 @@ enum { NPA_FLOAT32 = 0, NPA_FLOAT16 = 1, NPA_BFLOAT16 = 2, NPA_INT8 = 3, NPA_UIN
 /* Rows into 8-bit codes with one scale each: scale = max(fl32(max |x| / most), 2^-126), code = x / scale rounded to
  * nearest, ties to even; most = 127 (codes_type NPA_INT8), or 255 (NPA_UINT8: numbers below zero count as zero).  A row
  * that holds an infinity or a NaN gets the scale NaN and codes of zero.  Pitches are in elements; x_pitch may be 0 (one
- * row repeated).  npa_dequantize_rows writes code * scale, contiguous. */
+ * row repeated).  codes holds rows * codes_pitch bytes; where codes_pitch is cols rounded up to 16, the bytes behind a
+ * row's last code may be written too, with any other pitch they are left.  npa_dequantize_rows writes code * scale, contiguous. */
 int npa_quantize_rows(const void *x, int32_t x_type, int64_t x_pitch, int64_t rows, int32_t cols, void *codes,
                       int32_t codes_type, int64_t codes_pitch, float *scales, void *stream);
 int npa_dequantize_rows(const void *codes, int32_t codes_type, int64_t codes_pitch, const float *scales, int64_t rows,
@@ -668,7 +669,7 @@ int npa_mlp_int8(const float *z, int64_t z_pitch, const void *w1, int64_t w1_pit
 /* Activations in 8 bits for a backward pass: groups of 32 columns share a power of two, value = code * 2^(E - 133),
  * |code| <= 127, E = clamp((bits(max |x|) + 0x10000) >> 23, 7, 254), one byte per group, exponents [rows, ceil(cols / 32)];
  * a group that holds an infinity or a NaN has E = 255 and is restored as NaN.  Restored values beyond the largest
- * number of float16 become it. */
+ * number of float16 become it.  codes_pitch as above. */
 int npa_rows8_compress(const void *x, int32_t type, int64_t x_pitch, int64_t rows, int32_t cols, void *codes,
                        int64_t codes_pitch, uint8_t *exponents, void *stream);
 int npa_rows8_restore(const void *codes, int64_t codes_pitch, const uint8_t *exponents, int64_t rows, int32_t cols,

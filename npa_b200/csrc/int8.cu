@@ -102,7 +102,8 @@ __global__ void __launch_bounds__(T > 128 ? T : 128) quantize_rows_kernel(const 
 }
 
 // Rows of up to 32 kBlocks values whose addresses fit no vector: a warp takes eight of them, lane = column, so that its loads are lines
-// and the maxima share their shuffles.  Codes leave through shared memory in 16 bytes a lane where they may (`whole`).
+// and the maxima share their shuffles.  Codes leave through shared memory in 16 bytes a lane where a row's pitch is its length rounded up
+// to 16 (`whole`: what lies between is the row's own); in a wider pitch what follows a row stays as it was.
 template <typename X, bool UNSIGNED, int kBlocks>
 __global__ void __launch_bounds__(128) quantize_lanes_kernel(const X *__restrict__ x, long long pitch, long long rows, int cols, uint8_t *__restrict__ codes,
                                                              long long codes_pitch, float *__restrict__ scales) {
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(128) quantize_lanes_kernel(const X *__restrict
     float v[8][kBlocks];
     unsigned largest[8];
     const int there = rows - row0 < 8 ? (int)(rows - row0) : 8;
-    const bool whole = (reinterpret_cast<uintptr_t>(codes) | codes_pitch) % 16 == 0;
+    const bool whole = reinterpret_cast<uintptr_t>(codes) % 16 == 0 && codes_pitch == (cols + 15) / 16 * 16;
 #pragma unroll
     for (int r = 0; r < 8; ++r)
 #pragma unroll

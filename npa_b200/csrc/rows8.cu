@@ -29,7 +29,8 @@ __global__ void __launch_bounds__(256) rows8_compress_kernel(const T *__restrict
 }
 
 // Other rows: a warp takes eight groups that follow one another, lane = column, so that its loads are lines and the maxima share their
-// shuffles.  The codes leave through shared memory in pieces of 16 bytes (`whole`: where rows of codes lie on such; bytes otherwise):
+// shuffles.  The codes leave through shared memory in pieces of 16 bytes (`whole`: where a row's pitch is its
+// length rounded up to 16; in a wider one what follows a row stays as it was, and they leave as bytes):
 // a store of 32 single bytes costs 12 clocks of an SM, whatever it hits (95 us for 8,191 rows of 4,100).
 constexpr int kRowsFlight = 8;
 template <typename T>
@@ -194,7 +195,7 @@ int npa_rows8_compress(const void *x, int32_t type, int64_t x_pitch, int64_t row
         const uintptr_t lie = (uintptr_t)x | (uintptr_t)(x_pitch * (int64_t)sizeof(T));
         const bool vectors = lie % 8 == 0;
         const long long units = rows * rows8_groups(cols), blocks = vectors ? (4 * units + 255) / 256 : (units + 8 * kRowsFlight - 1) / (8 * kRowsFlight);
-        const int whole = ((uintptr_t)codes | (uintptr_t)codes_pitch) % 16 == 0;
+        const int whole = (uintptr_t)codes % 16 == 0 && codes_pitch == (cols + 15) / 16 * 16;
         if (vectors)
             launch_early(lie % 16 == 0 ? rows8_compress_kernel<T, 16> : rows8_compress_kernel<T, 8>, (unsigned)blocks, 256, 0, (cudaStream_t)stream, static_cast<const T *>(x), x_pitch, rows, cols,
                          static_cast<int8_t *>(codes), codes_pitch, exponents);

@@ -431,3 +431,21 @@ def test_upstream_that_is_not_finite():
     assert float((got[2][~alive] - want[2][~alive]).abs().max()) <= 4e-6 * float(want[2].abs().max())
     others = torch.arange(18, device="cuda") != 2
     assert torch.isfinite(got[4][others]).all() and not torch.isfinite(got[4][2]).all()
+
+
+@pytest.mark.parametrize("cols", [33, 66, 100, 163, 240])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_what_follows_a_row_of_codes_stays_as_it_was(cols, offset):
+    """Rows of codes inside wider ones: the columns behind them belong to the caller, whichever way the values are read."""
+    from npa_b200 import _native as n
+    rows, pitch = 77, 256
+    x = _rand(rows * cols + offset, seed=5).cuda()[offset:]
+    stream, at = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream), lambda t: ctypes.c_void_p(t.data_ptr())
+    exps, scales = torch.zeros(rows * 8, dtype=torch.uint8, device="cuda"), torch.zeros(rows, device="cuda")
+    packed = (cols + 15) // 16 * 16
+    for call in (lambda c, p: n.lib.npa_rows8_compress(at(x), 0, cols, rows, cols, at(c), p, at(exps), stream),
+                 lambda c, p: n.lib.npa_quantize_rows(at(x), 0, cols, rows, cols, at(c), 3, p, at(scales), stream)):
+        wide, narrow = (torch.full((rows, p), 99, dtype=torch.int8, device="cuda") for p in (pitch, packed))
+        assert call(wide, pitch) == 0 and call(narrow, packed) == 0
+        assert (wide[:, cols:] == 99).all()
+        assert torch.equal(wide[:, :cols], narrow[:, :cols])
