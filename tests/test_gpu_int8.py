@@ -157,7 +157,8 @@ def test_rows_do_not_depend_on_their_neighbours(M):
 def test_mlp_is_its_two_layers():
     from npa_b200.int8 import Int8MLP, linear_int8, mlp_int8, quantize_rows
     for rows, k, hidden, n, seed in [(1, 66, 128, 18, 0), (127, 5, 128, 1, 1), (2500, 66, 128, 18, 2), (1000, 163, 128, 35, 3), (513, 176, 128, 48, 4),
-                                     (300, 64, 256, 40, 5), (33, 200, 96, 7, 6), (70001, 83, 128, 19, 7)]:
+                                     (300, 64, 256, 40, 5), (33, 200, 96, 7, 6), (70001, 83, 128, 19, 7),
+                                     (60001, 114, 128, 24, 8), (40000, 250, 128, 64, 9)]:
         z = _rand(rows, k, seed=seed)
         z[rows // 2] = 0
         w1, t1 = quantize_rows(_rand(hidden, k, seed=10 + seed))
@@ -167,6 +168,9 @@ def test_mlp_is_its_two_layers():
         h = linear_int8(z, w1, t1, bias=b1, relu=True)
         q, s = quantize_rows(h, unsigned=True)
         _same(y, linear_int8(q, w2, t2, x_scales=s))
+        off = torch.empty(rows * k + 1, device="cuda")[1:].view(rows, k)  # rows that start off 16 bytes take the two products
+        off.copy_(z)
+        _same(mlp_int8(off, w1, t1, b1, w2, t2), y)
         codes, scales = ref.quantized(z)
         hr = ref.linear(codes, scales, w1, t1, b1, True)
         codes, scales = ref.quantized(hr, True)
