@@ -956,7 +956,8 @@ struct MlpCheckpointNode : Node {
     std::vector<int64_t> z_shape;
     variable_list apply(variable_list &&g) override {
         const Tensor w1 = w1_.unpack(), b1 = b1_.unpack().contiguous(), w2 = w2_.unpack(), kept = kept_.unpack();  // raise when the graph was released
-        const bool nz = should_compute_output(0), n1 = should_compute_output(1), nb = should_compute_output(2), n2 = should_compute_output(3);
+        // (of what needs gradients, what this backward was asked for: dz and the weights' sums are kernels of their own)
+        const bool nz = task_should_compute_output(0), n1 = task_should_compute_output(1), nb = task_should_compute_output(2), n2 = task_should_compute_output(3);
         const bool weights = n1 || nb || n2;
         if (!g[0].defined() || !(nz || weights)) return variable_list(4);
         c10::cuda::CUDAGuard guard(w1.device());
