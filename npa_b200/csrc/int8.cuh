@@ -181,6 +181,36 @@ __device__ __forceinline__ void store_codes(uint8_t *p, int left, bool aligned, 
     }
 }
 
+// ---- rows put together in shared memory ----------------------------------------------------------------------------------
+// 16 values (`left` of them exist) of a row in a tile whose rows follow one another without a gap, lane = row.  Word by word the lanes meet
+// in a bank as often as 32 and the length have a factor in common (32 ways for 32, 64, 96, 128, 160 columns); rows of a multiple of four
+// columns go by 16 bytes, each lane beginning with another of its four pieces where rows start in the same banks, which leaves two ways at most.
+__device__ __forceinline__ int first_piece(int cols, int lane) {
+    const int common = min((cols / 4) & -(cols / 4), 8);
+    return ((lane & 7) * common >> 3) & 3;
+}
+__device__ __forceinline__ void put_16_pieces(float *to, int left, int first, float (&v)[16]) {
+    float w[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = first & 1 ? v[(j + 4) % 16] : v[j];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = first & 2 ? w[(j + 8) % 16] : w[j];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int k = 4 * ((i + first) & 3);
+        if (k < left) *reinterpret_cast<float4 *>(to + k) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+}
+__device__ __forceinline__ void put_16(float *to, int left, int cols, int lane, float (&v)[16]) {
+    if (cols % 4 == 0) {
+        put_16_pieces(to, left, first_piece(cols, lane), v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < left) to[j] = v[j];
+    }
+}
+
 // ---- the product -----------------------------------------------------------------------------------------------------
 struct Int8Args {
     const void *x;       // [rows, in] codes, or values that the kernel for few rows quantises

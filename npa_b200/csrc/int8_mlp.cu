@@ -12,6 +12,9 @@
 //   * eight warps, two for a quarter of the rows, turn sums into h (64 units a thread, kept in registers between the maximum and the
 //     codes) and the second layer's sums into rows of y, which leave as one contiguous block.
 //
+// Measured (B200, us): 82 for 262,144 rows of 163 and 35 (the bytes alone: 32), 9.6 for 2,500 rows of 66 and 18.  The instructions bound it:
+// 20,800 a tile of 128 rows, issue slots 44 % taken, the tensor pipe 4 %.
+//
 // The MMA takes signed codes on both sides: h's are shifted by 128, and 128 times the sum of w2's row comes back in the epilogue.
 // Waits are bounded as in umma.cuh.
 #include "int8.cuh"
@@ -263,10 +266,10 @@ __global__ void __launch_bounds__(kMlpThreads, 1) mlp_int8_kernel(const __grid_c
                 unsigned r[16];
                 tmem_ld16(tlane + kMlpYCol + 64 * b + c0, r);
                 tc_wait_ld();
-                float *to = ytile + row * a.out + c0;
+                float y[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (c0 + j < a.out) to[j] = __fmul_rn(__int2float_rn((int)r[j] + sh.sums[c0 + j]), __fmul_rn(u, sh.t2[c0 + j]));
+                for (int j = 0; j < 16; ++j) y[j] = __fmul_rn(__int2float_rn((int)r[j] + sh.sums[c0 + j]), __fmul_rn(u, sh.t2[c0 + j]));
+                put_16(ytile + row * a.out + c0, a.out - c0, a.out, lane, y);
             }
             tc_fence_before();
             __syncwarp();

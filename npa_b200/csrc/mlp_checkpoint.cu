@@ -31,8 +31,9 @@
 //
 // Memory is the floor (B200, 262,144 rows of 163 and 35: 512 MB, 78 us) and not what bounds them: it is the way of a tile through
 // conversion, product, mask, product, one after another in what tensor and shared memory are left.  Measured there, us: forward 147
-// (the 32-bit forward that leaves its hidden layer: 143), dz 75, weights 137, their sum over CTAs 8; the parts of a tile's way stand at the
-// kernels.  At 32,768 rows of 66 and 18: 19, 12, 21 and 7, and the host takes 90 us a pass.
+// (the 32-bit forward that leaves its hidden layer: 143), dz 78, weights 137, their sum over CTAs 8; the parts of a tile's way stand at the
+// kernels.  At 32,768 rows of 66 and 18: 19, 12, 21 and 7, and the host takes 90 us a pass, 57 of them
+// torch's engine for the backward.
 //
 // Waits are bounded as in umma.cuh; they report through npa_linear_tcgen05_status (bits 1024, 2048, 4096: MMA lane, producers, epilogue).
 #include <mutex>
@@ -273,7 +274,8 @@ struct CkDzShared {
     int abort;
 };
 constexpr int kCkDzCol = 256;
-// A quarter's 32 rows of dz are put together as they lie in memory; two quarters share a buffer where four do not fit.
+// A quarter's 32 rows of dz are put together as they lie in memory; two quarters share a buffer where four do not fit.  (dz alone of
+// 262,144 rows, four / two buffers: 100 columns 56.2 / 63.3 us; 66, 67 and 128 the same.)
 __host__ __device__ constexpr int ck_dz_buffers(int in) { return in <= 128 ? 4 : 2; }
 static int ck_dz_smem(int chunks, int in) { return 1024 + (2 * chunks + 2) * kCkTile + 2 * kCkTile + ck_dz_buffers(in) * 128 * in; }
 __device__ inline void bulk_copy_s2g(void *dst, const void *src, unsigned bytes) {
@@ -283,7 +285,9 @@ __device__ inline void bulk_commit() { asm volatile("cp.async.bulk.commit_group;
 __device__ inline void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ inline void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-template <bool TWO>
+// PIECES: rows of a multiple of four columns leave by 16 bytes (put_16_pieces): 262,144 rows of 128 and 160 columns 191 -> 76 and 215 -> 84 us.  An
+// argument of the kernel: with both ways in one the registers of the other widths suffered (82 -> 89 us for 163).
+template <bool TWO, bool PIECES>
 __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const __grid_constant__ CkArgs a) {
     after_previous_kernel();
     extern __shared__ uint8_t ck_raw[];
@@ -429,9 +433,16 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
 #pragma unroll
                     for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * rest);
                 }
+                if constexpr (PIECES) {
+                    float v[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (decltype(full)::value || c0 + j < a.in) row[c0 + j] = __uint_as_float(r[j]) * unit;
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) * unit;
+                    put_16_pieces(row + c0, decltype(full)::value ? 16 : a.in - c0, first_piece(a.in, lane), v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (decltype(full)::value || c0 + j < a.in) row[c0 + j] = __uint_as_float(r[j]) * unit;
+                }
             };
             if (!free_again()) return false;
             auto block = [&](int c0, auto full) {
@@ -1107,10 +1118,10 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                 unsigned r[16];
                 tmem_ld16(tlane + 256 + 128 * b + c0, r);
                 tc_wait_ld();
-                float *to = ytile + row * a.out + c0;
+                float y[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (c0 + j < a.out) to[j] = __uint_as_float(r[j]) * unit * rest;
+                for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]) * unit * rest;
+                put_16(ytile + row * a.out + c0, a.out - c0, a.out, lane, y);
             }
             tc_fence_before();
             __syncwarp();
@@ -1282,7 +1293,9 @@ int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, con
     a.tiles = (int)((rows + kCkRows - 1) / kCkRows);
     if (!(a.status = umma_status_word())) return fail(NPA_ERR_CUDA, "%s: no status word", me);
     const bool two = out_dim > 32;
-    if (dz && (rc = ck_launch(two ? mlp_checkpoint_dz_kernel<true> : mlp_checkpoint_dz_kernel<false>, "mlp_checkpoint_dz_kernel", a, ck_dz_smem(a.chunks, in_dim), r.ctas, st)) !=
+    const auto dz_kernel = in_dim % 4 ? (two ? mlp_checkpoint_dz_kernel<true, false> : mlp_checkpoint_dz_kernel<false, false>)
+                                      : (two ? mlp_checkpoint_dz_kernel<true, true> : mlp_checkpoint_dz_kernel<false, true>);
+    if (dz && (rc = ck_launch(dz_kernel, "mlp_checkpoint_dz_kernel", a, ck_dz_smem(a.chunks, in_dim), r.ctas, st)) !=
                   NPA_OK)
         return rc;
     if (!dW1) return NPA_OK;
