@@ -163,11 +163,13 @@ __global__ void __launch_bounds__(256) dequantize_rows_kernel(const Code *__rest
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
 // Up to 16 rows (a token, a handful of particles): the weights are read once, from memory or L2, and that is the time.  Each block holds
-// the codes of all rows in shared memory (it quantises up to 8,192 values itself, from L2; of more, every block would do too much of the
-// same: a launch in front does it, linear_few_odd 13.0 -> 9 us),
+// the codes of all rows in shared memory.  It quantises up to 4,096 values itself; of more, every block does too much of the same, and a
+// launch in front does it (us inside / in front, weights in L2: 1 x 1,024 3.7 / 4.8, 1 x 4,096 5.8 / 5.9, 8 x 1,024 8.1 / 5.6,
+// 4 x 4,096 13.2 / 7.7).  Against the tensor cores' kernel, us (this / that): 1 x 4,096 x 4,096 5.8 / 18.5, 8 10.7 / 18.2, 16 16.1 / 17.6;
+// 16 x 1,024 x 1,024 6.9 / 8.1, 16 x 2,048 x 5,120 13.7 / 11.9: 16 rows is where they meet.
 // a warp takes NC channels and a lane 16 bytes of each at a time, NC x 4 loads in flight; four dp4a per row and 16 bytes are free
 // beside them.  Where the channels alone would not fill the SMs, the warps of a block share a channel's length.
-constexpr int kFewRows = 16, kFewBytes = 96 * 1024, kFewWarps = 8, kFewQuantized = 8192;
+constexpr int kFewRows = 16, kFewBytes = 96 * 1024, kFewWarps = 8, kFewQuantized = 4096;
 
 template <bool UNSIGNED>
 __device__ __forceinline__ int dot4(unsigned x, unsigned w, int acc) {
@@ -419,17 +421,21 @@ static void launch_quantize_type(const void *x, long long pitch, long long rows,
 #define NPA_QUANTIZE(T, V, W) launch_quantize_shape<X, UNSIGNED, T, V, W>(x, pitch, rows, cols, codes, codes_pitch, scales, st)
     const uintptr_t lie = (uintptr_t)x | (uintptr_t)(pitch * (long long)sizeof(X));
     if (lie % 16 == 0) {
-        // threads for a row so that it fits the registers of each
-        if (cols <= 128) NPA_QUANTIZE(8, 8, 16);
+        // the fewest threads whose registers hold a row.  Measured with 8, 32, 128, 256 of them, us (bf16, L2 flushed):
+        //   32,768 x 256 14.4, 23.6, 66.6, 126;  8,192 x 1,024 23.6, 13.4, 23.6, 37.9;  8,192 x 4,096 104, 45.0, 29.7, 44.0;
+        //   4,096 x 8,192 198, 54.2, 39.8, 29.7
+        if (cols <= 256) NPA_QUANTIZE(8, 8, 16);
         else if (cols <= 1024) NPA_QUANTIZE(32, 8, 16);
         else if (cols <= 4096) NPA_QUANTIZE(128, 8, 16);
         else NPA_QUANTIZE(256, 8, 16);
     } else if (lie % 8 == 0) {
-        if (cols <= 128) NPA_QUANTIZE(8, 8, 8);
+        if (cols <= 256) NPA_QUANTIZE(8, 8, 8);
         else if (cols <= 1024) NPA_QUANTIZE(32, 8, 8);
+        else if (cols <= 4096) NPA_QUANTIZE(128, 8, 8);
         else NPA_QUANTIZE(256, 8, 8);
     } else {
         if (cols <= 512) {
+            // (65,536 rows of 67, 163, 255 32-bit values: 14.3, 19.5, 25.6 us; by single values of 128 threads 52, 58, 60)
             void (*const kernel)(const X *, long long, long long, int, uint8_t *, long long, float *) =
                 cols <= 64 ? quantize_lanes_kernel<X, UNSIGNED, 2> : cols <= 128 ? quantize_lanes_kernel<X, UNSIGNED, 4>
                 : cols <= 192 ? quantize_lanes_kernel<X, UNSIGNED, 6> : cols <= 256 ? quantize_lanes_kernel<X, UNSIGNED, 8> : nullptr;
@@ -469,7 +475,9 @@ static int launch_few_rows_shape(const Int8Args &a, int share, cudaStream_t st) 
 static int padded_rows(long long rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 static bool few_rows(long long rows, int in) { return rows <= kFewRows && padded_rows(rows) * round16(in) <= kFewBytes; }
 static int launch_few_rows(const Int8Args &a, cudaStream_t st) {
-    // four channels a warp where that still gives every SM its eight warps; the length shared where single channels do not
+    // four channels a warp where that still gives every SM its eight warps (1 x 2,048: 8,192 channels 15.4 -> 13.2 us, 4,096 the same; 8
+    // rows, 4,096 channels 17.4 -> 13.3); the length shared where single channels do not (8,192 x 256: 15.4 us alone, 13.3 by two or
+    // four, 15.2 by eight)
     const bool wide = a.out_dim >= 148 * kFewWarps * 2;
     int share = 1;
     while (!wide && share < kFewWarps && (long long)a.out_dim * share < 148 * kFewWarps && a.in > 512 * share) share *= 2;
