@@ -12,8 +12,8 @@
 //   * eight warps, two for a quarter of the rows, turn sums into h (64 units a thread, kept in registers between the maximum and the
 //     codes) and the second layer's sums into rows of y, which leave as one contiguous block.
 //
-// Measured (B200, us): 82 for 262,144 rows of 163 and 35 (the bytes alone: 32), 9.6 for 2,500 rows of 66 and 18.  The instructions bound it:
-// 20,800 a tile of 128 rows, issue slots 44 % taken, the tensor pipe 4 %.
+// Measured (B200, us): 80 for 262,144 rows of 163 and 35 (the bytes alone: 32), 9.5 for 2,500 rows of 66 and 18.  The instructions bound it:
+// 20,500 a tile of 128 rows, issue slots 46 % taken, the tensor pipe 4 %.
 //
 // The MMA takes signed codes on both sides: h's are shifted by 128, and 128 times the sum of w2's row comes back in the epilogue.
 // Waits are bounded as in umma.cuh.

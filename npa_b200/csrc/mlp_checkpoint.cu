@@ -22,15 +22,15 @@
 //
 // What goes through memory is z, y, the checkpoint, dy and dz: no kernel writes a hidden layer (dh is made twice: 18 of 86 and of 127
 // thousand products a row at 163 inputs and 35 outputs, against 512 bytes each way).  An addition on the tensor cores cuts off what lies
-// below the sum's last bit, so products with tails come first or have a sum of their own.  Error against 64 bits, in norm: 3e-7 to 5e-7 for
-// every output; torch's own in 32 bits 2e-7 to 1.6e-6.
+// below the sum's last bit, so products with tails come first or have a sum of their own.  Error against 64 bits, in norm: 2e-7 to 5e-7 for
+// every output; torch's own in 32 bits 1e-7 (few rows and columns, where it is the smaller) to 1.6e-6.
 //
 // The layouts use that a swizzled tile of 16-bit numbers serves both ways: rows of 64 numbers (128 bytes, 128-byte swizzle) are a
 // K-major operand for sums over the columns and an MN-major one for sums over the rows.  So one image of W1 ([hidden][in]) is B of
 // z W1^T, A of zh W1^T and B of dh W1, and one tile of zh is B of both of its products, as is dy's.
 //
 // Memory is the floor (B200, 262,144 rows of 163 and 35: 512 MB, 78 us) and not what bounds them: it is the way of a tile through
-// conversion, product, mask, product, one after another in what tensor and shared memory are left.  Measured there, us: forward 147
+// conversion, product, mask, product, one after another in what tensor and shared memory are left.  Measured there, us: forward 142
 // (the 32-bit forward that leaves its hidden layer: 143), dz 78, weights 137, their sum over CTAs 8; the parts of a tile's way stand at the
 // kernels.  At 32,768 rows of 66 and 18: 19, 12, 21 and 7, and the host takes 90 us a pass, 57 of them
 // torch's engine for the backward.
