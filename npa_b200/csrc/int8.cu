@@ -520,6 +520,7 @@ struct Int8Plan {
 static int check_rows(const char *me, int64_t rows, int32_t cols) {
     if (rows <= 0 || cols <= 0) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: rows and columns must be positive", me);
     if (rows > ((int64_t)1 << 31) - 1) return fail(NPA_ERR_UNSUPPORTED, "%s: supports fewer than 2^31 rows, got %lld", me, (long long)rows);
+    if (cols > 1 << 30) return fail(NPA_ERR_UNSUPPORTED, "%s: supports up to 2^30 columns, got %d", me, (int)cols);
     return NPA_OK;
 }
 

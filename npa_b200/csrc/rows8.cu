@@ -173,6 +173,7 @@ static int check_rows8(const char *me, const void *floats, int type, const void 
     if (rows <= 0 || cols <= 0) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: rows and columns must be positive", me);
     if (rows * (int64_t)rows8_groups(cols) >= (int64_t)1 << 33 || rows * (int64_t)cols >= (int64_t)1 << 38)
         return fail(NPA_ERR_UNSUPPORTED, "%s: supports fewer than 2^33 groups and 2^38 values", me);
+    if (cols > 1 << 30) return fail(NPA_ERR_UNSUPPORTED, "%s: supports up to 2^30 columns, got %d", me, (int)cols);
     if (!float_size(type)) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: unknown type", me);
     if (!floats || !codes || !exps) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: every array must be non-NULL", me);
     if ((uintptr_t)floats % float_size(type)) return fail(NPA_ERR_INVALID_ARGUMENT, "%s: the values must be aligned to their type", me);

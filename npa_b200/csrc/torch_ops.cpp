@@ -765,6 +765,7 @@ void refuse_gradients(const char *name, const In &...inputs) {
     refuse_tangents(name, inputs...);
     if (recording(inputs...)) throw std::runtime_error(std::string(name) + " has no backward: call it under torch.no_grad(), or detach its inputs");
 }
+constexpr int64_t kMostColumns = (int64_t)1 << 30;  // a column and a block's step behind it are 32-bit numbers
 // The rows of a tensor [..., k] as the kernels read them: elements next to each other, one distance between rows.
 struct Rows {
     Tensor t;  // keeps the memory
@@ -773,6 +774,7 @@ struct Rows {
         if (x.dim() < 1) throw std::runtime_error(std::string(name) + " must have at least 1 dimension");
         cols = x.size(-1);
         if (cols < 1) throw std::runtime_error(std::string(name) + " must have at least one column, got " + shape_text(x.sizes()));
+        if (cols > kMostColumns) throw std::runtime_error(std::string(name) + " must have at most 2^30 columns, got " + shape_text(x.sizes()));
         rows = x.numel() / cols;
         t = x.is_contiguous() ? x : x.dim() == 2 ? x : x.reshape({rows, cols});
         if (t.dim() == 2 && !t.is_contiguous() && ((t.stride(1) != 1 && cols > 1) || t.stride(0) < 0)) t = t.contiguous();
@@ -837,6 +839,7 @@ Rows weight_rows(const Tensor &w, const Tensor &scales, const Tensor &like, int6
     if (w.scalar_type() != at::kChar) throw py::type_error(std::string(name) + ": expected int8, got " + toString(w.scalar_type()));
     if (w.dim() != 2) throw std::runtime_error(std::string(name) + " must have 2 dimensions, got " + std::to_string(w.dim()));
     if (in >= 0 && w.size(1) != in) throw std::runtime_error(std::string(name) + " must have " + std::to_string(in) + " columns, got " + shape_text(w.sizes()));
+    if (w.size(0) > kMostColumns) throw std::runtime_error(std::string(name) + " must have at most 2^30 channels, got " + shape_text(w.sizes()));
     need_scales(scales, w, scales_name);
     return Rows(w, name);
 }

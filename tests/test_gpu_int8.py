@@ -307,3 +307,16 @@ def test_rows_of_every_alignment(shift):
             want, want_scales = ref.quantized(x)
             assert torch.equal(codes.cpu().long(), want) and torch.equal(scales.cpu(), want_scales)
             assert torch.equal(compress_rows(x).restore(torch.float32).cpu(), ref.kept(x).float())
+
+
+def test_more_columns_than_32_bits_count():
+    """Refused before anything is read or allocated: the rows are one number repeated."""
+    from npa_b200 import int8, rows8
+    long = 2**32 + 32
+    x, codes, one = (torch.zeros(1, 1, dtype=d, device="cuda") for d in (torch.float32, torch.int8, torch.float32))
+    for call in (lambda: int8.quantize_rows(x.expand(1, long)), lambda: int8.dequantize_rows(codes.expand(1, long), one[0]),
+                 lambda: int8.linear_int8(x.expand(1, long), codes.expand(1, long), one[0]), lambda: rows8.compress_rows(x.expand(1, long))):
+        with pytest.raises(RuntimeError, match="columns"):
+            call()
+    with pytest.raises(RuntimeError, match="channels"):
+        int8.linear_int8(x, codes.expand(long, 1), one[0].expand(long))

@@ -36,6 +36,10 @@ def test_bad_arguments_of_the_c_abi():
         (small, "needed", lib.npa_linear_int8(ok, F32, 8, None, ok, 16, ok, None, 0, 0, ok, F32, 100, 8, 8, ok, 8, None)),
         (inv, "unknown type", lib.npa_linear_int8(ok, 9, 8, None, ok, 8, ok, None, 0, 0, ok, F32, 1, 8, 8, ok, 1 << 20, None)),
         (inv, "must be there", lib.npa_mlp_int8(ok, 8, ok, 16, ok, None, ok, 128, ok, ok, 1, 8, 128, 4, ok, 1 << 20, None)),
+        (uns, "2^30 columns", lib.npa_quantize_rows(ok, F32, 0, 1, (1 << 31) - 8, ok, I8, 1 << 31, ok, None)),
+        (uns, "2^30 columns", lib.npa_dequantize_rows(ok, I8, 0, ok, 1, (1 << 30) + 1, ok, F32, None)),
+        (uns, "2^30 columns", lib.npa_rows8_compress(ok, F32, 0, 1, (1 << 31) - 1, ok, 1 << 31, ok, None)),
+        (uns, "2^30 columns", lib.npa_rows8_restore(ok, 1 << 31, ok, 1, (1 << 30) + 1, ok, F32, None)),
         (inv, "positive", lib.npa_rows8_compress(ok, F32, 8, 1, 0, ok, 16, ok, None)),
         (inv, "overlap", lib.npa_rows8_compress(ok, F32, 8, 1, 8, ok, 7, ok, None)),
         (inv, "unknown type", lib.npa_rows8_restore(ok, 16, ok, 1, 8, ok, I8, None)),
