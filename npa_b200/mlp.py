@@ -132,9 +132,9 @@ def apply_mlp(module, z, checkpoint=False):
     """``module(z)``; with the fused weight-gradient backward when ``supported(module)``.
 
     ``checkpoint=True`` keeps for the backward, instead of ``z`` and the hidden layer in 32 bits (``4 (in + 128)`` bytes a
-    row), ``z`` in 8 bits (``rows8``) and the bits of the ReLU (``in + in / 32 + 16`` bytes a row, and for each call 65 to
-    131 KB of weights as the tensor cores read them): values and the gradients of
-    ``z`` and of the bias are those of the plain call, the gradients of the two weight matrices see ``z`` rounded to 8 bits.
+    row), ``z`` in 8 bits (``rows8``) and the bits of the ReLU (``in + in / 32 + 16`` bytes a row, and for each call 67 to
+    132 KB of weights as the tensor cores read them): values and the gradients of ``z`` and of the bias are those of the plain
+    call to the rounding of 32-bit sums, the gradients of the two weight matrices see ``z`` rounded to 8 bits.
     It needs a ``supported`` module on the default engine, and is refused (``ValueError``) otherwise;
     without a gradient to record the call is the plain one."""
     if checkpoint and torch.is_grad_enabled():
