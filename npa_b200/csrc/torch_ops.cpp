@@ -702,9 +702,21 @@ struct MlpNode : Node {
     }
 };
 
-// y = relu(z W1^T + b1) W2^T over the rows of z; the caller has checked the shapes (mlp.supported).
+// What mlp.supported does not look at: rows of another width would have the kernels read behind the weights, and a module whose layers
+// lie on different devices another one's memory.
+void check_mlp(const Tensor &z, const Tensor &w1, const Tensor &b1, const Tensor &w2) {
+    const int64_t k = w1.size(1);
+    if (z.dim() < 1 || z.size(-1) != k) throw std::runtime_error("z must have " + std::to_string(k) + " columns, got " + shape_text(z.sizes()));
+    if (k < 1 || w2.size(0) < 1) throw std::runtime_error("the adaptation MLP must have at least one input and one output");
+    for (const Tensor *t : {&z, &b1, &w2})
+        if (t->device() != w1.device() || t->scalar_type() != at::kFloat)
+            throw py::type_error("the adaptation MLP: expected float32 tensors on " + w1.device().str() + ", got " + toString(t->scalar_type()) + " on " + t->device().str());
+}
+
+// y = relu(z W1^T + b1) W2^T over the rows of z; the caller has checked the module (mlp.supported), and z is contiguous.
 Tensor mlp(const Tensor &z, const Tensor &w1, const Tensor &b1, const Tensor &w2) {
     refuse_tangents("the adaptation MLP", z, w1, b1, w2);
+    check_mlp(z, w1, b1, w2);
     c10::cuda::CUDAGuard guard(z.device());
     const int64_t k = z.size(-1), m = z.numel() / k, o = w2.size(0);
     std::vector<int64_t> shape = z.sizes().vec();
@@ -715,7 +727,8 @@ Tensor mlp(const Tensor &z, const Tensor &w1, const Tensor &b1, const Tensor &w2
     // without a backward the hidden layer stays in tensor memory
     Tensor y = floats(z, shape), h = record ? floats(z, {m, kHidden}) : Tensor(), image = floats(z, {bytes / 4});
     Tensor dz_image = dz_bytes ? floats(z, {dz_bytes / 4}) : Tensor();
-    check_status(npa_mlp_forward_tcgen05_images(fptr(z), fptr(w1), fptr(b1), fptr(w2), fmut(h), fmut(y), m, (int)k, (int)o, w1.stride(0), w1.stride(1),
+    const Tensor bias = b1.contiguous();
+    check_status(npa_mlp_forward_tcgen05_images(fptr(z), fptr(w1), fptr(bias), fptr(w2), fmut(h), fmut(y), m, (int)k, (int)o, w1.stride(0), w1.stride(1),
                                                 w2.stride(0), w2.stride(1), image.mutable_data_ptr(), bytes, fmut(dz_image), dz_bytes,
                                                 stream_of(z)));
     if (record) {
@@ -999,10 +1012,9 @@ Tensor mlp_checkpoint(const Tensor &z, const Tensor &w1, const Tensor &b1, const
     const bool record = recording(z, w1, b1, w2);
     if (!record && z.numel()) return mlp(z, w1, b1, w2);
     refuse_tangents("the adaptation MLP", z, w1, b1, w2);
+    check_mlp(z, w1, b1, w2);
     c10::cuda::CUDAGuard guard(z.device());
-    const int64_t k = w1.size(1), o = w2.size(0);
-    if (z.dim() < 1 || z.size(-1) != k) throw std::runtime_error("z must have " + std::to_string(k) + " columns, got " + shape_text(z.sizes()));
-    const int64_t m = z.numel() / k;
+    const int64_t k = w1.size(1), o = w2.size(0), m = z.numel() / k;
     std::vector<int64_t> shape = z.sizes().vec();
     shape.back() = o;
     const CheckpointPlaces p(m, k);

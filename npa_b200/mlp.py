@@ -146,7 +146,7 @@ def apply_mlp(module, z, checkpoint=False):
         if z.device != w1.device or z.dtype != torch.float32:
             raise TypeError(f"z: expected a float32 tensor on {w1.device}, got {z.dtype} on {z.device}")
         return N.ops.mlp_checkpoint(z.contiguous(), w1, first.bias, last.weight)
-    if not (supported(module) and z.is_cuda and z.dtype == torch.float32):
+    if not (supported(module) and z.is_cuda and z.dtype == torch.float32 and z.dim() and z.shape[-1] == module[0].in_features):
         return module(z)
     if TENSOR_ENGINE == "tcgen05" and FUSED_FORWARD and FUSED_HIDDEN_GRAD:
         return N.ops.mlp(z.contiguous(), module[0].weight, module[0].bias, module[2].weight)
