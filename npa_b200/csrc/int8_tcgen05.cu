@@ -36,7 +36,7 @@ struct Int8Shape {
 };
 
 struct Int8Shared {
-    uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
+    uint64_t full[8], empty[8], acc_full[2], acc_empty[2], columns;
     uint32_t tmem_base;
     int abort;
 };
@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) int8_umma_kernel(const __grid_c
             mbar_init(&sh.acc_full[q], 1);
             mbar_init(&sh.acc_empty[q], kI8EpilogueWarps);
         }
+        mbar_init(&sh.columns, kI8EpilogueWarps);
         sh.abort = 0;
         mbar_fence_init();
     }
@@ -177,7 +178,10 @@ __global__ void __launch_bounds__(kI8Threads, 1) int8_umma_kernel(const __grid_c
                 sums[c] = there && a.w_sums ? 128 * __ldg(a.w_sums + n0 + c) : 0;
             }
             const float row_scale = lane < nrows ? __ldg(a.x_scales + row0 + lane) : 0.f;
-            asm volatile("bar.sync 1, %0;" ::"n"(kI8EpilogueWarps * 32) : "memory");
+            // (a bounded wait as all others: at a barrier of the hardware a warp would stay for good when another has given up and left)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.columns);
+            if (!(ok = umma_wait(&sh.columns, it & 1, &sh.abort))) break;
             if (!(ok = umma_wait(&sh.acc_full[acc], (it >> 1) & 1, &sh.abort, kUmmaWaitNs, 100))) break;
             tc_fence_after();
 #pragma unroll 1
