@@ -52,7 +52,8 @@ def mlp_int8(z, w1, w1_scales, b1, w2, w2_scales):
 class Int8MLP(torch.nn.Module):
     """``Sequential(Linear, ReLU, Linear(bias=False))`` in float32, for evaluation in 8-bit integers (``mlp_int8``).
 
-    Takes the place of ``model.model`` in an NPA model; the buffers travel with ``state_dict`` and ``to``."""
+    Takes the place of ``model.model`` in an NPA model; the buffers travel with ``state_dict`` and ``to``.  The rows of the
+    codes lie a multiple of 16 bytes apart, as the kernel for both layers reads them, whatever gave them other memory."""
 
     def __init__(self, module):
         super().__init__()
@@ -71,6 +72,24 @@ class Int8MLP(torch.nn.Module):
                 self.register_buffer(name + "_scales", scales)
             self.register_buffer("b1", first.bias.detach().float().clone())
         self.in_features, self.out_features = first.in_features, last.out_features
+
+    def _lay_out(self):
+        """A copy that is moved has dense rows (66 bytes apart, say), and so has an assigned one: back to multiples of 16."""
+        for name in ("w1", "w2"):
+            codes = getattr(self, name)
+            if codes.stride(1) != 1 or codes.stride(0) % 16 or (codes.is_cuda and codes.data_ptr() % 16):
+                wide = codes.new_zeros(codes.shape[0], -(-codes.shape[1] // 16) * 16)
+                wide[:, : codes.shape[1]] = codes
+                setattr(self, name, wide[:, : codes.shape[1]])
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._lay_out()
+        return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._lay_out()
 
     def forward(self, z):
         return mlp_int8(z, self.w1, self.w1_scales, self.b1, self.w2, self.w2_scales)
