@@ -58,9 +58,12 @@ unsigned *umma_status_word();  // mlp_tcgen05.cu
 int launch_grad_reduce(const GradReduce &a, cudaStream_t st);  // mlp_grad_tcgen05.cu
 
 // ---- numbers ---------------------------------------------------------------------------------------------------------
-// Exponent of the power of two at or below a magnitude; 0 for zero and for what is not finite (it goes through unscaled).
-__device__ __forceinline__ int binade(unsigned magnitude_bits) {
-    return magnitude_bits == 0 || magnitude_bits >= 0x7f800000u ? 0 : max((int)(magnitude_bits >> 23), 1) - 127;
+// Exponent of the power of two at or below a finite magnitude; 0 for zero.
+__device__ __forceinline__ int binade(unsigned magnitude_bits) { return magnitude_bits == 0 ? 0 : max((int)(magnitude_bits >> 23), 1) - 127; }
+// A magnitude as a unit sees it: what is not finite has no part in it, so that its neighbours keep their accuracy.
+__device__ __forceinline__ unsigned finite_magnitude(float v) {
+    const unsigned m = magnitude(v);
+    return m < 0x7f800000u ? m : 0u;
 }
 __device__ __forceinline__ float power_of_two(int e) { return e < -126 ? 0.f : __uint_as_float((unsigned)(min(e, 127) + 127) << 23); }
 // a in the lower half.
@@ -102,21 +105,21 @@ __global__ void __launch_bounds__(512) mlp_checkpoint_image_kernel(const __grid_
         for (int i = 0; i < 32 * kCkMaxIn / 512; ++i) {
             const int q = threadIdx.x + 512 * i;
             const float4 v = q < 32 * a.in ? __ldg(reinterpret_cast<const float4 *>(a.W1) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
-            m[0] = max(m[0], max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w))));
+            m[0] = max(m[0], max(max(finite_magnitude(v.x), finite_magnitude(v.y)), max(finite_magnitude(v.z), finite_magnitude(v.w))));
         }
     } else {
 #pragma unroll 8
         for (int q = threadIdx.x; q < 128 * a.in; q += 512) {
             const int j = q / a.in, k = q - j * a.in;
-            m[0] = max(m[0], magnitude(__ldg(a.W1 + j * a.s1o + k * a.s1i)));
+            m[0] = max(m[0], finite_magnitude(__ldg(a.W1 + j * a.s1o + k * a.s1i)));
         }
     }
 #pragma unroll
     for (int i = 0; i < 128 * kCkMaxOut / 512; ++i) {
         const int q = threadIdx.x + 512 * i;
-        m[1] = max(m[1], q < 128 * a.out ? magnitude(__ldg(a.W2 + (q >> 7) * a.s2o + (q & 127) * a.s2i)) : 0u);
+        m[1] = max(m[1], q < 128 * a.out ? finite_magnitude(__ldg(a.W2 + (q >> 7) * a.s2o + (q & 127) * a.s2i)) : 0u);
     }
-    if (threadIdx.x < 128) m[2] = magnitude(__ldg(a.b1 + threadIdx.x));
+    if (threadIdx.x < 128) m[2] = finite_magnitude(__ldg(a.b1 + threadIdx.x));
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
         m[q] = warp_max(m[q]);
@@ -193,11 +196,6 @@ struct CkArgs {
 // smallest), and 1 / unit.
 __device__ __forceinline__ unsigned row_unit(unsigned largest) { return min(max(largest >> 23, 1u), 253u); }
 __device__ __forceinline__ float from_row_unit(unsigned field) { return __uint_as_float((254u - field) << 23); }
-// A magnitude as the unit sees it: what is not finite has no part in it, so that its neighbours keep their accuracy.
-__device__ __forceinline__ unsigned finite_magnitude(float v) {
-    const unsigned m = magnitude(v);
-    return m < 0x7f800000u ? m : 0u;
-}
 
 // One producer warp's 32 rows of dy, two neighbouring columns a lane: half a warp for a row of up to 32 columns, 24 lanes for one of up
 // to 48 (TWO).  Loaded a tile ahead ...
