@@ -8,22 +8,22 @@
 // dz and db1 are those of a backward in 32 bits, because the bits are those of the forward; dW1 and dW2 see the rounding of z to codes.
 //
 // All products run on the fifth-generation tensor cores at 32-bit accuracy with half the work of TF32: kind::f16 runs at twice its rate.
-// A number is taken apart into a head and a tail of float16, 22 bits (the dropped tail x tail is 2^-24); zh needs no tail, its codes
+// A number is taken apart into a head and a tail of float16, 22 bits (the dropped tail x tail is 2^-22); zh needs no tail, its codes
 // have 8 bits.  The price is float16's range, paid in powers of two, all exact:
 //
-//   * weights in units of their matrix, so that the largest is between 1 and 2;
+//   * weights in units of their matrix;
 //   * z in the forward, and dy for dz, in units of their row: rows of any size keep their accuracy, and the unit comes back in the epilogue;
-//   * dy and zh for the sums over rows in the unit of the largest of their tile of 128 rows: what falls below 2^-25 of dy's or 2^-32 of
-//     zh's largest would not be seen in the sum; a tile's unit comes in when its sum leaves the accumulator;
-//   * h in a unit that its products and the largest bias cannot exceed.
+//   * dy and zh for the sums over rows in the unit of the largest of their tile of 128 rows; a tile's unit comes in when its sum leaves the
+//     accumulator;
+//   * h in a unit that its products and the largest bias cannot exceed, dh times a power of two that brings its largest sum back in range.
 //
-// dh is |dy'| |W2'| <= 48 x 4 at most, so it fits float16 with 2^-25 below; nothing here can overflow.  What is not finite has no part
-// in a unit, so that its neighbours keep theirs.
+// The largest of a unit is an operand of 2^14 to 2^15 (accumulators have 32 bits, only operands are short), which leaves 22 bits to what is
+// up to 2^17 below it, and 2^-39 of the largest to the rest.  Nothing here can overflow.  What is not finite has no part in a unit, so that
+// its neighbours keep theirs.
 //
 // What goes through memory is z, y, the checkpoint, dy and dz: no kernel writes a hidden layer (dh is made twice: 18 of 86 and of 127
 // thousand products a row at 163 inputs and 35 outputs, against 512 bytes each way).  An addition on the tensor cores cuts off what lies
-// below the sum's last bit, so products with tails come first or have a sum of their own.  Error against 64 bits, in norm: 1e-7 to 5e-7 for
-// every output; torch's own in 32 bits 1e-7 (few rows and columns, where it is the smaller) to 1.6e-6.
+// below the sum's last bit, so products with tails come first or have a sum of their own.
 //
 // The layouts use that a swizzled tile of 16-bit numbers serves both ways: rows of 64 numbers (128 bytes, 128-byte swizzle) are a
 // K-major operand for sums over the columns and an MN-major one for sums over the rows.  So one image of W1 ([hidden][in]) is B of
@@ -73,6 +73,9 @@ __device__ __forceinline__ unsigned pack_halves(float a, float b) {
     return r;
 }
 __device__ __forceinline__ float2 unpack_halves(unsigned v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+// The largest of what shares a unit becomes an operand of 2^kOperand to twice that, the last binade that float16 rounds without overflow:
+// a tail's last bit is 2^-24, so that the top 17 binades keep 22 bits, and what lies below is off by 2^-39 of the largest.
+constexpr int kOperand = 14;
 // Heads and tails of two numbers.
 __device__ __forceinline__ void split_halves(float a, float b, unsigned &head, unsigned &tail) {
     head = pack_halves(a, b);
@@ -127,7 +130,6 @@ __global__ void __launch_bounds__(512) mlp_checkpoint_image_kernel(const __grid_
     }
     __syncthreads();
     const int e1 = min(binade(most[0]), 126), e2 = min(binade(most[1]), 126);
-    const float u1 = power_of_two(-e1), u2 = power_of_two(-e2);
     const int pairs1 = a.chunks * 128 * 32, total = pairs1 + 128 * 32;
     for (int q = blockIdx.x * 512 + threadIdx.x; q < total; q += gridDim.x * 512) {
         const bool first = q < pairs1;
@@ -135,8 +137,8 @@ __global__ void __launch_bounds__(512) mlp_checkpoint_image_kernel(const __grid_
         float v[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            v[i] = first ? (k + i < a.in ? __ldg(a.W1 + row * a.s1o + (k + i) * a.s1i) * u1 : 0.f)
-                         : (k + i < a.out ? __ldg(a.W2 + (k + i) * a.s2o + row * a.s2i) * u2 : 0.f);
+            v[i] = first ? (k + i < a.in ? scalbnf(__ldg(a.W1 + row * a.s1o + (k + i) * a.s1i), kOperand - e1) : 0.f)
+                         : (k + i < a.out ? scalbnf(__ldg(a.W2 + (k + i) * a.s2o + row * a.s2i), kOperand - e2) : 0.f);
         unsigned head, tail;
         split_halves(v[0], v[1], head, tail);
         uint8_t *base = a.image + kCkHeader + (first ? (long long)c : 2ll * a.chunks) * kCkTile;
@@ -192,10 +194,13 @@ struct CkArgs {
     unsigned *status;
 };
 
-// Exponent field of the unit of a row from its largest finite magnitude (a multiple of that unit is below 4; zero rows have the
-// smallest), and 1 / unit.
-__device__ __forceinline__ unsigned row_unit(unsigned largest) { return min(max(largest >> 23, 1u), 253u); }
-__device__ __forceinline__ float from_row_unit(unsigned field) { return __uint_as_float((254u - field) << 23); }
+// Exponent field of the unit of a row from its largest finite magnitude (which is below 2 units; rows below 2^-112 have that unit), and
+// 2^kOperand / unit.
+__device__ __forceinline__ unsigned row_unit(unsigned largest) { return min(max(largest >> 23, kOperand + 1u), 254u); }
+__device__ __forceinline__ float from_row_unit(unsigned field) { return __uint_as_float((254u + kOperand - field) << 23); }
+// dh as it leaves its accumulator is below 48 (2^15)^2: times this it is an operand again.
+constexpr int kDhDown = 21;
+constexpr float kDhUnit = 1.f / (1 << kDhDown);
 
 // One producer warp's 32 rows of dy, two neighbouring columns a lane: half a warp for a row of up to 32 columns, 24 lanes for one of up
 // to 48 (TWO).  Loaded a tile ahead ...
@@ -409,7 +414,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             if (!umma_wait(&sh.dz_full, t & 1, &sh.abort)) return false;
             tc_fence_after();
             // the row's unit times those of the weights: one power of two unless it is out of range
-            const int e = sh.units[t % kCkRowRing][quarter * 32 + lane] + head.w1 + head.w2, e1 = max(min(e, 127), -126);
+            const int e = sh.units[t % kCkRowRing][quarter * 32 + lane] + head.w1 + head.w2 + kDhDown - 3 * kOperand, e1 = max(min(e, 127), -126);
             const float unit = power_of_two(e1), rest = power_of_two(max(e - e1, -126));
             const bool far = __any_sync(kFull, e != e1);
             float *row = stg + lane * a.in;
@@ -490,8 +495,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
                 tc_wait_ld();
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    split_halves(bits >> (2 * j) & 1u ? __uint_as_float(r[2 * j]) : 0.f, bits >> (2 * j + 1) & 1u ? __uint_as_float(r[2 * j + 1]) : 0.f, parts[j],
-                                 parts[8 + j]);
+                    split_halves(bits >> (2 * j) & 1u ? __uint_as_float(r[2 * j]) * kDhUnit : 0.f,
+                                 bits >> (2 * j + 1) & 1u ? __uint_as_float(r[2 * j + 1]) * kDhUnit : 0.f, parts[j], parts[8 + j]);
                 tmem_st16(d + 16 * c, parts);
             }
             tc_wait_st();
@@ -790,7 +795,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             };
             float partial[4] = {};
             apart(tlane + kCkDhCol, [&](float v, bool alive, int q) {
-                v = alive ? v : 0.f;
+                v = alive ? v * kDhUnit : 0.f;
                 partial[q] += v;
                 return v;
             });
@@ -799,9 +804,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
                 if (warp == 0) ok = sums_of_w1(t);
             }
             __syncwarp();
-            // units: zh 2^zu, W1 2^w1; h in units of 2^hu, which the largest sum (176 x 2 x 32512 in the accumulator's) and bias leave below 2^15
+            // units: zh 2^zu, W1 2^(w1 - 14); h in units of 2^hu, which the largest sum (176 x 2^15 x 32512 in the accumulator's) and bias leave
+            // below 1.2 x 2^15
             const int unit = sh.dy_unit, zu = sh.z_unit, hu = max(zu + head.w1 + 24, head.b1 + 2) - 15;
-            const float to_h = power_of_two(max(zu + head.w1 - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
+            const float to_h = power_of_two(max(zu + head.w1 - kOperand - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
             if (!umma_wait(&sh.pre_full, t & 1, &sh.abort, kUmmaWaitNs, 50)) ok = false;
             tc_fence_after();
             apart(tlane + kCkPreCol, [&](float v, bool alive, int) { return alive ? __fmaf_rn(v, to_h, bias) : 0.f; });
@@ -812,11 +818,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             if (!(ok = __shfl_sync(kFull, (int)ok, 0) != 0)) break;
             // what the tile's sums are multiples of: products of powers of two, zero where they fall below the smallest number
             auto scale = [](int e) { return power_of_two(max(min(e, 127), -126)) * power_of_two(max(min(e + 126, 0), -126)); };
-            db += (partial[0] + partial[1] + (partial[2] + partial[3])) * scale(unit + head.w2);
+            db += (partial[0] + partial[1] + (partial[2] + partial[3])) * scale(unit + head.w2 + kDhDown - 2 * kOperand);
             if (!(ok = umma_wait(&sh.g1_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
             tc_fence_after();
             bool both = false;  // dW2's sums are there as well
-            const float f1 = scale(unit + head.w2 + zu), f2 = scale(unit + hu);
+            const float f1 = scale(unit + head.w2 + kDhDown - 2 * kOperand + zu), f2 = scale(unit - kOperand + hu);
 #pragma unroll
             for (int i = 0; i < kBlocks; ++i) {
                 const int b = 2 * i + half;
@@ -1101,12 +1107,12 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
         };
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
         const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
-        // h is below 2^(zr + w1 + 10) by its products (176 of numbers below 2 x 2) and 2^(b1 + 1) by its bias: twice 2^14 of its units
+        // h is below 2^(zr + w1 + 10) by its products (176 of numbers below two units each) and 2^(b1 + 1) by its bias: twice 2^14 of its units
         auto unit_of = [&](int t) { return max(sh.units[t & 3][row] + head.w1 + 10, head.b1 + 1) - 14; };
         auto leave = [&](int t) -> bool {  // y of tile t
             const int b = t & 1;
             const long long row0 = row_of(t);
-            const int e = unit_of(t) + head.w2, e1 = max(min(e, 127), -126);
+            const int e = unit_of(t) + head.w2 - kOperand, e1 = max(min(e, 127), -126);
             const float unit = power_of_two(e1), rest = power_of_two(max(e - e1, -126));
             if (!umma_wait(&sh.y_copied, (t & 1) ^ 1, &sh.abort)) return false;
             if (!umma_wait(&sh.y_full[b], (t >> 1) & 1, &sh.abort)) return false;
@@ -1144,7 +1150,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
             if (!(ok = umma_wait(&sh.h_full[b], (t >> 1) & 1, &sh.abort))) break;
             tc_fence_after();
             const int hu = unit_of(t);
-            const float f1 = power_of_two(max(sh.units[t & 3][row] + head.w1 - hu, -126)), f2 = power_of_two(min(max(-hu, -126), 127));
+            const float f1 = power_of_two(max(sh.units[t & 3][row] + head.w1 - 2 * kOperand - hu, -126)), f2 = power_of_two(min(max(-hu, -126), 127));
             unsigned bits[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) bits[w] = 0;

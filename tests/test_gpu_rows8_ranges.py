@@ -1,0 +1,122 @@
+"""The MLP with an 8-bit checkpoint where channels differ in size: inputs, hidden units, outputs and their gradients up to 2^40 apart.
+Every element of every output is held to the sum of the magnitudes behind it, as 32-bit sums of products would hold it."""
+import ctypes
+
+import pytest
+import torch
+
+import rows8_reference as ref
+
+pytestmark = pytest.mark.gpu
+NAMES = ["y", "dz", "dW1", "db1", "dW2"]
+
+# A number held as two of float16 is off by 2^-22 of itself, and the product of two tails is left out: 3 * 2^-22 a product, in each of two
+# layers.  A sum is cut off at 2^-24 of what it has come to: 33 times in z W1^T (11 steps of 16 columns, three products each), 24 times
+# in a sum over 128 hidden units or rows, 14 times over a CTA's tiles, 26 times over the CTAs, and in 32 bits around them: below 100.
+BAR = 6 * 2.0**-22 + 100 * 2.0**-24
+
+
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    yield
+    from npa_b200 import _native as n
+    status = ctypes.c_uint32(0)
+    n.check(n.lib.npa_linear_tcgen05_status(ctypes.byref(status), 1))
+    assert status.value == 0
+
+
+def _powers(n, how, seed):
+    """n powers of two: half of them 2^-12, or all between 2^-20 and 2^20 in any order, or in rising order."""
+    if how == "half":
+        e = torch.where(torch.arange(n) % 2 == 1, -12.0, 0.0)
+    elif how == "rising":
+        e = torch.linspace(-20, 20, n).round()
+    else:
+        e = torch.linspace(-20, 20, n).round()[torch.randperm(n, generator=torch.Generator().manual_seed(seed))]
+    return torch.exp2(e).cuda()
+
+
+def _rand(*shape, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*shape, device="cuda", generator=g) * torch.exp(0.5 * torch.randn(*shape[:-1], 1, device="cuda", generator=g))
+
+
+def _module(w1, b1, w2):
+    module = torch.nn.Sequential(torch.nn.Linear(w1.shape[1], 128), torch.nn.ReLU(), torch.nn.Linear(128, w2.shape[0], bias=False)).cuda()
+    with torch.no_grad():
+        for p, v in zip(module.parameters(), (w1, b1, w2)):
+            p.copy_(v)
+    return module
+
+
+def _weights(k, o, seed):
+    torch.manual_seed(seed)
+    module = torch.nn.Sequential(torch.nn.Linear(k, 128), torch.nn.ReLU(), torch.nn.Linear(128, o, bias=False)).cuda()
+    return [p.detach().clone() for p in module.parameters()]
+
+
+def _run(module, z, up):
+    from npa_b200.mlp import apply_mlp
+    z = z.detach().clone().requires_grad_(True)
+    y = apply_mlp(module, z, checkpoint=True)
+    return [y.detach(), *torch.autograd.grad(y, [z, *module.parameters()], up)]
+
+
+def _sizes(z, w1, b1, w2, up):
+    """Sums of the magnitudes behind (y, dz, dW1, db1, dW2), element by element."""
+    alive = (z.double() @ w1.double().t() + b1.double() > 0).double()
+    held, z, w1, b1, w2, up = (t.detach().double().abs().to(z.device) for t in (ref.kept(z), z, w1, b1, w2, up))
+    h, again, dh = (z @ w1.t() + b1) * alive, (held @ w1.t() + b1) * alive, (up @ w2) * alive
+    return h @ w2.t(), dh @ w1, dh.t() @ held, dh.sum(0), up.t() @ again
+
+
+def _check(w1, b1, w2, z, up, least, bar=BAR):
+    z = ref.clear_of_the_corner(z, w1, b1)
+    up = up[: len(z)]
+    assert len(z) >= least
+    truth = ref.mlp_with_checkpoint(z, w1, b1, w2, up)
+    theirs = ref.mlp_with_checkpoint(z, w1, b1, w2, up, torch.float32)
+    size = _sizes(z, w1, b1, w2, up)
+    worst = {}
+    for name, a, b, t, m in zip(NAMES, _run(_module(w1, b1, w2), z, up), theirs, truth, size):
+        floor = m.clamp_min(2.0**-120)
+        worst[name] = (float(((a.double() - t).abs() / floor).max()), float(((b.double() - t).abs() / floor).max()))
+    print({n: f"{v[0]:.1e} (torch fp32 {v[1]:.1e})" for n, v in worst.items()})
+    assert all(v[0] <= bar for v in worst.values()), worst
+
+
+CASES = {
+    "alike": {},
+    "inputs": {"z": 1},
+    "inputs against weights": {"z": 1, "w1_in": -1},
+    "weights of inputs": {"w1_in": 1},
+    "hidden units": {"w1_out": 1, "b1": 1},
+    "hidden units, not their biases": {"w1_out": 1},
+    "hidden units against outputs": {"w1_out": 1, "b1": 1, "w2_in": -1},
+    "weights of hidden units": {"w2_in": 1},
+    "outputs": {"w2_out": 1},
+    "outputs against their gradients": {"w2_out": 1, "up": -1},
+    "gradients": {"up": 1},
+}
+
+
+@pytest.mark.parametrize("rows,k,o", [(300, 66, 18), (1500, 163, 35)])
+@pytest.mark.parametrize("how", ["half"])
+@pytest.mark.parametrize("case", list(CASES))
+def test_channels_of_different_size(case, how, rows, k, o):
+    w1, b1, w2 = _weights(k, o, 1)
+    z, up = _rand(2 * rows, k, seed=2), _rand(2 * rows, o, seed=3)
+    sign = CASES[case]
+    inputs, hidden, outputs = _powers(k, how, 4), _powers(128, how, 5), _powers(o, how, 6)
+    z = z * inputs ** sign.get("z", 0)
+    w1 = w1 * inputs ** sign.get("w1_in", 0) * hidden[:, None] ** sign.get("w1_out", 0)
+    b1 = b1 * hidden ** sign.get("b1", 0)
+    w2 = w2 * hidden ** sign.get("w2_in", 0) * outputs[:, None] ** sign.get("w2_out", 0)
+    up = up * outputs ** sign.get("up", 0)
+    _check(w1, b1, w2, z, up, rows)
+
+
+@pytest.mark.parametrize("rows,k,o", [(1, 66, 18), (129, 5, 3), (4103, 163, 35), (20001, 176, 48), (65536, 96, 33)])
+def test_elements_to_their_own_size(rows, k, o):
+    w1, b1, w2 = _weights(k, o, rows)
+    _check(w1, b1, w2, _rand(rows + rows // 4 + 8, k, seed=2), _rand(rows + rows // 4 + 8, o, seed=3), rows)
