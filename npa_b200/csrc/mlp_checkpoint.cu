@@ -11,7 +11,9 @@
 // A number is taken apart into a head and a tail of float16, 22 bits (the dropped tail x tail is 2^-22); zh needs no tail, its codes
 // have 8 bits.  The price is float16's range, paid in powers of two, all exact:
 //
-//   * weights in units of their matrix;
+//   * weights in units of their matrix, and of a row or column that lies apart from it (CkHeader): input columns, hidden units and outputs of
+//     any size keep their own accuracy.  A unit of a summed index goes to the other operand or comes back into the image once in front of the
+//     tiles; one of an index that stays comes back in the epilogue.  Weights that lie together take neither way;
 //   * z in the forward, and dy for dz, in units of their row: rows of any size keep their accuracy, and the unit comes back in the epilogue;
 //   * dy and zh for the sums over rows in the unit of the largest of their tile of 128 rows; a tile's unit comes in when its sum leaves the
 //     accumulator;
@@ -85,68 +87,164 @@ __device__ __forceinline__ void split_halves(float a, float b, unsigned &head, u
 // Byte of number (row, k), k < 64, in a swizzled tile.
 __host__ __device__ constexpr int half_place(int row, int k) { return row * 128 + ((((k >> 3) ^ row) & 7) << 4) + (k & 7) * 2; }
 
+// v 2^e, for exponents of up to twice a number's.
+__device__ __forceinline__ float times_power(float v, int e) {
+    const int part = max(min(e, 127), -126);
+    return v * power_of_two(part) * power_of_two(max(min(e - part, 127), -126));
+}
+
 // ---- the weights' image ------------------------------------------------------------------------------------------------
+// W1 in units of 2^(w1 + hidden1[j] + inputs[k]), W2 in units of 2^(w2 + hidden2[j] + outputs[c]): a channel whose largest number lies 2^kApart
+// or more below the matrix's has a unit of its own, so that it is held as accurately as the largest.  Channels have 0 where that is not so.
+// A hidden unit's row of W1 counts together with its bias, which is then no larger than the matrix either.
+constexpr int kApart = 6, kFarthest = 100;
 struct CkHeader {
-    int w1, w2, b1;  // exponents of the units of W1 and W2, and of the largest bias (-1000: there is none)
+    int w1, w2, b1;      // exponents of the matrices' units, and of the largest positive bias over its row's unit (-1000: there is none)
+    int hidden;          // the largest hidden1[j] + hidden2[j]
+    int inputs_apart, hidden_apart, outputs_apart, unused;  // whether they differ (`hidden_apart`: in their sum)
+    int8_t hidden1[128], hidden2[128], inputs[192], outputs[64];
 };
+static_assert(sizeof(CkHeader) <= kCkHeader, "in front of the matrices");
 struct CkImageArgs {
     const float *W1, *b1, *W2;
     long long s1o, s1i, s2o, s2i;
     int in, out, chunks;
     uint8_t *image;  // header | W1 heads [chunks] | W1 tails [chunks] | W2 heads | W2 tails, each 128 rows of 64 numbers
 };
-__global__ void __launch_bounds__(512) mlp_checkpoint_image_kernel(const __grid_constant__ CkImageArgs a) {
+// Exponent of a channel's unit, from its largest magnitude and the matrix's exponent.
+__device__ __forceinline__ int channel_unit(unsigned largest, int e) {
+    const int d = binade(largest) - e;
+    return largest == 0 || d > -kApart ? 0 : max(d, -kFarthest);
+}
+constexpr int kImageThreads = 512;
+static int ck_image_blocks(int chunks) { return (chunks + 1) * 128 * 32 / kImageThreads; }  // a thread makes one pair
+__global__ void __launch_bounds__(kImageThreads) mlp_checkpoint_image_kernel(const __grid_constant__ CkImageArgs a) {
     after_previous_kernel();
-    __shared__ unsigned most[3];
-    if (threadIdx.x < 3) most[threadIdx.x] = 0;
+    __shared__ unsigned most[3], rows1[128], columns1[192], rows2[64], columns2[128];
+    __shared__ int hidden1[128], inputs[192], hidden2[128], outputs[64], hidden[2];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    if (t < 3) most[t] = 0;
+    if (t < 192) columns1[t] = 0;
+    if (t < 64) rows2[t] = 0;
+    if (t < 128) columns2[t] = 0;
+    if (t < 2) hidden[t] = -1000;
+    // this thread's pair of numbers, and, as every block looks at all weights (they are few, and a launch in between would cost more), eight
+    // rows of W1 a warp and a quarter of a column of W2 a thread: loads of a fixed number, so that all are in flight at once
+    const int q = blockIdx.x * kImageThreads + t, pairs1 = a.chunks * 128 * 32;
+    const bool first = q < pairs1;
+    const int at = first ? q : q - pairs1, row = (at >> 5) & 127, chunk = at >> 12, k0 = chunk * 64 + 2 * (at & 31);
+    float v[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        v[i] = first ? (k0 + i < a.in ? __ldg(a.W1 + row * a.s1o + (k0 + i) * a.s1i) : 0.f) : (k0 + i < a.out ? __ldg(a.W2 + (k0 + i) * a.s2o + row * a.s2i) : 0.f);
+    constexpr int kRows1 = 8, kColumns1 = (kCkMaxIn + 31) / 32, kRows2 = 128 * kCkMaxOut / kImageThreads;
+    float v1[kRows1][kColumns1], v2[kRows2];
+#pragma unroll
+    for (int r = 0; r < kRows1; ++r)
+#pragma unroll
+        for (int i = 0; i < kColumns1; ++i) {
+            const int k = lane + 32 * i;
+            v1[r][i] = k < a.in ? __ldg(a.W1 + (warp + 16 * r) * a.s1o + k * a.s1i) : 0.f;
+        }
+    const int unit2 = t & 127, c0 = t >> 7;
+#pragma unroll
+    for (int i = 0; i < kRows2; ++i) v2[i] = c0 + 4 * i < a.out ? __ldg(a.W2 + (c0 + 4 * i) * a.s2o + unit2 * a.s2i) : 0.f;
+    const float bias = t < 128 ? __ldg(a.b1 + t) : 0.f;
     __syncthreads();
-    unsigned m[3] = {};
-    // every block looks at all weights: they are few, and a launch in between would cost more
-    // (loads of a fixed number, so that all are in flight at once)
-    if (a.s1i == 1 && a.s1o == a.in && (uintptr_t)a.W1 % 16 == 0) {
+    // the largest of rows and columns, the columns as they are: that is what they are in units of their rows unless those lie apart
+    unsigned m1[kRows1], m2[16], column[kColumns1] = {}, column2 = 0;
 #pragma unroll
-        for (int i = 0; i < 32 * kCkMaxIn / 512; ++i) {
-            const int q = threadIdx.x + 512 * i;
-            const float4 v = q < 32 * a.in ? __ldg(reinterpret_cast<const float4 *>(a.W1) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
-            m[0] = max(m[0], max(max(finite_magnitude(v.x), finite_magnitude(v.y)), max(finite_magnitude(v.z), finite_magnitude(v.w))));
-        }
-    } else {
-#pragma unroll 8
-        for (int q = threadIdx.x; q < 128 * a.in; q += 512) {
-            const int j = q / a.in, k = q - j * a.in;
-            m[0] = max(m[0], finite_magnitude(__ldg(a.W1 + j * a.s1o + k * a.s1i)));
+    for (int r = 0; r < kRows1; ++r) {
+        m1[r] = 0;
+#pragma unroll
+        for (int i = 0; i < kColumns1; ++i) {
+            const unsigned m = finite_magnitude(v1[r][i]);
+            m1[r] = max(m1[r], m);
+            column[i] = max(column[i], m);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 128 * kCkMaxOut / 512; ++i) {
-        const int q = threadIdx.x + 512 * i;
-        m[1] = max(m[1], q < 128 * a.out ? finite_magnitude(__ldg(a.W2 + (q >> 7) * a.s2o + (q & 127) * a.s2i)) : 0u);
+    for (int i = 0; i < 16; ++i) {
+        m2[i] = i < kRows2 ? finite_magnitude(v2[i]) : 0u;
+        column2 = max(column2, m2[i]);
     }
-    if (threadIdx.x < 128) m[2] = finite_magnitude(__ldg(a.b1 + threadIdx.x));
+    {
+        const unsigned one = gather_max8(m1), two = gather_max8(*reinterpret_cast<unsigned(*)[8]>(m2)), three = gather_max8(*reinterpret_cast<unsigned(*)[8]>(m2 + 8));
+        if (lane % 4 == 0) {
+            rows1[warp + 16 * (lane / 4)] = one;
+            atomicMax(&rows2[c0 + 4 * (lane / 4)], two);
+            if (lane < 16) atomicMax(&rows2[c0 + 4 * (8 + lane / 4)], three);
+        }
+        const unsigned all1 = warp_max(one), all2 = warp_max(max(two, three));
+        if (lane == 0) {
+            atomicMax(&most[0], all1);
+            atomicMax(&most[1], all2);
+        }
+    }
 #pragma unroll
-    for (int q = 0; q < 3; ++q) {
-        m[q] = warp_max(m[q]);
-        if (threadIdx.x % 32 == 0) atomicMax(&most[q], m[q]);
-    }
+    for (int i = 0; i < kColumns1; ++i) atomicMax(&columns1[lane + 32 * i], column[i]);
+    atomicMax(&columns2[unit2], column2);
     __syncthreads();
     const int e1 = min(binade(most[0]), 126), e2 = min(binade(most[1]), 126);
-    const int pairs1 = a.chunks * 128 * 32, total = pairs1 + 128 * 32;
-    for (int q = blockIdx.x * 512 + threadIdx.x; q < total; q += gridDim.x * 512) {
-        const bool first = q < pairs1;
-        const int at = first ? q : q - pairs1, row = (at >> 5) & 127, c = at >> 12, k = c * 64 + 2 * (at & 31);
-        float v[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            v[i] = first ? (k + i < a.in ? scalbnf(__ldg(a.W1 + row * a.s1o + (k + i) * a.s1i), kOperand - e1) : 0.f)
-                         : (k + i < a.out ? scalbnf(__ldg(a.W2 + (k + i) * a.s2o + row * a.s2i), kOperand - e2) : 0.f);
-        unsigned head, tail;
-        split_halves(v[0], v[1], head, tail);
-        uint8_t *base = a.image + kCkHeader + (first ? (long long)c : 2ll * a.chunks) * kCkTile;
-        const int place = half_place(row, k & 63);
-        *reinterpret_cast<unsigned *>(base + place) = head;
-        *reinterpret_cast<unsigned *>(base + (first ? a.chunks : 1) * kCkTile + place) = tail;
+    int apart1 = 0, apart2 = 0;
+    if (t < 128) {
+        apart1 = hidden1[t] = channel_unit(max(rows1[t], min(finite_magnitude(bias), (unsigned)(e1 + 127) << 23)), e1);
+        const unsigned m = warp_max(bias > 0.f ? finite_magnitude(bias * power_of_two(-apart1)) : 0u);
+        if (lane == 0) atomicMax(&most[2], m);
+    } else if (t < 192) {
+        apart2 = outputs[t - 128] = channel_unit(rows2[t - 128], e2);
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<CkHeader *>(a.image) = CkHeader{e1, e2, most[2] == 0 ? -1000 : binade(most[2])};
+    const int outputs_apart = __syncthreads_or(apart2);
+    if (__syncthreads_or(apart1)) {
+        if (t < 192) columns1[t] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kColumns1; ++i) {
+            unsigned m = 0;
+#pragma unroll
+            for (int r = 0; r < kRows1; ++r) m = max(m, finite_magnitude(v1[r][i] * power_of_two(-hidden1[warp + 16 * r])));
+            atomicMax(&columns1[lane + 32 * i], m);
+        }
+        __syncthreads();
+    }
+    if (outputs_apart) {
+        if (t < 128) columns2[t] = 0;
+        __syncthreads();
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < kRows2; ++i) m = max(m, finite_magnitude(v2[i] * power_of_two(-outputs[c0 + 4 * i])));
+        atomicMax(&columns2[unit2], m);
+        __syncthreads();
+    }
+    int apart = 0;
+    if (t < 192) {
+        apart = inputs[t] = channel_unit(columns1[t], e1);
+    } else if (t < 320) {
+        const int j = t - 192, both = hidden1[j] + (hidden2[j] = channel_unit(columns2[j], e2));
+        atomicMax(&hidden[0], both);
+        atomicMax(&hidden[1], -both);
+    }
+    const int inputs_apart = __syncthreads_or(apart);
+    const int e = first ? e1 + hidden1[row] : e2 + hidden2[row];
+    const int *columns = first ? inputs : outputs;
+    unsigned head, tail;
+    split_halves(times_power(v[0], kOperand - e - columns[k0]), times_power(v[1], kOperand - e - columns[k0 + 1]), head, tail);
+    uint8_t *base = a.image + kCkHeader + (first ? (long long)chunk : 2ll * a.chunks) * kCkTile;
+    const int place = half_place(row, k0 & 63);
+    *reinterpret_cast<unsigned *>(base + place) = head;
+    *reinterpret_cast<unsigned *>(base + (first ? a.chunks : 1) * kCkTile + place) = tail;
+    if (blockIdx.x != 0) return;
+    CkHeader *h = reinterpret_cast<CkHeader *>(a.image);
+    if (t < 128) {
+        h->hidden1[t] = (int8_t)hidden1[t];
+        h->hidden2[t] = (int8_t)hidden2[t];
+    }
+    if (t < 192) h->inputs[t] = (int8_t)inputs[t];
+    if (t < 64) h->outputs[t] = (int8_t)outputs[t];
+    if (t == 0) {
+        h->w1 = e1; h->w2 = e2; h->b1 = most[2] == 0 ? -1000 : binade(most[2]);
+        h->hidden = hidden[0]; h->hidden_apart = hidden[0] != -hidden[1]; h->inputs_apart = inputs_apart; h->outputs_apart = outputs_apart;
+    }
 }
 
 // ---- what both kernels share ---------------------------------------------------------------------------------------------
@@ -229,6 +327,15 @@ struct DyRows {
             *reinterpret_cast<unsigned *>(tails + place) = tail;
         }
     }
+    // The columns in other units: column[] of 64, powers of two.
+    __device__ __forceinline__ void times(const float *column, int lane) {
+        const float2 f = reinterpret_cast<const float2 *>(column)[TWO ? lane : lane & 15];
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            v[i].x *= f.x;
+            v[i].y *= f.y;
+        }
+    }
     // ... and stored as heads and tails in units of their rows, whose exponents go to `units`: a lane works out one row's (four or two
     // lanes the same) and hands it round.
     __device__ __forceinline__ void store_by_row(uint8_t *heads, uint8_t *tails, int *units, int first, int lane) const {
@@ -259,11 +366,30 @@ struct DyRows {
     }
 };
 
-__device__ __forceinline__ void ck_copy_image(uint8_t *dst, const CkArgs &a, uint64_t *bar) {
-    const int tiles = 2 * a.chunks + 2;
+__device__ __forceinline__ void ck_copy_image(uint8_t *dst, const uint8_t *image, int chunks, uint64_t *bar) {
+    const int tiles = 2 * chunks + 2;
     mbar_arrive_expect(bar, (unsigned)(tiles * kCkTile));
-    for (int q = 0; q < tiles; ++q) bulk_copy_g2s(dst + q * kCkTile, a.image + kCkHeader + (long long)q * kCkTile, kCkTile, bar);
+    for (int q = 0; q < tiles; ++q) bulk_copy_g2s(dst + q * kCkTile, image + kCkHeader + (long long)q * kCkTile, kCkTile, bar);
 }
+
+// Channels of the image in other units, once in front of the tiles (a copy has landed, the MMAs have not begun): the rows are multiplied by
+// row[] and the columns by column[], powers of two (NULL: 1).  Only where channels lie apart: a microsecond or two for the 128 KB of 163 inputs.
+__device__ __noinline__ void ck_rescale(uint8_t *heads, uint8_t *tails, int chunks, const float *row, const float *column) {
+    for (int q = threadIdx.x; q < chunks * 128 * 8; q += blockDim.x) {
+        const int r = (q >> 3) & 127, k = (q >> 10) * 64 + (((q & 7) ^ (r & 7)) << 3);
+        const float f = row ? row[r] : 1.f;
+        uint4 head = reinterpret_cast<uint4 *>(heads)[q], tail = reinterpret_cast<uint4 *>(tails)[q];
+        unsigned h[4] = {head.x, head.y, head.z, head.w}, l[4] = {tail.x, tail.y, tail.z, tail.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 a = unpack_halves(h[i]), b = unpack_halves(l[i]);  // (the sum is exact: 22 bits)
+            split_halves((a.x + b.x) * (column ? f * column[k + 2 * i] : f), (a.y + b.y) * (column ? f * column[k + 2 * i + 1] : f), h[i], l[i]);
+        }
+        reinterpret_cast<uint4 *>(heads)[q] = make_uint4(h[0], h[1], h[2], h[3]);
+        reinterpret_cast<uint4 *>(tails)[q] = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+}
+__device__ __forceinline__ float channel_factor(int e) { return power_of_two(max(e, -126)); }
 
 // ---- dz ----------------------------------------------------------------------------------------------------------------
 // Warp-specialised, one persistent CTA per SM, tiles of 128 rows: four producer warps (32 rows of dy each, a tile ahead in registers;
@@ -273,6 +399,8 @@ __device__ __forceinline__ void ck_copy_image(uint8_t *dst, const CkArgs &a, uin
 struct CkDzShared {
     uint64_t image, op_full, op_empty, dh_full[2], dh_ready[2], dz_full, dz_empty, staged[4], copied[4];
     int units[kCkRowRing][kCkRows];
+    alignas(8) float outputs[64], inputs[192];  // units of W2's and W1's columns
+    float hidden[128];                          // what a hidden unit weighs against the largest
     uint32_t tmem_base;
     int abort;
 };
@@ -315,7 +443,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
         mbar_init(&sh.dz_empty, 8);
         sh.abort = 0;
         mbar_fence_init();
+        ck_copy_image(base, a.image, a.chunks, &sh.image);
     }
+    const CkHeader &units = *reinterpret_cast<const CkHeader *>(a.image);
+    const bool inputs_apart = units.inputs_apart, outputs_apart = units.outputs_apart, hidden_apart = units.hidden_apart;
     if (warp == kCkProducer0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -323,6 +454,18 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (inputs_apart || outputs_apart || hidden_apart) {
+        if (threadIdx.x < 64) sh.outputs[threadIdx.x] = channel_factor(units.outputs[threadIdx.x]);
+        if (threadIdx.x < 192) sh.inputs[threadIdx.x] = channel_factor(units.inputs[threadIdx.x]);
+        if (threadIdx.x < 128) sh.hidden[threadIdx.x] = channel_factor(units.hidden1[threadIdx.x] + units.hidden2[threadIdx.x] - units.hidden);
+        __syncthreads();
+        if (hidden_apart) {  // dh with what its hidden unit weighs in dz
+            umma_wait(&sh.image, 0, &sh.abort);
+            ck_rescale(w2, w2 + kCkTile, 1, sh.hidden, nullptr);
+            fence_proxy_async();
+            __syncthreads();
+        }
+    }
     const unsigned tmem = sh.tmem_base;
     const int ntile = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     auto row_of = [&](int it) { return ((long long)blockIdx.x + (long long)it * gridDim.x) * kCkRows; };
@@ -333,7 +476,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
         // tile before
         const bool issues = warp == kCkProducer0;
         const int mine = (warp - kCkProducer0) * 32;
-        if (issues && lane == 0) ck_copy_image(base, a, &sh.image);
         const unsigned id1 = f16_idesc(128, false), id2 = f16_idesc((a.in + 15) / 16 * 16, true);
         const int ks1 = (a.out + 15) / 16;
         const uint64_t w2h = umma_desc(smem_u32(w2)), w2l = umma_desc(smem_u32(w2 + kCkTile));
@@ -375,6 +517,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
 #pragma unroll 1
         for (int t = 0; t < ntile && ok; ++t) {
             if (!(ok = umma_wait(&sh.op_empty, (t & 1) ^ 1, &sh.abort))) break;
+            if (outputs_apart) rows.times(sh.outputs, lane);
             rows.store_by_row(ops, ops + kCkTile, sh.units[t % kCkRowRing], mine, lane);
             fence_proxy_async();
             __syncwarp();
@@ -400,7 +543,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
     } else {
         const int quarter = warp & 3, half = warp >> 2;  // rows 32 quarter + lane; hidden units 64 half and up, every second 16 columns of dz
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
-        const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
+        const int unit_of_w = units.w1 + units.w2 + units.hidden + kDhDown - 3 * kOperand;
         const int buffers = ck_dz_buffers(a.in);  // (with two of them quarters 0 and 2, 1 and 3 take turns)
         float *stg = staged + quarter % buffers * 32 * a.in;
         const bool aligned = (uintptr_t)a.dz % 16 == 0;
@@ -414,9 +557,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             if (!umma_wait(&sh.dz_full, t & 1, &sh.abort)) return false;
             tc_fence_after();
             // the row's unit times those of the weights: one power of two unless it is out of range
-            const int e = sh.units[t % kCkRowRing][quarter * 32 + lane] + head.w1 + head.w2 + kDhDown - 3 * kOperand, e1 = max(min(e, 127), -126);
+            const int e = sh.units[t % kCkRowRing][quarter * 32 + lane] + unit_of_w, e1 = max(min(e, 127), -126);
             const float unit = power_of_two(e1), rest = power_of_two(max(e - e1, -126));
-            const bool far = __any_sync(kFull, e != e1);
+            const bool far = __any_sync(kFull, e != e1) || inputs_apart;
             float *row = stg + lane * a.in;
             auto emptied = [&]() {
                 tc_fence_before();
@@ -434,7 +577,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             auto put = [&](unsigned(&r)[16], int c0, auto full) {
                 if (far) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * rest);
+                    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * rest * (inputs_apart ? sh.inputs[c0 + j] : 1.f));
                 }
                 if constexpr (PIECES) {
                     float v[16];
@@ -534,6 +677,7 @@ struct CkWeightsShared {
     alignas(16) uint8_t exponents[kCkRows * 6];
     float both[kCkRows];
     int z_unit;
+    alignas(8) float inputs[192], outputs[64];  // units of W1's and W2's columns
     uint32_t tmem_base;
     int abort;
 };
@@ -581,7 +725,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         mbar_init(&sh.g2_full, 1);
         sh.abort = 0;
         mbar_fence_init();
+        ck_copy_image(base, a.image, a.chunks, &sh.image);
     }
+    const CkHeader &head = *reinterpret_cast<const CkHeader *>(a.image);
+    const bool inputs_apart = head.inputs_apart, outputs_apart = head.outputs_apart;
     if (warp == kCkProducer0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -589,6 +736,18 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // zh and dy are whole where the image's columns are in units: those come back into it.  (The hidden units are lanes here, and theirs
+    // come in at the end.)
+    if (inputs_apart || outputs_apart) {
+        if (threadIdx.x < 192) sh.inputs[threadIdx.x] = channel_factor(head.inputs[threadIdx.x]);
+        if (threadIdx.x < 64) sh.outputs[threadIdx.x] = channel_factor(head.outputs[threadIdx.x]);
+        __syncthreads();
+        umma_wait(&sh.image, 0, &sh.abort);
+        if (inputs_apart) ck_rescale(base, base + a.chunks * kCkTile, a.chunks, nullptr, sh.inputs);
+        if (outputs_apart) ck_rescale(w2, w2 + kCkTile, 1, nullptr, sh.outputs);
+        fence_proxy_async();
+        __syncthreads();
+    }
     const unsigned tmem = sh.tmem_base;
     const int ntile = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     auto row_of = [&](int it) { return ((long long)blockIdx.x + (long long)it * gridDim.x) * kCkRows; };
@@ -597,7 +756,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
     if (warp >= kCkProducer0) {
         // the first of the producers issues the products that make the A operands (one lane)
         const bool issues = warp == kCkProducer0;
-        if (issues && lane == 0) ck_copy_image(base, a, &sh.image);
         // (operands are described where they are used: kept over the loop they would cost the producers their registers, and a spilled
         // register comes back from L2)
         const int chunks = a.chunks;
@@ -732,7 +890,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
     } else {
         const int quarter = warp & 3, half = warp >> 2;  // hidden units 32 quarter + lane, rows 64 half .. + 63 of a tile
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
-        const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
+        const int w1 = head.w1, w2_unit = head.w2 + kDhDown - 2 * kOperand;
         // a lane of the first warp issues the sums over the rows: it knows first that their operands are there
         auto sums_of_w1 = [&](int t) -> bool {
             if (!umma_wait(&sh.dh_ready, t & 1, &sh.abort)) return false;  // which also says that tile t - 1 has left its accumulators
@@ -757,7 +915,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             umma_commit(&sh.g2_full);
             return true;
         };
-        const float b1 = __ldg(a.b1 + quarter * 32 + lane);
+        const int unit1 = head.hidden1[quarter * 32 + lane];
+        const float b1 = __ldg(a.b1 + quarter * 32 + lane) * power_of_two(-unit1);
+        const int b1_unit = b1 > 0.f && finite_magnitude(b1) ? binade(finite_magnitude(b1)) : -1000;  // (below zero it makes h smaller)
         const int nb1 = (a.in + 15) / 16, nb = nb1 + (a.out + 15) / 16;
         float sums[kBlocks][16], db = 0.f;
 #pragma unroll
@@ -806,8 +966,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             __syncwarp();
             // units: zh 2^zu, W1 2^(w1 - 14); h in units of 2^hu, which the largest sum (176 x 2^15 x 32512 in the accumulator's) and bias leave
             // below 1.2 x 2^15
-            const int unit = sh.dy_unit, zu = sh.z_unit, hu = max(zu + head.w1 + 24, head.b1 + 2) - 15;
-            const float to_h = power_of_two(max(zu + head.w1 - kOperand - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
+            const int unit = sh.dy_unit, zu = sh.z_unit, hu = max(zu + w1 + 24, b1_unit + 2) - 15;
+            const float to_h = power_of_two(max(zu + w1 - kOperand - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
             if (!umma_wait(&sh.pre_full, t & 1, &sh.abort, kUmmaWaitNs, 50)) ok = false;
             tc_fence_after();
             apart(tlane + kCkPreCol, [&](float v, bool alive, int) { return alive ? __fmaf_rn(v, to_h, bias) : 0.f; });
@@ -818,11 +978,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             if (!(ok = __shfl_sync(kFull, (int)ok, 0) != 0)) break;
             // what the tile's sums are multiples of: products of powers of two, zero where they fall below the smallest number
             auto scale = [](int e) { return power_of_two(max(min(e, 127), -126)) * power_of_two(max(min(e + 126, 0), -126)); };
-            db += (partial[0] + partial[1] + (partial[2] + partial[3])) * scale(unit + head.w2 + kDhDown - 2 * kOperand);
+            db += (partial[0] + partial[1] + (partial[2] + partial[3])) * scale(unit + w2_unit);
             if (!(ok = umma_wait(&sh.g1_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
             tc_fence_after();
             bool both = false;  // dW2's sums are there as well
-            const float f1 = scale(unit + head.w2 + kDhDown - 2 * kOperand + zu), f2 = scale(unit - kOperand + hu);
+            const float f1 = scale(unit + w2_unit + zu), f2 = scale(unit - kOperand + hu);
 #pragma unroll
             for (int i = 0; i < kBlocks; ++i) {
                 const int b = 2 * i + half;
@@ -844,6 +1004,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         }
         if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_EPILOGUE);
         // db1 in column `in`: both halves of the rows through shared memory.  (A warp that gave up comes here as well: the barriers want all.)
+        const float f1 = channel_factor(head.hidden2[quarter * 32 + lane]), f2 = channel_factor(unit1);
+        db *= f1;
         float *prow = a.partial + ((long long)blockIdx.x * 128 + quarter * 32 + lane) * (a.N1p + a.N2p);
         if (half == 1) sh.both[quarter * 32 + lane] = db;
 #pragma unroll
@@ -851,8 +1013,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             const int b = 2 * i + half;
             if (b >= nb) break;
             float *to = prow + (b < nb1 ? 16 * b : a.N1p + 16 * (b - nb1));
+            const float f = b < nb1 ? f1 : f2;
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4 *>(to + j) = make_float4(sums[i][j], sums[i][j + 1], sums[i][j + 2], sums[i][j + 3]);
+            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4 *>(to + j) = make_float4(sums[i][j] * f, sums[i][j + 1] * f, sums[i][j + 2] * f, sums[i][j + 3] * f);
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");  // (column `in` may lie in a block of the other half)
         if (half == 0) prow[a.in] = db + sh.both[quarter * 32 + lane];
@@ -881,6 +1044,7 @@ struct CkForwardShared {
     uint64_t image, slot_full[kFwSlots], slot_empty[kFwSlots], h_full[2], h_ready[2], y_full[2], y_read[2], y_written, y_copied;
     alignas(16) float b1[128];
     int units[4][kCkRows];
+    alignas(8) float inputs[192], outputs[64], hidden[128];  // units of W1's and W2's columns, and what a hidden unit weighs against the largest
     uint32_t tmem_base;
     int abort;
 };
@@ -922,8 +1086,11 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
         mbar_init(&sh.y_copied, 4);
         sh.abort = 0;
         mbar_fence_init();
+        ck_copy_image(base, a.image, kChunks, &sh.image);
     }
-    if (threadIdx.x < 128) sh.b1[threadIdx.x] = __ldg(a.b1 + threadIdx.x);
+    const CkHeader &head = *reinterpret_cast<const CkHeader *>(a.image);
+    const bool inputs_apart = head.inputs_apart, outputs_apart = head.outputs_apart, hidden_apart = head.hidden_apart;
+    if (threadIdx.x < 128) sh.b1[threadIdx.x] = __ldg(a.b1 + threadIdx.x) * power_of_two(-head.hidden1[threadIdx.x]);
     if (warp == kFwProducers) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -931,6 +1098,18 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (inputs_apart || outputs_apart || hidden_apart) {
+        if (threadIdx.x < 64) sh.outputs[threadIdx.x] = channel_factor(head.outputs[threadIdx.x]);
+        if (threadIdx.x < 192) sh.inputs[threadIdx.x] = channel_factor(head.inputs[threadIdx.x]);
+        if (threadIdx.x < 128) sh.hidden[threadIdx.x] = channel_factor(head.hidden1[threadIdx.x] + head.hidden2[threadIdx.x] - head.hidden);
+        __syncthreads();
+        if (hidden_apart) {  // W2 with what its hidden unit weighs in y
+            umma_wait(&sh.image, 0, &sh.abort);
+            ck_rescale(w2, w2 + kCkTile, 1, sh.hidden, nullptr);
+            fence_proxy_async();
+            __syncthreads();
+        }
+    }
     const unsigned tmem = sh.tmem_base;  // h of two tiles at 0 and 128, what goes with tails (then y) at 256 and 384
     const int ntile = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     auto row_of = [&](int it) { return ((long long)blockIdx.x + (long long)it * gridDim.x) * kCkRows; };
@@ -946,7 +1125,6 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
         for (int t = 0; t < ntile && ok; ++t) {
             const long long row0 = row_of(t) + first;
             float2 v[8][kChunks];
-            unsigned row_most[8];
             {
                 const int k = 64 * (kChunks - 1) + 2 * lane, in = worked_out_here(a.in);
                 const bool one = k < a.in, two = k + 1 < a.in;
@@ -962,8 +1140,6 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                     }
                 }
             }
-#pragma unroll
-            for (int r = 0; r < 8; ++r) row_most[r] = 0;
             // codes are put together in this warp's rows of the slot that the first chunk is going to: five rows where its heads will be,
             // three where its tails (in two bytes a lane they would go to memory in pieces of sectors, which cost 13,000 clocks a tile)
             if (!(ok = umma_wait(&sh.slot_empty[s], ph, &sh.abort))) break;
@@ -1017,6 +1193,21 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                 }
             }
             __syncwarp();
+            if (inputs_apart) {  // in units of W1's columns, of which the row's largest is another
+                unsigned m[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    m[r] = 0;
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c) {
+                        const float2 f = reinterpret_cast<const float2 *>(sh.inputs)[32 * c + lane];
+                        v[r][c].x *= f.x;
+                        v[r][c].y *= f.y;
+                        m[r] = max(m[r], max(finite_magnitude(v[r][c].x), finite_magnitude(v[r][c].y)));
+                    }
+                }
+                own = __shfl_sync(kFull, gather_max8(m), 4 * ((lane & 15) >> 1));
+            }
             const unsigned field = row_unit(own);
             if (lane < 16 && (lane & 1) == 0) sh.units[t & 3][first + (lane >> 1)] = (int)field - 127;
             const float scale = from_row_unit(field);
@@ -1054,11 +1245,6 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
         const int quarter = warp & 3, row = quarter * 32 + lane;
         // a lane of the first warp issues the MMAs as well: while the producers fill the slots there is little else for it to do
         const bool issues = quarter == 0;
-        if (issues && lane == 0) {
-            const int tiles = 2 * kChunks + 2;
-            mbar_arrive_expect(&sh.image, (unsigned)(tiles * kCkTile));
-            for (int q = 0; q < tiles; ++q) bulk_copy_g2s(base + q * kCkTile, a.image + kCkHeader + (long long)q * kCkTile, kCkTile, &sh.image);
-        }
         auto first_layer = [&](int t) -> bool {
             const int b = t & 1, steps = (a.in + 15) / 16;
             const unsigned id1 = f16_idesc(128, false);
@@ -1106,13 +1292,13 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
             return did;
         };
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
-        const CkHeader head = *reinterpret_cast<const CkHeader *>(a.image);
+        const int w1 = head.w1, b1_unit = head.b1, w2_unit = head.w2 + head.hidden - kOperand;
         // h is below 2^(zr + w1 + 10) by its products (176 of numbers below two units each) and 2^(b1 + 1) by its bias: twice 2^14 of its units
-        auto unit_of = [&](int t) { return max(sh.units[t & 3][row] + head.w1 + 10, head.b1 + 1) - 14; };
+        auto unit_of = [&](int t) { return max(sh.units[t & 3][row] + w1 + 10, b1_unit + 1) - 14; };
         auto leave = [&](int t) -> bool {  // y of tile t
             const int b = t & 1;
             const long long row0 = row_of(t);
-            const int e = unit_of(t) + head.w2 - kOperand, e1 = max(min(e, 127), -126);
+            const int e = unit_of(t) + w2_unit, e1 = max(min(e, 127), -126);
             const float unit = power_of_two(e1), rest = power_of_two(max(e - e1, -126));
             if (!umma_wait(&sh.y_copied, (t & 1) ^ 1, &sh.abort)) return false;
             if (!umma_wait(&sh.y_full[b], (t >> 1) & 1, &sh.abort)) return false;
@@ -1125,6 +1311,10 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                 float y[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]) * unit * rest;
+                if (outputs_apart) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) y[j] *= sh.outputs[c0 + j];
+                }
                 put_16(ytile + row * a.out + c0, a.out - c0, a.out, lane, y);
             }
             tc_fence_before();
@@ -1150,7 +1340,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
             if (!(ok = umma_wait(&sh.h_full[b], (t >> 1) & 1, &sh.abort))) break;
             tc_fence_after();
             const int hu = unit_of(t);
-            const float f1 = power_of_two(max(sh.units[t & 3][row] + head.w1 - 2 * kOperand - hu, -126)), f2 = power_of_two(min(max(-hu, -126), 127));
+            const float f1 = power_of_two(max(sh.units[t & 3][row] + w1 - 2 * kOperand - hu, -126)), f2 = power_of_two(min(max(-hu, -126), 127));
             unsigned bits[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) bits[w] = 0;
@@ -1257,7 +1447,7 @@ int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1,
     if (!(a.status = umma_status_word())) return fail(NPA_ERR_CUDA, "%s: no status word", me);
     const cudaStream_t st = (cudaStream_t)stream;
     const CkImageArgs make{W1, b1, W2, w1_stride_out, w1_stride_in, w2_stride_out, w2_stride_in, in_dim, out_dim, a.chunks, static_cast<uint8_t *>(image)};
-    launch_early(mlp_checkpoint_image_kernel, 8 * (a.chunks + 1), 512, 0, st, make);
+    launch_early(mlp_checkpoint_image_kernel, ck_image_blocks(a.chunks), kImageThreads, 0, st, make);
     if ((rc = check_launch("mlp_checkpoint_image_kernel")) != NPA_OK) return rc;
     const auto kernel = a.chunks == 1 ? mlp_checkpoint_forward_kernel<1> : a.chunks == 2 ? mlp_checkpoint_forward_kernel<2> : mlp_checkpoint_forward_kernel<3>;
     const int smem = ck_forward_smem(a.chunks, out_dim);

@@ -97,12 +97,12 @@ CASES = {
     "outputs": {"w2_out": 1},
     "outputs against their gradients": {"w2_out": 1, "up": -1},
     "gradients": {"up": 1},
+    "everything": {"z": 1, "w1_in": -1, "w1_out": 1, "b1": 1, "w2_in": -1, "w2_out": 1, "up": -1},
 }
 
 
 @pytest.mark.parametrize("rows,k,o", [(300, 66, 18), (1500, 163, 35)])
-@pytest.mark.parametrize("how", ["half"])
-@pytest.mark.parametrize("case", list(CASES))
+@pytest.mark.parametrize("case,how", [(c, h) for c in CASES for h in ("half", "mixed", "rising") if h == "half" or not {"z", "up"} & set(CASES[c])])
 def test_channels_of_different_size(case, how, rows, k, o):
     w1, b1, w2 = _weights(k, o, 1)
     z, up = _rand(2 * rows, k, seed=2), _rand(2 * rows, o, seed=3)
