@@ -677,8 +677,9 @@ int npa_rows8_restore(const void *codes, int64_t codes_pitch, const uint8_t *exp
 
 /* The adaptation MLP (hidden width 128, in <= 176, out <= 48) whose backward reads z in 8 bits.  The forward leaves
  * codes [rows, in rounded up to 16], exponents, mask [rows, 4] with the bits of h > 0 (unit 32 w + i is bit i of word w),
- * and an image of the weights (npa_mlp_checkpoint_image_bytes() bytes) as the tensor cores read them, which is the
- * backward's as well; the backward makes the hidden layer again.  dz may be NULL, and dW1, db1 and dW2 together.  codes,
+ * and an image (npa_mlp_checkpoint_image_bytes() bytes): the weights as the tensor cores read them, and the sizes of z's
+ * groups of columns.  The backward takes all four for the same rows, and makes the hidden layer again.  dz may be NULL, and dW1, db1
+ * and dW2 together.  codes,
  * exponents, mask, image, dy and scratch 16-byte aligned; waits are bounded as in npa_linear_tcgen05, whose status has
  * bits 1024, 2048, 4096 for the MMA lane, producers and epilogue of these kernels. */
 int64_t npa_mlp_checkpoint_image_bytes(int32_t in_dim);

@@ -15,8 +15,8 @@
 //     any size keep their own accuracy.  A unit of a summed index goes to the other operand or comes back into the image once in front of the
 //     tiles; one of an index that stays comes back in the epilogue.  Weights that lie together take neither way;
 //   * z in the forward, and dy for dz, in units of their row: rows of any size keep their accuracy, and the unit comes back in the epilogue;
-//   * dy and zh for the sums over rows in the unit of the largest of their tile of 128 rows; a tile's unit comes in when its sum leaves the
-//     accumulator;
+//   * dy and zh for the sums over rows in the unit of the largest of their tile of 128 rows, which comes in when the tile's sum leaves the
+//     accumulator, and, where they lie apart, of their column and group of columns (ck_look);
 //   * h in a unit that its products and the largest bias cannot exceed, dh times a power of two that brings its largest sum back in range.
 //
 // The largest of a unit is an operand of 2^14 to 2^15 (accumulators have 32 bits, only operands are short), which leaves 22 bits to what is
@@ -287,6 +287,9 @@ struct CkArgs {
     const float *dy, *b1;
     const uint8_t *image;
     float *dz, *partial;   // dz [rows, in]; partial [ctas][128][N1p + N2p], db1 in column `in`
+    unsigned *dy_columns;  // [ctas][kCkProducers][64]: the largest finite magnitude of each column of dy in a warp's rows, the same in both kernels
+    int looked;            // whether they are there (the weights' kernel looks for itself otherwise)
+    const uint8_t *z_groups;  // [ctas][8]: the largest exponent of each group of z, in the same rows
     long long rows;
     int in, out, pitch, chunks, N1p, N2p, tiles;
     unsigned *status;
@@ -318,18 +321,18 @@ struct DyRows {
             v[i].y = there && two ? __ldg(p + i * kEach * out + 1) : 0.f;
         }
     }
-    __device__ __forceinline__ void put(uint8_t *heads, uint8_t *tails, int first, int i, float scale, int lane) const {
+    __device__ __forceinline__ void put(uint8_t *heads, uint8_t *tails, int first, int i, float2 scale, int lane) const {
         unsigned head, tail;
-        split_halves(v[i].x * scale, v[i].y * scale, head, tail);
+        split_halves(v[i].x * scale.x, v[i].y * scale.y, head, tail);
         const int place = half_place(first + (TWO ? 0 : lane >> 4) + i * kEach, TWO ? 2 * lane : 2 * (lane & 15));  // (`first` is a multiple of 32)
         if (!TWO || lane < 24) {
             *reinterpret_cast<unsigned *>(heads + place) = head;
             *reinterpret_cast<unsigned *>(tails + place) = tail;
         }
     }
-    // The columns in other units: column[] of 64, powers of two.
-    __device__ __forceinline__ void times(const float *column, int lane) {
-        const float2 f = reinterpret_cast<const float2 *>(column)[TWO ? lane : lane & 15];
+    // The columns in other units: units[] of 64, powers of two.
+    __device__ __forceinline__ void times(const float *units, int lane) {
+        const float2 f = reinterpret_cast<const float2 *>(units)[column(lane)];
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
             v[i].x *= f.x;
@@ -338,32 +341,52 @@ struct DyRows {
     }
     // ... and stored as heads and tails in units of their rows, whose exponents go to `units`: a lane works out one row's (four or two
     // lanes the same) and hands it round.
-    __device__ __forceinline__ void store_by_row(uint8_t *heads, uint8_t *tails, int *units, int first, int lane) const {
+    __device__ __forceinline__ void store_by_row(uint8_t *heads, uint8_t *tails, int *units, int first, int lane, uint2 &most) const {
         constexpr int kLanes = TWO ? 32 : 16;
 #pragma unroll
         for (int i0 = 0; i0 < kPasses; i0 += 8) {
             unsigned m[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m[i] = max(finite_magnitude(v[i0 + i].x), finite_magnitude(v[i0 + i].y));
+            for (int i = 0; i < 8; ++i) {
+                const unsigned x = finite_magnitude(v[i0 + i].x), y = finite_magnitude(v[i0 + i].y);
+                most = make_uint2(max(most.x, x), max(most.y, y));
+                m[i] = max(x, y);
+            }
             const unsigned field = row_unit(gather_max8<kLanes>(m));
             const float scale = from_row_unit(field);
             const int pass = i0 + (lane & (kLanes - 1)) / (kLanes / 8);
             if (lane % (kLanes / 8) == 0) units[first + (TWO ? 0 : lane >> 4) + pass * kEach] = (int)field - 127;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) put(heads, tails, first, i0 + i, __shfl_sync(kFull, scale, max8_lane<kLanes>(i)), lane);
+            for (int i = 0; i < 8; ++i) {
+                const float u = __shfl_sync(kFull, scale, max8_lane<kLanes>(i));
+                put(heads, tails, first, i0 + i, make_float2(u, u), lane);
+            }
         }
     }
-    // The largest finite magnitude of the warp's rows; and heads and tails in one unit.
-    __device__ __forceinline__ unsigned largest() const {
-        unsigned m = 0;
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) m = max(m, max(finite_magnitude(v[i].x), finite_magnitude(v[i].y)));
-        return warp_max(m);
+    // The largest of a lane's two columns (in `units`, where they are in any) to memory as they were, [32] pairs a warp.
+    static __device__ __forceinline__ void put_columns(unsigned *to, uint2 most, const float *units, int lane) {
+        if (!TWO) most = make_uint2(max(most.x, __shfl_xor_sync(kFull, most.x, 16)), max(most.y, __shfl_xor_sync(kFull, most.y, 16)));
+        if (units) {
+            const float2 f = reinterpret_cast<const float2 *>(units)[column(lane)];
+            most = make_uint2(finite_magnitude(__uint_as_float(most.x) / f.x), finite_magnitude(__uint_as_float(most.y) / f.y));
+        }
+        reinterpret_cast<uint2 *>(to)[lane] = TWO || lane < 16 ? most : make_uint2(0, 0);
     }
-    __device__ __forceinline__ void store(uint8_t *heads, uint8_t *tails, float scale, int first, int lane) const {
+    // The largest finite magnitude of the warp's rows with the columns times `f`; and heads and tails of the columns times `scale`.
+    __device__ __forceinline__ unsigned largest(float2 f) const {
+        unsigned x = 0, y = 0;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            x = max(x, finite_magnitude(v[i].x));
+            y = max(y, finite_magnitude(v[i].y));
+        }
+        return warp_max(max(finite_magnitude(__uint_as_float(x) * f.x), finite_magnitude(__uint_as_float(y) * f.y)));
+    }
+    __device__ __forceinline__ void store(uint8_t *heads, uint8_t *tails, float2 scale, int first, int lane) const {
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) put(heads, tails, first, i, scale, lane);
     }
+    static __device__ __forceinline__ int column(int lane) { return TWO ? lane : lane & 15; }  // this lane's pair of columns
 };
 
 __device__ __forceinline__ void ck_copy_image(uint8_t *dst, const uint8_t *image, int chunks, uint64_t *bar) {
@@ -374,8 +397,8 @@ __device__ __forceinline__ void ck_copy_image(uint8_t *dst, const uint8_t *image
 
 // Channels of the image in other units, once in front of the tiles (a copy has landed, the MMAs have not begun): the rows are multiplied by
 // row[] and the columns by column[], powers of two (NULL: 1).  Only where channels lie apart: a microsecond or two for the 128 KB of 163 inputs.
-__device__ __noinline__ void ck_rescale(uint8_t *heads, uint8_t *tails, int chunks, const float *row, const float *column) {
-    for (int q = threadIdx.x; q < chunks * 128 * 8; q += blockDim.x) {
+__device__ __noinline__ void ck_rescale(uint8_t *heads, uint8_t *tails, int chunks, const float *row, const float *column, int threads) {
+    for (int q = threadIdx.x; q < chunks * 128 * 8; q += threads) {
         const int r = (q >> 3) & 127, k = (q >> 10) * 64 + (((q & 7) ^ (r & 7)) << 3);
         const float f = row ? row[r] : 1.f;
         uint4 head = reinterpret_cast<uint4 *>(heads)[q], tail = reinterpret_cast<uint4 *>(tails)[q];
@@ -461,7 +484,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
         __syncthreads();
         if (hidden_apart) {  // dh with what its hidden unit weighs in dz
             umma_wait(&sh.image, 0, &sh.abort);
-            ck_rescale(w2, w2 + kCkTile, 1, sh.hidden, nullptr);
+            ck_rescale(w2, w2 + kCkTile, 1, sh.hidden, nullptr, blockDim.x);
             fence_proxy_async();
             __syncthreads();
         }
@@ -513,12 +536,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             return true;
         };
         DyRows<TWO> rows;
+        uint2 most = make_uint2(0, 0);
         if (ntile > 0) rows.load(a, row_of(0) + mine, lane);
 #pragma unroll 1
         for (int t = 0; t < ntile && ok; ++t) {
             if (!(ok = umma_wait(&sh.op_empty, (t & 1) ^ 1, &sh.abort))) break;
             if (outputs_apart) rows.times(sh.outputs, lane);
-            rows.store_by_row(ops, ops + kCkTile, sh.units[t % kCkRowRing], mine, lane);
+            rows.store_by_row(ops, ops + kCkTile, sh.units[t % kCkRowRing], mine, lane, most);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
@@ -535,6 +559,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
                 ok = __shfl_sync(kFull, (int)ok, 0) != 0;
             }
         }
+        rows.put_columns(a.dy_columns + (blockIdx.x * kCkProducers + warp - kCkProducer0) * 64, most, outputs_apart ? sh.outputs : nullptr, lane);
         if (!ok && lane == 0) {
             atomicOr(a.status, issues ? CK_STATUS_MMA : CK_STATUS_PRODUCER);
             __nanosleep(20000);  // copies in flight land before the CTA leaves
@@ -670,14 +695,22 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
 // meanwhile, its own mask 1,900 with dW1's products meanwhile, dW2's products 1,700 with the next zh (2,400) meanwhile.  In the order zh,
 // dy, products, masks, sums it was 24,000.
 struct CkWeightsShared {
-    uint64_t image, op_full, z_empty, dy_empty, dy_known, dh_full, pre_full, dh_ready, pre_ready, g1_full, g2_full;
+    uint64_t image, units, op_full, z_empty, dy_empty, dy_known, dh_full, pre_full, dh_ready, pre_ready, g1_full, g2_full;
     alignas(16) unsigned mask[4][kCkRows];
     unsigned dy_most[2][kCkProducers];     // of two tiles: largest finite magnitude of each producer's rows
     int dy_unit;
     alignas(16) uint8_t exponents[kCkRows * 6];
     float both[kCkRows];
     int z_unit;
-    alignas(8) float inputs[192], outputs[64];  // units of W1's and W2's columns
+    // of this CTA's rows: the largest finite dy of each column, the largest exponent of each group of z, the magnitudes of each column's codes
+    // (a byte each, whose first bit is that of the largest); and what follows from them (ck_own_units)
+    unsigned dy_columns[64], z_groups[8], used[44];
+    alignas(8) float inputs[192], outputs[64];  // factors of the image's columns
+    alignas(8) float dy_units[64], dy_back[64];
+    float z_back[8];
+    unsigned z_shift[kCkRows * 6 / 4];  // what a tile's exponents are moved by, four a word
+    uint8_t z_move[8];
+    int add1, add2, most1, apart, least_field;
     uint32_t tmem_base;
     int abort;
 };
@@ -703,6 +736,107 @@ __device__ __forceinline__ void decode_codes(const uint4 &q, __half2 scale, uint
     hi = make_uint4(out[4], out[5], out[6], out[7]);
 }
 
+// A gradient of W2 sums one column of dy, and one of W1 a group of z's: neither has to do with the size of the others.  So a column of dy, and a
+// group of z, whose largest in this CTA's rows lies far below the largest of all has a unit of its own: it is multiplied by a power of two,
+// the image's column by the inverse (dh and zh W1^T sum over them), and the power comes back when the CTA's sums leave.  Columns of W1 come out
+// of their own units on the same way, in the unit of the largest that meets a code (a column whose codes are all zero has no size).
+// The epilogue's warps see to this in front of the tiles, while the producers have the first one's loads on their way.  The sizes are those
+// that the forward (groups of z) and dz's kernel (columns of dy) saw in the same rows; where dz was not asked for dy is read once more (141 ->
+// 150 us for 262,144 rows of 163 and 35), and so are the codes where columns of W1 lie apart.
+constexpr int kGroupsApart = 16, kGroupsFarthest = 120;  // zh is exact 2^32 below the largest of its tile: 2^16 are left to the rows
+constexpr int kCkLook = 256;
+enum { CK_APART_W1 = 1, CK_APART_W2 = 2, CK_APART_Z = 4 };
+template <typename Row>
+__device__ __forceinline__ void ck_look(CkWeightsShared &sh, const CkArgs &a, int ntile, Row row_of, bool codes, unsigned seen_dy, unsigned seen_z) {
+    const int t = threadIdx.x, out = a.out;  // (t < kCkLook)
+    const bool last = ntile > 0 && row_of(ntile - 1) + kCkRows >= a.rows;  // this CTA's rows end with the last one
+    if (t < 8) sh.z_groups[t] = seen_z;
+    if (seen_dy) atomicMax(&sh.dy_columns[t % 64], seen_dy);
+    // a thread goes on by a multiple of the columns, so that it stays in the same ones
+    if (!a.looked) {
+        const int turn = kCkLook / out * out, each = 32 * out, total = ntile * each;
+        const long long end = a.rows * out;
+        unsigned m[4] = {};
+        if (t < turn) {
+#pragma unroll 8
+            for (int i = t; i < total; i += turn) {
+                const int tile = i / each;
+                const long long at = row_of(tile) * out + 4 * (i - tile * each);
+                const float4 v = at + 4 <= end ? __ldg(reinterpret_cast<const float4 *>(a.dy + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                m[0] = max(m[0], finite_magnitude(v.x));
+                m[1] = max(m[1], finite_magnitude(v.y));
+                m[2] = max(m[2], finite_magnitude(v.z));
+                m[3] = max(m[3], finite_magnitude(v.w));
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) atomicMax(&sh.dy_columns[(4 * t + q) % out], m[q]);
+        }
+        if (last && t < (int)(end & 3)) atomicMax(&sh.dy_columns[((end & ~3ll) + t) % out], finite_magnitude(__ldg(a.dy + (end & ~3ll) + t)));
+    }
+    if (codes) {
+        const int units = a.pitch / 16, turn = kCkLook / units * units, each = kCkRows * units, total = ntile * each;
+        uint4 any = make_uint4(0, 0, 0, 0);
+        if (t < turn) {
+#pragma unroll 4
+            for (int i = t; i < total; i += turn) {
+                const int tile = i / each;
+                const long long at = row_of(tile) * units + (i - tile * each);
+                const uint4 v = at < a.rows * units ? __ldg(reinterpret_cast<const uint4 *>(a.codes) + at) : make_uint4(0, 0, 0, 0);
+                any.x |= __vabs4(v.x); any.y |= __vabs4(v.y); any.z |= __vabs4(v.z); any.w |= __vabs4(v.w);
+            }
+            const int u = t % units;
+            atomicOr(&sh.used[4 * u], any.x);
+            atomicOr(&sh.used[4 * u + 1], any.y);
+            atomicOr(&sh.used[4 * u + 2], any.z);
+            atomicOr(&sh.used[4 * u + 3], any.w);
+        }
+    }
+}
+__device__ __forceinline__ void ck_look_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kCkLook) : "memory"); }
+// Behind a barrier of those threads; ends with one.
+__device__ __forceinline__ void ck_own_units(CkWeightsShared &sh, const CkArgs &a, const CkHeader &head, bool inputs_apart, bool outputs_apart) {
+    const int t = threadIdx.x, lane = t & 31;
+    int mine = 0;
+    bool counts = false;
+    if (t < 64) {
+        const unsigned all = warp_max(max(sh.dy_columns[lane], sh.dy_columns[lane + 32]));  // (columns that do not exist are zero)
+        const int p = channel_unit(sh.dy_columns[t], binade(all));
+        sh.dy_units[t] = power_of_two(-p);
+        sh.dy_back[t] = power_of_two(p);
+        counts = t < a.out;
+        mine = p + (outputs_apart ? head.outputs[t] : 0);
+        if (counts) atomicMax(&sh.add2, mine);
+        if (p) atomicMax(&sh.least_field, kOperand + 1 - p);  // (no power of two leaves 32 bits)
+    } else {
+        const int k = t - 64, g = k / 32;
+        const unsigned all = warp_max(sh.z_groups[lane & 7]);
+        const int far = (int)sh.z_groups[g] - (int)all, q = sh.z_groups[g] == 0 || far > -kGroupsApart ? 0 : max(far, -kGroupsFarthest);
+        if (k % 32 == 0) {
+            sh.z_back[g] = channel_factor(q);
+            sh.z_move[g] = (uint8_t)-q;
+            if (q) atomicOr(&sh.apart, CK_APART_Z);
+        }
+        const unsigned codes = !inputs_apart ? 127u : k < a.in ? sh.used[k / 4] >> (8 * (k % 4)) & 0xffu : 0u;
+        counts = k < a.in && codes != 0;
+        mine = q + (inputs_apart ? head.inputs[k] : 0);
+        if (counts) {
+            atomicMax(&sh.add1, mine);
+            atomicMax(&sh.most1, mine - (__clz(codes) - 25));
+        }
+    }
+    ck_look_barrier();
+    if (t < 64) {
+        sh.outputs[t] = counts ? channel_factor(mine - sh.add2) : 0.f;
+        if (counts && mine != sh.add2) atomicOr(&sh.apart, CK_APART_W2);
+    } else {
+        sh.inputs[t - 64] = counts ? channel_factor(mine - sh.add1) : 0.f;
+        if (counts && mine != sh.add1) atomicOr(&sh.apart, CK_APART_W1);
+    }
+    if (sh.apart & CK_APART_Z)
+        for (int b = t; b < kCkRows * 6; b += kCkLook) reinterpret_cast<uint8_t *>(sh.z_shift)[b] = sh.z_move[b % ((a.in + 31) / 32)];
+    ck_look_barrier();
+}
+
 template <int kBlocks, bool TWO>
 __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(const __grid_constant__ CkArgs a) {
     after_previous_kernel();
@@ -723,12 +857,20 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         mbar_init(&sh.pre_ready, 8);
         mbar_init(&sh.g1_full, 1);
         mbar_init(&sh.g2_full, 1);
+        mbar_init(&sh.units, 8);
         sh.abort = 0;
         mbar_fence_init();
         ck_copy_image(base, a.image, a.chunks, &sh.image);
     }
     const CkHeader &head = *reinterpret_cast<const CkHeader *>(a.image);
     const bool inputs_apart = head.inputs_apart, outputs_apart = head.outputs_apart;
+    static_assert(64 * kCkProducers == kCkLook, "a word a thread");
+    const unsigned seen_dy = a.looked && threadIdx.x < kCkLook ? __ldg(a.dy_columns + blockIdx.x * kCkLook + threadIdx.x) : 0u;
+    const unsigned seen_z = threadIdx.x < 8 ? __ldg(a.z_groups + blockIdx.x * 8 + threadIdx.x) : 0u;
+    if (threadIdx.x < 64) sh.dy_columns[threadIdx.x] = 0;
+    else if (threadIdx.x < 72) sh.z_groups[threadIdx.x - 64] = 0;
+    else if (threadIdx.x < 116) sh.used[threadIdx.x - 72] = 0;
+    else if (threadIdx.x == 116) sh.add1 = sh.add2 = sh.most1 = -1000, sh.apart = 0, sh.least_field = kOperand + 1;
     if (warp == kCkProducer0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -736,18 +878,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    // zh and dy are whole where the image's columns are in units: those come back into it.  (The hidden units are lanes here, and theirs
-    // come in at the end.)
-    if (inputs_apart || outputs_apart) {
-        if (threadIdx.x < 192) sh.inputs[threadIdx.x] = channel_factor(head.inputs[threadIdx.x]);
-        if (threadIdx.x < 64) sh.outputs[threadIdx.x] = channel_factor(head.outputs[threadIdx.x]);
-        __syncthreads();
-        umma_wait(&sh.image, 0, &sh.abort);
-        if (inputs_apart) ck_rescale(base, base + a.chunks * kCkTile, a.chunks, nullptr, sh.inputs);
-        if (outputs_apart) ck_rescale(w2, w2 + kCkTile, 1, nullptr, sh.outputs);
-        fence_proxy_async();
-        __syncthreads();
-    }
     const unsigned tmem = sh.tmem_base;
     const int ntile = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     auto row_of = [&](int it) { return ((long long)blockIdx.x + (long long)it * gridDim.x) * kCkRows; };
@@ -823,8 +953,17 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             }
         };
         if (ntile > 0) load(0);
+        ok = umma_wait(&sh.units, 0, &sh.abort);
+        const int apart = sh.apart;
 #pragma unroll 1
         for (int t = 0; t < ntile && ok; ++t) {
+            if (apart & CK_APART_Z) {  // exponents in units of their groups (neither 255 nor a byte that does not exist)
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    const unsigned keep = __vcmpeq4(exps[i], 0xffffffffu) | __vcmpeq4(exps[i], 0u);
+                    exps[i] = __vaddus4(exps[i], sh.z_shift[i * 32 + lane] & ~keep);
+                }
+            }
             unsigned most = 0x07070707u;
 #pragma unroll
             for (int i = 0; i < kWords; ++i) most = __vmaxu4(most, exps[i] & ~__vcmpeq4(exps[i], 0xffffffffu));
@@ -853,7 +992,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
                 *reinterpret_cast<uint4 *>(to + half_place(first + row, k + 8)) = hi;
             }
             // dy: the largest of the tile from the four of them (the sums over its rows want one unit, and dh is as good in it)
-            const unsigned mine = rows.largest();
+            const float2 own = reinterpret_cast<const float2 *>(sh.dy_units)[rows.column(lane)];
+            const unsigned mine = rows.largest(own);
             if (lane == 0) {
                 sh.dy_most[t & 1][warp - kCkProducer0] = mine;
                 mbar_arrive(&sh.dy_known);
@@ -862,9 +1002,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             unsigned field = 0;
 #pragma unroll
             for (int q = 0; q < kCkProducers; ++q) field = max(field, sh.dy_most[t & 1][q]);
-            field = row_unit(field);
+            field = max(row_unit(field), (unsigned)sh.least_field);
             if (!(ok = umma_wait(&sh.dy_empty, (t & 1) ^ 1, &sh.abort))) break;
-            rows.store(dyt, dyt + kCkTile, from_row_unit(field), first, lane);
+            rows.store(dyt, dyt + kCkTile, make_float2(from_row_unit(field) * own.x, from_row_unit(field) * own.y), first, lane);
             sh.mask[0][first + lane] = mask.x;
             sh.mask[1][first + lane] = mask.y;
             sh.mask[2][first + lane] = mask.z;
@@ -890,7 +1030,18 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
     } else {
         const int quarter = warp & 3, half = warp >> 2;  // hidden units 32 quarter + lane, rows 64 half .. + 63 of a tile
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
-        const int w1 = head.w1, w2_unit = head.w2 + kDhDown - 2 * kOperand;
+        ck_look(sh, a, ntile, row_of, inputs_apart, seen_dy, seen_z);
+        ck_look_barrier();
+        ck_own_units(sh, a, head, inputs_apart, outputs_apart);
+        if (sh.apart & (CK_APART_W1 | CK_APART_W2)) {
+            umma_wait(&sh.image, 0, &sh.abort);
+            if (sh.apart & CK_APART_W1) ck_rescale(base, base + a.chunks * kCkTile, a.chunks, nullptr, sh.inputs, kCkLook);
+            if (sh.apart & CK_APART_W2) ck_rescale(w2, w2 + kCkTile, 1, nullptr, sh.outputs, kCkLook);
+            fence_proxy_async();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.units);
+        const int w1 = head.w1, w2_unit = head.w2 + sh.add2 + kDhDown - 2 * kOperand;
         // a lane of the first warp issues the sums over the rows: it knows first that their operands are there
         auto sums_of_w1 = [&](int t) -> bool {
             if (!umma_wait(&sh.dh_ready, t & 1, &sh.abort)) return false;  // which also says that tile t - 1 has left its accumulators
@@ -966,8 +1117,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             __syncwarp();
             // units: zh 2^zu, W1 2^(w1 - 14); h in units of 2^hu, which the largest sum (176 x 2^15 x 32512 in the accumulator's) and bias leave
             // below 1.2 x 2^15
-            const int unit = sh.dy_unit, zu = sh.z_unit, hu = max(zu + w1 + 24, b1_unit + 2) - 15;
-            const float to_h = power_of_two(max(zu + w1 - kOperand - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
+            const int unit = sh.dy_unit, zu = sh.z_unit, hu = max(zu + w1 + max(sh.most1, -400) + 24, b1_unit + 2) - 15;
+            const float to_h = power_of_two(max(zu + w1 + max(sh.add1, -400) - kOperand - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
             if (!umma_wait(&sh.pre_full, t & 1, &sh.abort, kUmmaWaitNs, 50)) ok = false;
             tc_fence_after();
             apart(tlane + kCkPreCol, [&](float v, bool alive, int) { return alive ? __fmaf_rn(v, to_h, bias) : 0.f; });
@@ -1013,9 +1164,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             const int b = 2 * i + half;
             if (b >= nb) break;
             float *to = prow + (b < nb1 ? 16 * b : a.N1p + 16 * (b - nb1));
-            const float f = b < nb1 ? f1 : f2;
+            const float f = b < nb1 ? f1 * sh.z_back[b / 2] : f2, *back = b < nb1 ? nullptr : sh.dy_back + 16 * (b - nb1);
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4 *>(to + j) = make_float4(sums[i][j] * f, sums[i][j + 1] * f, sums[i][j + 2] * f, sums[i][j + 3] * f);
+            for (int j = 0; j < 16; ++j) sums[i][j] *= back ? f * back[j] : f;
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4 *>(to + j) = make_float4(sums[i][j], sums[i][j + 1], sums[i][j + 2], sums[i][j + 3]);
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");  // (column `in` may lie in a block of the other half)
         if (half == 0) prow[a.in] = db + sh.both[quarter * 32 + lane];
@@ -1044,6 +1197,7 @@ struct CkForwardShared {
     uint64_t image, slot_full[kFwSlots], slot_empty[kFwSlots], h_full[2], h_ready[2], y_full[2], y_read[2], y_written, y_copied;
     alignas(16) float b1[128];
     int units[4][kCkRows];
+    unsigned z_groups[8];  // the largest exponent of each group in this CTA's rows
     alignas(8) float inputs[192], outputs[64], hidden[128];  // units of W1's and W2's columns, and what a hidden unit weighs against the largest
     uint32_t tmem_base;
     int abort;
@@ -1054,7 +1208,8 @@ struct CkForwardArgs {
     float *y;
     int8_t *codes;
     uint8_t *exponents;
-    uint2 *mask;  // [rows][2]
+    uint2 *mask;          // [rows][2]
+    uint8_t *z_groups;    // [ctas][8]
     long long rows;
     int in, out, pitch, chunks, tiles;
     unsigned *status;
@@ -1091,6 +1246,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
     const CkHeader &head = *reinterpret_cast<const CkHeader *>(a.image);
     const bool inputs_apart = head.inputs_apart, outputs_apart = head.outputs_apart, hidden_apart = head.hidden_apart;
     if (threadIdx.x < 128) sh.b1[threadIdx.x] = __ldg(a.b1 + threadIdx.x) * power_of_two(-head.hidden1[threadIdx.x]);
+    if (threadIdx.x < 8) sh.z_groups[threadIdx.x] = 0;
     if (warp == kFwProducers) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -1105,7 +1261,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
         __syncthreads();
         if (hidden_apart) {  // W2 with what its hidden unit weighs in y
             umma_wait(&sh.image, 0, &sh.abort);
-            ck_rescale(w2, w2 + kCkTile, 1, sh.hidden, nullptr);
+            ck_rescale(w2, w2 + kCkTile, 1, sh.hidden, nullptr, blockDim.x);
             fence_proxy_async();
             __syncthreads();
         }
@@ -1120,7 +1276,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
         // place of (row r, columns 2 lane, 2 lane + 1) in a slot: units of eight columns change places by the row's lowest three bits
         const int word = (lane & 3) * 4;
         int s = 0;
-        unsigned ph = 1;
+        unsigned ph = 1, groups_most = 0;  // a byte for each chunk: group 2 c + lane / 16
 #pragma unroll 1
         for (int t = 0; t < ntile && ok; ++t) {
             const long long row0 = row_of(t) + first;
@@ -1156,6 +1312,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                 const float to_units = rows8_to_units(e);
                 const int r8 = (lane & 15) >> 1, g = 2 * c + (lane >> 4);
                 if ((lane & 1) == 0 && g < groups) high[768 + r8 * groups + g] = (uint8_t)e;
+                groups_most = __vmaxu4(groups_most, (finite && e > 7u ? e : 0u) << (8 * c));  // (7: nothing but zeros, or next to it)
                 unsigned f = finite ? most : 0u;
                 if (__any_sync(kFull, !finite)) {  // what is finite of such groups, for the unit of the row
 #pragma unroll
@@ -1240,6 +1397,8 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                 }
             }
         }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) atomicMax(&sh.z_groups[2 * c + (lane >> 4)], groups_most >> (8 * c) & 0xffu);
         if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_PRODUCER);
     } else {
         const int quarter = warp & 3, row = quarter * 32 + lane;
@@ -1386,6 +1545,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
 
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x < 8) a.z_groups[blockIdx.x * 8 + threadIdx.x] = (uint8_t)sh.z_groups[threadIdx.x];
     if (warp == kFwProducers) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
@@ -1393,7 +1553,9 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-static int64_t ck_image_bytes(int in_dim) { return kCkHeader + (int64_t)(2 * ((in_dim + 63) / 64) + 2) * kCkTile; }
+// header | matrices | what the forward saw of its CTAs' rows: the largest exponent of each group of z
+static int64_t ck_matrices_end(int in_dim) { return kCkHeader + (int64_t)(2 * ((in_dim + 63) / 64) + 2) * kCkTile; }
+static int64_t ck_image_bytes(int in_dim) { return ck_matrices_end(in_dim) + 148 * 8; }
 static GradReduce ck_reduce(int64_t rows, int in_dim, int out_dim) {
     GradReduce r = {};
     const int64_t tiles = (rows + kCkRows - 1) / kCkRows;
@@ -1402,6 +1564,7 @@ static GradReduce ck_reduce(int64_t rows, int in_dim, int out_dim) {
     return r;
 }
 static int64_t ck_partial_floats(const GradReduce &r) { return (int64_t)r.ctas * kCkRows * (r.N1p + r.N2p); }
+static int64_t ck_column_words(const GradReduce &r) { return (int64_t)r.ctas * kCkProducers * 64; }
 
 template <typename Kernel>
 static int ck_launch(Kernel kernel, const char *name, const CkArgs &a, int smem, int ctas, cudaStream_t st) {
@@ -1442,7 +1605,7 @@ int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1,
     if (image_bytes < need) return fail(NPA_ERR_SCRATCH_TOO_SMALL, "%s: image has %lld bytes, %lld needed", me, (long long)image_bytes, (long long)need);
     CkForwardArgs a = {};
     a.z = z; a.b1 = b1; a.image = static_cast<const uint8_t *>(image); a.y = y; a.codes = static_cast<int8_t *>(codes); a.exponents = exponents;
-    a.mask = reinterpret_cast<uint2 *>(mask); a.rows = rows; a.in = in_dim; a.out = out_dim; a.pitch = (int)rows8_pitch(in_dim);
+    a.mask = reinterpret_cast<uint2 *>(mask); a.z_groups = static_cast<uint8_t *>(image) + ck_matrices_end(in_dim); a.rows = rows; a.in = in_dim; a.out = out_dim; a.pitch = (int)rows8_pitch(in_dim);
     a.chunks = (in_dim + 63) / 64; a.tiles = (int)((rows + kCkRows - 1) / kCkRows);
     if (!(a.status = umma_status_word())) return fail(NPA_ERR_CUDA, "%s: no status word", me);
     const cudaStream_t st = (cudaStream_t)stream;
@@ -1459,7 +1622,8 @@ int npa_mlp_checkpoint_forward(const float *z, const float *W1, const float *b1,
 
 int64_t npa_mlp_checkpoint_backward_scratch_bytes(int64_t rows, int32_t in_dim, int32_t out_dim) {
     if (rows <= 0 || in_dim <= 0 || out_dim <= 0) return 0;
-    return 4 * ck_partial_floats(ck_reduce(rows, in_dim, out_dim));
+    const GradReduce r = ck_reduce(rows, in_dim, out_dim);
+    return 4 * (ck_partial_floats(r) + ck_column_words(r));
 }
 
 int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, const uint32_t *mask, const void *image, int64_t image_bytes, const float *b1,
@@ -1483,6 +1647,8 @@ int npa_mlp_checkpoint_backward(const void *codes, const uint8_t *exponents, con
     CkArgs a = {};
     a.codes = static_cast<const int8_t *>(codes); a.exponents = exponents; a.mask = reinterpret_cast<const uint4 *>(mask); a.dy = dy; a.b1 = b1;
     a.image = static_cast<const uint8_t *>(image); a.dz = dz; a.partial = static_cast<float *>(scratch);
+    a.dy_columns = reinterpret_cast<unsigned *>(a.partial + ck_partial_floats(r)); a.looked = dz != nullptr;
+    a.z_groups = a.image + ck_matrices_end(in_dim);
     a.rows = rows; a.in = in_dim; a.out = out_dim; a.pitch = (int)rows8_pitch(in_dim); a.chunks = (in_dim + 63) / 64; a.N1p = r.N1p; a.N2p = r.N2p;
     a.tiles = (int)((rows + kCkRows - 1) / kCkRows);
     if (!(a.status = umma_status_word())) return fail(NPA_ERR_CUDA, "%s: no status word", me);
