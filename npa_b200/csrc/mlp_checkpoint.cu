@@ -16,7 +16,7 @@
 //     tiles; one of an index that stays comes back in the epilogue.  Weights that lie together take neither way;
 //   * z in the forward, and dy for dz, in units of their row: rows of any size keep their accuracy, and the unit comes back in the epilogue;
 //   * dy and zh for the sums over rows in the unit of the largest of their tile of 128 rows, which comes in when the tile's sum leaves the
-//     accumulator, and, where they lie apart, of their column and group of columns (ck_look);
+//     accumulator, and, where they lie apart, of their column and group of columns (ck_settle);
 //   * h in a unit that its products and the largest bias cannot exceed, dh times a power of two that brings its largest sum back in range.
 //
 // The largest of a unit is an operand of 2^14 to 2^15 (accumulators have 32 bits, only operands are short), which leaves 22 bits to what is
@@ -32,10 +32,10 @@
 // z W1^T, A of zh W1^T and B of dh W1, and one tile of zh is B of both of its products, as is dy's.
 //
 // Memory is the floor (B200, 262,144 rows of 163 and 35: 512 MB, 78 us) and not what bounds them: it is the way of a tile through
-// conversion, product, mask, product, one after another in what tensor and shared memory are left.  Measured there, us: forward 142
-// (the 32-bit forward that leaves its hidden layer: 143), dz 78, weights 137, their sum over CTAs 8; the parts of a tile's way stand at the
-// kernels.  At 32,768 rows of 66 and 18: 19, 12, 21 and 7, and the host takes 90 us a pass, 57 of them
-// torch's engine for the backward.
+// conversion, product, mask, product, one after another in what tensor and shared memory are left.  Measured there, us, each from a cold L2:
+// image 6, forward 143 (the 32-bit forward that leaves its hidden layer: 143), dz 89, weights 148, their sum over CTAs 5; the parts of a
+// tile's way stand at the kernels.  At 32,768 rows of 66 and 18: 6, 18, 15, 21 and 5, and the host takes 90 us a pass, 57 of them torch's engine for
+// the backward.
 //
 // Waits are bounded as in umma.cuh; they report through npa_linear_tcgen05_status (bits 1024, 2048, 4096: MMA lane, producers, epilogue).
 #include <mutex>
@@ -98,10 +98,11 @@ __device__ __forceinline__ float times_power(float v, int e) {
 // or more below the matrix's has a unit of its own, so that it is held as accurately as the largest.  Channels have 0 where that is not so.
 // A hidden unit's row of W1 counts together with its bias, which is then no larger than the matrix either.
 constexpr int kApart = 6, kFarthest = 100;
+enum { CK_INPUTS = 1, CK_HIDDEN = 2, CK_OUTPUTS = 4 };
 struct CkHeader {
     int w1, w2, b1;      // exponents of the matrices' units, and of the largest positive bias over its row's unit (-1000: there is none)
     int hidden;          // the largest hidden1[j] + hidden2[j]
-    int inputs_apart, hidden_apart, outputs_apart, unused;  // whether they differ (`hidden_apart`: in their sum)
+    int apart;           // which of them differ (CK_HIDDEN: in the sum of both)
     int8_t hidden1[128], hidden2[128], inputs[192], outputs[64];
 };
 static_assert(sizeof(CkHeader) <= kCkHeader, "in front of the matrices");
@@ -152,23 +153,24 @@ __global__ void __launch_bounds__(kImageThreads) mlp_checkpoint_image_kernel(con
     const float bias = t < 128 ? __ldg(a.b1 + t) : 0.f;
     __syncthreads();
     // the largest of rows and columns, the columns as they are: that is what they are in units of their rows unless those lie apart
-    unsigned m1[kRows1], m2[16], column[kColumns1] = {}, column2 = 0;
+    // (first of everything; where that is not finite, of what is)
+    auto look = [&](auto size) {
+        unsigned m1[kRows1], m2[16], column[kColumns1] = {}, column2 = 0;
 #pragma unroll
-    for (int r = 0; r < kRows1; ++r) {
-        m1[r] = 0;
+        for (int r = 0; r < kRows1; ++r) {
+            m1[r] = 0;
 #pragma unroll
-        for (int i = 0; i < kColumns1; ++i) {
-            const unsigned m = finite_magnitude(v1[r][i]);
-            m1[r] = max(m1[r], m);
-            column[i] = max(column[i], m);
+            for (int i = 0; i < kColumns1; ++i) {
+                const unsigned m = size(v1[r][i]);
+                m1[r] = max(m1[r], m);
+                column[i] = max(column[i], m);
+            }
         }
-    }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        m2[i] = i < kRows2 ? finite_magnitude(v2[i]) : 0u;
-        column2 = max(column2, m2[i]);
-    }
-    {
+        for (int i = 0; i < 16; ++i) {
+            m2[i] = i < kRows2 ? size(v2[i]) : 0u;
+            column2 = max(column2, m2[i]);
+        }
         const unsigned one = gather_max8(m1), two = gather_max8(*reinterpret_cast<unsigned(*)[8]>(m2)), three = gather_max8(*reinterpret_cast<unsigned(*)[8]>(m2 + 8));
         if (lane % 4 == 0) {
             rows1[warp + 16 * (lane / 4)] = one;
@@ -180,11 +182,21 @@ __global__ void __launch_bounds__(kImageThreads) mlp_checkpoint_image_kernel(con
             atomicMax(&most[0], all1);
             atomicMax(&most[1], all2);
         }
-    }
 #pragma unroll
-    for (int i = 0; i < kColumns1; ++i) atomicMax(&columns1[lane + 32 * i], column[i]);
-    atomicMax(&columns2[unit2], column2);
-    __syncthreads();
+        for (int i = 0; i < kColumns1; ++i) atomicMax(&columns1[lane + 32 * i], column[i]);
+        atomicMax(&columns2[unit2], column2);
+        __syncthreads();
+    };
+    look([](float v) { return magnitude(v); });
+    if (max(most[0], most[1]) >= 0x7f800000u) {
+        __syncthreads();
+        if (t < 2) most[t] = 0;
+        if (t < 192) columns1[t] = 0;
+        if (t < 64) rows2[t] = 0;
+        if (t < 128) columns2[t] = 0;
+        __syncthreads();
+        look([](float v) { return finite_magnitude(v); });
+    }
     const int e1 = min(binade(most[0]), 126), e2 = min(binade(most[1]), 126);
     int apart1 = 0, apart2 = 0;
     if (t < 128) {
@@ -243,7 +255,7 @@ __global__ void __launch_bounds__(kImageThreads) mlp_checkpoint_image_kernel(con
     if (t < 64) h->outputs[t] = (int8_t)outputs[t];
     if (t == 0) {
         h->w1 = e1; h->w2 = e2; h->b1 = most[2] == 0 ? -1000 : binade(most[2]);
-        h->hidden = hidden[0]; h->hidden_apart = hidden[0] != -hidden[1]; h->inputs_apart = inputs_apart; h->outputs_apart = outputs_apart;
+        h->hidden = hidden[0]; h->apart = (inputs_apart ? CK_INPUTS : 0) | (hidden[0] != -hidden[1] ? CK_HIDDEN : 0) | (outputs_apart ? CK_OUTPUTS : 0);
     }
 }
 
@@ -398,7 +410,7 @@ __device__ __forceinline__ void ck_copy_image(uint8_t *dst, const uint8_t *image
 // Channels of the image in other units, once in front of the tiles (a copy has landed, the MMAs have not begun): the rows are multiplied by
 // row[] and the columns by column[], powers of two (NULL: 1).  Only where channels lie apart: a microsecond or two for the 128 KB of 163 inputs.
 __device__ __noinline__ void ck_rescale(uint8_t *heads, uint8_t *tails, int chunks, const float *row, const float *column, int threads) {
-    for (int q = threadIdx.x; q < chunks * 128 * 8; q += threads) {
+    for (int q = threadIdx.x % threads; q < chunks * 128 * 8; q += threads) {
         const int r = (q >> 3) & 127, k = (q >> 10) * 64 + (((q & 7) ^ (r & 7)) << 3);
         const float f = row ? row[r] : 1.f;
         uint4 head = reinterpret_cast<uint4 *>(heads)[q], tail = reinterpret_cast<uint4 *>(tails)[q];
@@ -412,6 +424,9 @@ __device__ __noinline__ void ck_rescale(uint8_t *heads, uint8_t *tails, int chun
         reinterpret_cast<uint4 *>(tails)[q] = make_uint4(l[0], l[1], l[2], l[3]);
     }
 }
+// The eight warps of the epilogue of dz's and the weights' kernel, which see to the units; never inside a loop that a bounded wait may leave.
+constexpr int kCkEpilogue = 256;
+__device__ __forceinline__ void ck_epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kCkEpilogue) : "memory"); }
 __device__ __forceinline__ float channel_factor(int e) { return power_of_two(max(e, -126)); }
 
 // ---- dz ----------------------------------------------------------------------------------------------------------------
@@ -420,7 +435,7 @@ __device__ __forceinline__ float channel_factor(int e) { return power_of_two(max
 // 16 columns of the accumulator they came from) and store dz of the tile before.  dh has two accumulators, so that the next tile's is made
 // meanwhile.
 struct CkDzShared {
-    uint64_t image, op_full, op_empty, dh_full[2], dh_ready[2], dz_full, dz_empty, staged[4], copied[4];
+    uint64_t image, units_known, op_full, op_empty, dh_full[2], dh_ready[2], dz_full, dz_empty, staged[4], copied[4];
     int units[kCkRowRing][kCkRows];
     alignas(8) float outputs[64], inputs[192];  // units of W2's and W1's columns
     float hidden[128];                          // what a hidden unit weighs against the largest
@@ -464,12 +479,12 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
         }
         mbar_init(&sh.dz_full, 2);  // the products, and the MMA lane itself: what it has seen of the producers' writes the epilogue sees
         mbar_init(&sh.dz_empty, 8);
+        mbar_init(&sh.units_known, 8);
         sh.abort = 0;
         mbar_fence_init();
-        ck_copy_image(base, a.image, a.chunks, &sh.image);
     }
     const CkHeader &units = *reinterpret_cast<const CkHeader *>(a.image);
-    const bool inputs_apart = units.inputs_apart, outputs_apart = units.outputs_apart, hidden_apart = units.hidden_apart;
+    const int apart = units.apart;  // (looked at behind the barrier)
     if (warp == kCkProducer0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -477,18 +492,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (inputs_apart || outputs_apart || hidden_apart) {
-        if (threadIdx.x < 64) sh.outputs[threadIdx.x] = channel_factor(units.outputs[threadIdx.x]);
-        if (threadIdx.x < 192) sh.inputs[threadIdx.x] = channel_factor(units.inputs[threadIdx.x]);
-        if (threadIdx.x < 128) sh.hidden[threadIdx.x] = channel_factor(units.hidden1[threadIdx.x] + units.hidden2[threadIdx.x] - units.hidden);
-        __syncthreads();
-        if (hidden_apart) {  // dh with what its hidden unit weighs in dz
-            umma_wait(&sh.image, 0, &sh.abort);
-            ck_rescale(w2, w2 + kCkTile, 1, sh.hidden, nullptr, blockDim.x);
-            fence_proxy_async();
-            __syncthreads();
-        }
-    }
     const unsigned tmem = sh.tmem_base;
     const int ntile = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     auto row_of = [&](int it) { return ((long long)blockIdx.x + (long long)it * gridDim.x) * kCkRows; };
@@ -499,6 +502,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
         // tile before
         const bool issues = warp == kCkProducer0;
         const int mine = (warp - kCkProducer0) * 32;
+        if (issues && lane == 0) ck_copy_image(base, a.image, a.chunks, &sh.image);
         const unsigned id1 = f16_idesc(128, false), id2 = f16_idesc((a.in + 15) / 16 * 16, true);
         const int ks1 = (a.out + 15) / 16;
         const uint64_t w2h = umma_desc(smem_u32(w2)), w2l = umma_desc(smem_u32(w2 + kCkTile));
@@ -538,10 +542,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
         DyRows<TWO> rows;
         uint2 most = make_uint2(0, 0);
         if (ntile > 0) rows.load(a, row_of(0) + mine, lane);
+        if (apart) ok = umma_wait(&sh.units_known, 0, &sh.abort);
 #pragma unroll 1
         for (int t = 0; t < ntile && ok; ++t) {
             if (!(ok = umma_wait(&sh.op_empty, (t & 1) ^ 1, &sh.abort))) break;
-            if (outputs_apart) rows.times(sh.outputs, lane);
+            if (apart & CK_OUTPUTS) rows.times(sh.outputs, lane);
             rows.store_by_row(ops, ops + kCkTile, sh.units[t % kCkRowRing], mine, lane, most);
             fence_proxy_async();
             __syncwarp();
@@ -559,7 +564,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
                 ok = __shfl_sync(kFull, (int)ok, 0) != 0;
             }
         }
-        rows.put_columns(a.dy_columns + (blockIdx.x * kCkProducers + warp - kCkProducer0) * 64, most, outputs_apart ? sh.outputs : nullptr, lane);
+        rows.put_columns(a.dy_columns + (blockIdx.x * kCkProducers + warp - kCkProducer0) * 64, most, apart & CK_OUTPUTS ? sh.outputs : nullptr, lane);
         if (!ok && lane == 0) {
             atomicOr(a.status, issues ? CK_STATUS_MMA : CK_STATUS_PRODUCER);
             __nanosleep(20000);  // copies in flight land before the CTA leaves
@@ -568,6 +573,19 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
     } else {
         const int quarter = warp & 3, half = warp >> 2;  // rows 32 quarter + lane; hidden units 64 half and up, every second 16 columns of dz
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
+        if (apart) {
+            if (threadIdx.x < 64) sh.outputs[threadIdx.x] = channel_factor(units.outputs[threadIdx.x]);
+            if (threadIdx.x < 192) sh.inputs[threadIdx.x] = channel_factor(units.inputs[threadIdx.x]);
+            if (threadIdx.x < 128) sh.hidden[threadIdx.x] = channel_factor(units.hidden1[threadIdx.x] + units.hidden2[threadIdx.x] - units.hidden);
+            ck_epilogue_barrier();
+            if (apart & CK_HIDDEN) {  // dh with what its hidden unit weighs in dz
+                umma_wait(&sh.image, 0, &sh.abort);
+                ck_rescale(w2, w2 + kCkTile, 1, sh.hidden, nullptr, kCkEpilogue);
+                fence_proxy_async();
+                __syncwarp();
+            }
+            if (lane == 0) mbar_arrive(&sh.units_known);
+        }
         const int unit_of_w = units.w1 + units.w2 + units.hidden + kDhDown - 3 * kOperand;
         const int buffers = ck_dz_buffers(a.in);  // (with two of them quarters 0 and 2, 1 and 3 take turns)
         float *stg = staged + quarter % buffers * 32 * a.in;
@@ -584,7 +602,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             // the row's unit times those of the weights: one power of two unless it is out of range
             const int e = sh.units[t % kCkRowRing][quarter * 32 + lane] + unit_of_w, e1 = max(min(e, 127), -126);
             const float unit = power_of_two(e1), rest = power_of_two(max(e - e1, -126));
-            const bool far = __any_sync(kFull, e != e1) || inputs_apart;
+            const bool far = __any_sync(kFull, e != e1) || (apart & CK_INPUTS);
             float *row = stg + lane * a.in;
             auto emptied = [&]() {
                 tc_fence_before();
@@ -602,7 +620,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             auto put = [&](unsigned(&r)[16], int c0, auto full) {
                 if (far) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * rest * (inputs_apart ? sh.inputs[c0 + j] : 1.f));
+                    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * rest * (apart & CK_INPUTS ? sh.inputs[c0 + j] : 1.f));
                 }
                 if constexpr (PIECES) {
                     float v[16];
@@ -703,14 +721,16 @@ struct CkWeightsShared {
     float both[kCkRows];
     int z_unit;
     // of this CTA's rows: the largest finite dy of each column, the largest exponent of each group of z, the magnitudes of each column's codes
-    // (a byte each, whose first bit is that of the largest); and what follows from them (ck_own_units)
+    // (a byte each, whose first bit is that of the largest); and what follows from them (ck_settle)
     unsigned dy_columns[64], z_groups[8], used[44];
     alignas(8) float inputs[192], outputs[64];  // factors of the image's columns
     alignas(8) float dy_units[64], dy_back[64];
     float z_back[8];
     unsigned z_shift[kCkRows * 6 / 4];  // what a tile's exponents are moved by, four a word
     uint8_t z_move[8];
-    int add1, add2, most1, apart, least_field;
+    float2 back[2][128];
+    int add1, add2, most1;  // exponents of the units of W1 and W2 (of dh as it leaves its accumulator), and of the largest of zh W1^T's products
+    int apart, least_field, settle;
     uint32_t tmem_base;
     int abort;
 };
@@ -741,27 +761,39 @@ __device__ __forceinline__ void decode_codes(const uint4 &q, __half2 scale, uint
 // the image's column by the inverse (dh and zh W1^T sum over them), and the power comes back when the CTA's sums leave.  Columns of W1 come out
 // of their own units on the same way, in the unit of the largest that meets a code (a column whose codes are all zero has no size).
 // The epilogue's warps see to this in front of the tiles, while the producers have the first one's loads on their way.  The sizes are those
-// that the forward (groups of z) and dz's kernel (columns of dy) saw in the same rows; where dz was not asked for dy is read once more (141 ->
-// 150 us for 262,144 rows of 163 and 35), and so are the codes where columns of W1 lie apart.
+// that the forward (groups of z) and dz's kernel (columns of dy) saw in the same rows; where dz was not asked for dy is read once more (148 ->
+// 164 us for 262,144 rows of 163 and 35), and so are the codes where columns of W1 lie apart.  Where nothing does it is a few instructions
+// (ck_apart): all that runs once a CTA comes from memory, and the whole of it, always run, cost 3 us.
 constexpr int kGroupsApart = 16, kGroupsFarthest = 120;  // zh is exact 2^32 below the largest of its tile: 2^16 are left to the rows
-constexpr int kCkLook = 256;
 enum { CK_APART_W1 = 1, CK_APART_W2 = 2, CK_APART_Z = 4 };
-template <typename Row>
-__device__ __forceinline__ void ck_look(CkWeightsShared &sh, const CkArgs &a, int ntile, Row row_of, bool codes, unsigned seen_dy, unsigned seen_z) {
-    const int t = threadIdx.x, out = a.out;  // (t < kCkLook)
-    const bool last = ntile > 0 && row_of(ntile - 1) + kCkRows >= a.rows;  // this CTA's rows end with the last one
-    if (t < 8) sh.z_groups[t] = seen_z;
-    if (seen_dy) atomicMax(&sh.dy_columns[t % 64], seen_dy);
-    // a thread goes on by a multiple of the columns, so that it stays in the same ones
-    if (!a.looked) {
-        const int turn = kCkLook / out * out, each = 32 * out, total = ntile * each;
+// Whether anything lies apart; a warp's lanes hold the columns `lane` and `lane` + 32 of dy, and eight of them the groups of z.
+__device__ __forceinline__ bool ck_apart(const CkArgs &a, int header, unsigned column, unsigned further, unsigned group) {
+    auto field = [](unsigned m) { return (int)max(m >> 23, 1u); };
+    const unsigned all = __reduce_max_sync(kFull, max(column, further)), least = __reduce_min_sync(kFull, min(column ? column : ~0u, further ? further : ~0u));
+    const unsigned most = __reduce_max_sync(kFull, group), small = __reduce_min_sync(kFull, group ? group : ~0u);
+    return (header & (CK_INPUTS | CK_OUTPUTS)) || !a.looked || (all && field(all) - field(least) >= kApart) || (most && most - small >= kGroupsApart);
+}
+// The units of a CTA where something does, by the epilogue's threads.  (Out of line: instructions that run once come from memory.)
+__device__ __forceinline__ void ck_settle(CkWeightsShared &sh, const CkArgs &a, uint8_t *base, int ntile) {
+    const CkHeader &head = *reinterpret_cast<const CkHeader *>(a.image);
+    const int t = threadIdx.x, lane = t & 31, out = a.out, units = a.pitch / 16, header = head.apart;
+    const long long row0 = (long long)blockIdx.x * kCkRows, rows_on = (long long)gridDim.x * kCkRows;  // of this CTA's first tile, to the next
+    if (t < 64) sh.dy_columns[t] = 0;
+    if (t < 44) sh.used[t] = 0;
+    if (t < 8) sh.z_groups[t] = __ldg(a.z_groups + blockIdx.x * 8 + t);
+    if (t == 0) sh.add1 = sh.add2 = sh.most1 = -1000;  // (what comes to the matrices' exponents, which are added last)
+    ck_epilogue_barrier();
+    if (a.looked) {
+        atomicMax(&sh.dy_columns[t % 64], __ldg(a.dy_columns + blockIdx.x * kCkProducers * 64 + t));
+    } else {  // a thread goes on by a multiple of the columns, so that it stays in the same ones
+        const int turn = kCkEpilogue / out * out, each = 32 * out, total = ntile * each;
         const long long end = a.rows * out;
         unsigned m[4] = {};
         if (t < turn) {
 #pragma unroll 8
             for (int i = t; i < total; i += turn) {
                 const int tile = i / each;
-                const long long at = row_of(tile) * out + 4 * (i - tile * each);
+                const long long at = (row0 + tile * rows_on) * out + 4 * (i - tile * each);
                 const float4 v = at + 4 <= end ? __ldg(reinterpret_cast<const float4 *>(a.dy + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 m[0] = max(m[0], finite_magnitude(v.x));
                 m[1] = max(m[1], finite_magnitude(v.y));
@@ -771,16 +803,17 @@ __device__ __forceinline__ void ck_look(CkWeightsShared &sh, const CkArgs &a, in
 #pragma unroll
             for (int q = 0; q < 4; ++q) atomicMax(&sh.dy_columns[(4 * t + q) % out], m[q]);
         }
+        const bool last = ntile > 0 && row0 + (ntile - 1) * rows_on + kCkRows >= a.rows;  // this CTA's rows end with the last one
         if (last && t < (int)(end & 3)) atomicMax(&sh.dy_columns[((end & ~3ll) + t) % out], finite_magnitude(__ldg(a.dy + (end & ~3ll) + t)));
     }
-    if (codes) {
-        const int units = a.pitch / 16, turn = kCkLook / units * units, each = kCkRows * units, total = ntile * each;
+    if (header & CK_INPUTS) {
+        const int turn = kCkEpilogue / units * units, each = kCkRows * units, total = ntile * each;
         uint4 any = make_uint4(0, 0, 0, 0);
         if (t < turn) {
 #pragma unroll 4
             for (int i = t; i < total; i += turn) {
                 const int tile = i / each;
-                const long long at = row_of(tile) * units + (i - tile * each);
+                const long long at = (row0 + tile * rows_on) * units + (i - tile * each);
                 const uint4 v = at < a.rows * units ? __ldg(reinterpret_cast<const uint4 *>(a.codes) + at) : make_uint4(0, 0, 0, 0);
                 any.x |= __vabs4(v.x); any.y |= __vabs4(v.y); any.z |= __vabs4(v.z); any.w |= __vabs4(v.w);
             }
@@ -791,11 +824,7 @@ __device__ __forceinline__ void ck_look(CkWeightsShared &sh, const CkArgs &a, in
             atomicOr(&sh.used[4 * u + 3], any.w);
         }
     }
-}
-__device__ __forceinline__ void ck_look_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kCkLook) : "memory"); }
-// Behind a barrier of those threads; ends with one.
-__device__ __forceinline__ void ck_own_units(CkWeightsShared &sh, const CkArgs &a, const CkHeader &head, bool inputs_apart, bool outputs_apart) {
-    const int t = threadIdx.x, lane = t & 31;
+    ck_epilogue_barrier();
     int mine = 0;
     bool counts = false;
     if (t < 64) {
@@ -803,8 +832,8 @@ __device__ __forceinline__ void ck_own_units(CkWeightsShared &sh, const CkArgs &
         const int p = channel_unit(sh.dy_columns[t], binade(all));
         sh.dy_units[t] = power_of_two(-p);
         sh.dy_back[t] = power_of_two(p);
-        counts = t < a.out;
-        mine = p + (outputs_apart ? head.outputs[t] : 0);
+        counts = t < out;
+        mine = p + head.outputs[t];
         if (counts) atomicMax(&sh.add2, mine);
         if (p) atomicMax(&sh.least_field, kOperand + 1 - p);  // (no power of two leaves 32 bits)
     } else {
@@ -816,15 +845,16 @@ __device__ __forceinline__ void ck_own_units(CkWeightsShared &sh, const CkArgs &
             sh.z_move[g] = (uint8_t)-q;
             if (q) atomicOr(&sh.apart, CK_APART_Z);
         }
-        const unsigned codes = !inputs_apart ? 127u : k < a.in ? sh.used[k / 4] >> (8 * (k % 4)) & 0xffu : 0u;
+        const unsigned codes = !(header & CK_INPUTS) ? 127u : k < a.in ? sh.used[k / 4] >> (8 * (k % 4)) & 0xffu : 0u;
         counts = k < a.in && codes != 0;
-        mine = q + (inputs_apart ? head.inputs[k] : 0);
+        mine = q + head.inputs[k];
         if (counts) {
             atomicMax(&sh.add1, mine);
             atomicMax(&sh.most1, mine - (__clz(codes) - 25));
         }
     }
-    ck_look_barrier();
+    ck_epilogue_barrier();
+    if (t == 64 && sh.add1 == -1000) sh.add1 = sh.most1 = 0;  // (no column has a code)
     if (t < 64) {
         sh.outputs[t] = counts ? channel_factor(mine - sh.add2) : 0.f;
         if (counts && mine != sh.add2) atomicOr(&sh.apart, CK_APART_W2);
@@ -833,8 +863,21 @@ __device__ __forceinline__ void ck_own_units(CkWeightsShared &sh, const CkArgs &
         if (counts && mine != sh.add1) atomicOr(&sh.apart, CK_APART_W1);
     }
     if (sh.apart & CK_APART_Z)
-        for (int b = t; b < kCkRows * 6; b += kCkLook) reinterpret_cast<uint8_t *>(sh.z_shift)[b] = sh.z_move[b % ((a.in + 31) / 32)];
-    ck_look_barrier();
+        for (int b = t; b < kCkRows * 6; b += kCkEpilogue) reinterpret_cast<uint8_t *>(sh.z_shift)[b] = sh.z_move[b % ((a.in + 31) / 32)];
+    ck_epilogue_barrier();
+    uint8_t *w2 = base + 2 * a.chunks * kCkTile;
+    if (sh.apart & (CK_APART_W1 | CK_APART_W2)) {
+        umma_wait(&sh.image, 0, &sh.abort);
+        if (sh.apart & CK_APART_W1) ck_rescale(base, base + a.chunks * kCkTile, a.chunks, nullptr, sh.inputs, kCkEpilogue);
+        if (sh.apart & CK_APART_W2) ck_rescale(w2, w2 + kCkTile, 1, nullptr, sh.outputs, kCkEpilogue);
+        fence_proxy_async();
+    }
+    if (t == 0) {
+        sh.add1 += head.w1;
+        sh.most1 += head.w1;
+        sh.add2 += head.w2 + kDhDown - 2 * kOperand;
+    }
+    ck_epilogue_barrier();
 }
 
 template <int kBlocks, bool TWO>
@@ -860,17 +903,23 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         mbar_init(&sh.units, 8);
         sh.abort = 0;
         mbar_fence_init();
-        ck_copy_image(base, a.image, a.chunks, &sh.image);
     }
     const CkHeader &head = *reinterpret_cast<const CkHeader *>(a.image);
-    const bool inputs_apart = head.inputs_apart, outputs_apart = head.outputs_apart;
-    static_assert(64 * kCkProducers == kCkLook, "a word a thread");
-    const unsigned seen_dy = a.looked && threadIdx.x < kCkLook ? __ldg(a.dy_columns + blockIdx.x * kCkLook + threadIdx.x) : 0u;
-    const unsigned seen_z = threadIdx.x < 8 ? __ldg(a.z_groups + blockIdx.x * 8 + threadIdx.x) : 0u;
-    if (threadIdx.x < 64) sh.dy_columns[threadIdx.x] = 0;
-    else if (threadIdx.x < 72) sh.z_groups[threadIdx.x - 64] = 0;
-    else if (threadIdx.x < 116) sh.used[threadIdx.x - 72] = 0;
-    else if (threadIdx.x == 116) sh.add1 = sh.add2 = sh.most1 = -1000, sh.apart = 0, sh.least_field = kOperand + 1;
+    unsigned column = 0, further = 0, group = 0;  // (what is loaded here is looked at behind the barrier)
+    int header = 0, w1 = 0, w2_unit = 0;
+    if (warp == 0) {
+        header = head.apart; w1 = head.w1; w2_unit = head.w2 + kDhDown - 2 * kOperand;
+        if (a.looked) {
+            const unsigned *p = a.dy_columns + blockIdx.x * kCkProducers * 64 + lane;
+            column = max(max(__ldg(p), __ldg(p + 64)), max(__ldg(p + 128), __ldg(p + 192)));
+            further = max(max(__ldg(p + 32), __ldg(p + 96)), max(__ldg(p + 160), __ldg(p + 224)));
+        }
+        if (lane < 8) group = __ldg(a.z_groups + blockIdx.x * 8 + lane);
+    }
+    static_assert(kCkProducers == 4, "as read here");
+    if (threadIdx.x < 64) sh.dy_units[threadIdx.x] = sh.dy_back[threadIdx.x] = 1.f;
+    else if (threadIdx.x < 72) sh.z_back[threadIdx.x - 64] = 1.f;
+    else if (threadIdx.x == 72) sh.apart = 0, sh.least_field = kOperand + 1;
     if (warp == kCkProducer0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -886,6 +935,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
     if (warp >= kCkProducer0) {
         // the first of the producers issues the products that make the A operands (one lane)
         const bool issues = warp == kCkProducer0;
+        if (issues && lane == 0) ck_copy_image(base, a.image, a.chunks, &sh.image);
         // (operands are described where they are used: kept over the loop they would cost the producers their registers, and a spilled
         // register comes back from L2)
         const int chunks = a.chunks;
@@ -1030,18 +1080,23 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
     } else {
         const int quarter = warp & 3, half = warp >> 2;  // hidden units 32 quarter + lane, rows 64 half .. + 63 of a tile
         const unsigned tlane = tmem + ((unsigned)(quarter * 32) << 16);
-        ck_look(sh, a, ntile, row_of, inputs_apart, seen_dy, seen_z);
-        ck_look_barrier();
-        ck_own_units(sh, a, head, inputs_apart, outputs_apart);
-        if (sh.apart & (CK_APART_W1 | CK_APART_W2)) {
-            umma_wait(&sh.image, 0, &sh.abort);
-            if (sh.apart & CK_APART_W1) ck_rescale(base, base + a.chunks * kCkTile, a.chunks, nullptr, sh.inputs, kCkLook);
-            if (sh.apart & CK_APART_W2) ck_rescale(w2, w2 + kCkTile, 1, nullptr, sh.outputs, kCkLook);
-            fence_proxy_async();
+        const int unit1 = head.hidden1[quarter * 32 + lane], unit2 = head.hidden2[quarter * 32 + lane];
+        const float bias = __ldg(a.b1 + quarter * 32 + lane);
+        if (warp == 0) {
+            const bool settle = ck_apart(a, header, column, further, group);
+            if (lane == 0) {
+                sh.settle = settle;
+                sh.add1 = sh.most1 = w1;
+                sh.add2 = w2_unit;
+            }
         }
-        __syncwarp();
+        ck_epilogue_barrier();
+        if (sh.settle) ck_settle(sh, a, base, ntile);
         if (lane == 0) mbar_arrive(&sh.units);
-        const int w1 = head.w1, w2_unit = head.w2 + sh.add2 + kDhDown - 2 * kOperand;
+        const int add1 = sh.add1, most1 = sh.most1, add2 = sh.add2;
+        sh.back[half][quarter * 32 + lane] = make_float2(channel_factor(unit2), channel_factor(unit1));  // of a hidden unit's dW1 and dW2
+        const float b1 = bias * power_of_two(-unit1);
+        const int b1_unit = b1 > 0.f && finite_magnitude(b1) ? binade(finite_magnitude(b1)) : -1000;  // (below zero it makes h smaller)
         // a lane of the first warp issues the sums over the rows: it knows first that their operands are there
         auto sums_of_w1 = [&](int t) -> bool {
             if (!umma_wait(&sh.dh_ready, t & 1, &sh.abort)) return false;  // which also says that tile t - 1 has left its accumulators
@@ -1066,9 +1121,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             umma_commit(&sh.g2_full);
             return true;
         };
-        const int unit1 = head.hidden1[quarter * 32 + lane];
-        const float b1 = __ldg(a.b1 + quarter * 32 + lane) * power_of_two(-unit1);
-        const int b1_unit = b1 > 0.f && finite_magnitude(b1) ? binade(finite_magnitude(b1)) : -1000;  // (below zero it makes h smaller)
         const int nb1 = (a.in + 15) / 16, nb = nb1 + (a.out + 15) / 16;
         float sums[kBlocks][16], db = 0.f;
 #pragma unroll
@@ -1117,11 +1169,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             __syncwarp();
             // units: zh 2^zu, W1 2^(w1 - 14); h in units of 2^hu, which the largest sum (176 x 2^15 x 32512 in the accumulator's) and bias leave
             // below 1.2 x 2^15
-            const int unit = sh.dy_unit, zu = sh.z_unit, hu = max(zu + w1 + max(sh.most1, -400) + 24, b1_unit + 2) - 15;
-            const float to_h = power_of_two(max(zu + w1 + max(sh.add1, -400) - kOperand - hu, -126)), bias = b1 * power_of_two(min(max(-hu, -126), 127));
+            const int dyu = sh.dy_unit, zu = sh.z_unit, hu = max(zu + most1 + 24, b1_unit + 2) - 15;
+            const float to_h = power_of_two(max(zu + add1 - kOperand - hu, -126)), shift = b1 * power_of_two(min(max(-hu, -126), 127));
             if (!umma_wait(&sh.pre_full, t & 1, &sh.abort, kUmmaWaitNs, 50)) ok = false;
             tc_fence_after();
-            apart(tlane + kCkPreCol, [&](float v, bool alive, int) { return alive ? __fmaf_rn(v, to_h, bias) : 0.f; });
+            apart(tlane + kCkPreCol, [&](float v, bool alive, int) { return alive ? __fmaf_rn(v, to_h, shift) : 0.f; });
             if (lane == 0) {
                 mbar_arrive(&sh.pre_ready);
                 if (warp == 0) ok = ok && sums_of_w2(t);
@@ -1129,11 +1181,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
             if (!(ok = __shfl_sync(kFull, (int)ok, 0) != 0)) break;
             // what the tile's sums are multiples of: products of powers of two, zero where they fall below the smallest number
             auto scale = [](int e) { return power_of_two(max(min(e, 127), -126)) * power_of_two(max(min(e + 126, 0), -126)); };
-            db += (partial[0] + partial[1] + (partial[2] + partial[3])) * scale(unit + w2_unit);
+            db += (partial[0] + partial[1] + (partial[2] + partial[3])) * scale(dyu + add2);
             if (!(ok = umma_wait(&sh.g1_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;
             tc_fence_after();
             bool both = false;  // dW2's sums are there as well
-            const float f1 = scale(unit + w2_unit + zu), f2 = scale(unit - kOperand + hu);
+            const float f1 = scale(dyu + add2 + zu), f2 = scale(dyu - kOperand + hu);
 #pragma unroll
             for (int i = 0; i < kBlocks; ++i) {
                 const int b = 2 * i + half;
@@ -1155,7 +1207,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
         }
         if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_EPILOGUE);
         // db1 in column `in`: both halves of the rows through shared memory.  (A warp that gave up comes here as well: the barriers want all.)
-        const float f1 = channel_factor(head.hidden2[quarter * 32 + lane]), f2 = channel_factor(unit1);
+        const float f1 = sh.back[half][quarter * 32 + lane].x, f2 = sh.back[half][quarter * 32 + lane].y;
         db *= f1;
         float *prow = a.partial + ((long long)blockIdx.x * 128 + quarter * 32 + lane) * (a.N1p + a.N2p);
         if (half == 1) sh.both[quarter * 32 + lane] = db;
@@ -1170,7 +1222,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
 #pragma unroll
             for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4 *>(to + j) = make_float4(sums[i][j], sums[i][j + 1], sums[i][j + 2], sums[i][j + 3]);
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // (column `in` may lie in a block of the other half)
+        ck_epilogue_barrier();  // (column `in` may lie in a block of the other half)
         if (half == 0) prow[a.in] = db + sh.both[quarter * 32 + lane];
     }
 
@@ -1198,7 +1250,7 @@ struct CkForwardShared {
     alignas(16) float b1[128];
     int units[4][kCkRows];
     unsigned z_groups[8];  // the largest exponent of each group in this CTA's rows
-    alignas(8) float inputs[192], outputs[64], hidden[128];  // units of W1's and W2's columns, and what a hidden unit weighs against the largest
+    float outputs[64], hidden[128];  // units of W2's columns, and what a hidden unit weighs against the largest
     uint32_t tmem_base;
     int abort;
 };
@@ -1241,10 +1293,9 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
         mbar_init(&sh.y_copied, 4);
         sh.abort = 0;
         mbar_fence_init();
-        ck_copy_image(base, a.image, kChunks, &sh.image);
     }
     const CkHeader &head = *reinterpret_cast<const CkHeader *>(a.image);
-    const bool inputs_apart = head.inputs_apart, outputs_apart = head.outputs_apart, hidden_apart = head.hidden_apart;
+    const int apart = head.apart;
     if (threadIdx.x < 128) sh.b1[threadIdx.x] = __ldg(a.b1 + threadIdx.x) * power_of_two(-head.hidden1[threadIdx.x]);
     if (threadIdx.x < 8) sh.z_groups[threadIdx.x] = 0;
     if (warp == kFwProducers) {
@@ -1254,18 +1305,6 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (inputs_apart || outputs_apart || hidden_apart) {
-        if (threadIdx.x < 64) sh.outputs[threadIdx.x] = channel_factor(head.outputs[threadIdx.x]);
-        if (threadIdx.x < 192) sh.inputs[threadIdx.x] = channel_factor(head.inputs[threadIdx.x]);
-        if (threadIdx.x < 128) sh.hidden[threadIdx.x] = channel_factor(head.hidden1[threadIdx.x] + head.hidden2[threadIdx.x] - head.hidden);
-        __syncthreads();
-        if (hidden_apart) {  // W2 with what its hidden unit weighs in y
-            umma_wait(&sh.image, 0, &sh.abort);
-            ck_rescale(w2, w2 + kCkTile, 1, sh.hidden, nullptr, blockDim.x);
-            fence_proxy_async();
-            __syncthreads();
-        }
-    }
     const unsigned tmem = sh.tmem_base;  // h of two tiles at 0 and 128, what goes with tails (then y) at 256 and 384
     const int ntile = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     auto row_of = [&](int it) { return ((long long)blockIdx.x + (long long)it * gridDim.x) * kCkRows; };
@@ -1350,14 +1389,14 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                 }
             }
             __syncwarp();
-            if (inputs_apart) {  // in units of W1's columns, of which the row's largest is another
+            if (apart & CK_INPUTS) {  // in units of W1's columns, of which the row's largest is another
                 unsigned m[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
                     m[r] = 0;
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c) {
-                        const float2 f = reinterpret_cast<const float2 *>(sh.inputs)[32 * c + lane];
+                        const float2 f = make_float2(channel_factor(head.inputs[64 * c + 2 * lane]), channel_factor(head.inputs[64 * c + 2 * lane + 1]));
                         v[r][c].x *= f.x;
                         v[r][c].y *= f.y;
                         m[r] = max(m[r], max(finite_magnitude(v[r][c].x), finite_magnitude(v[r][c].y)));
@@ -1398,10 +1437,23 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
             }
         }
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) atomicMax(&sh.z_groups[2 * c + (lane >> 4)], groups_most >> (8 * c) & 0xffu);
+        for (int d = 1; d < 16; d *= 2) groups_most = __vmaxu4(groups_most, __shfl_xor_sync(kFull, groups_most, d));
+        if ((lane & 15) < kChunks) atomicMax(&sh.z_groups[2 * (lane & 15) + (lane >> 4)], groups_most >> (8 * (lane & 15)) & 0xffu);
         if (!ok && lane == 0) atomicOr(a.status, CK_STATUS_PRODUCER);
     } else {
         const int quarter = warp & 3, row = quarter * 32 + lane;
+        if (quarter == 0 && lane == 0) ck_copy_image(base, a.image, kChunks, &sh.image);
+        if (apart & (CK_OUTPUTS | CK_HIDDEN)) {
+            if (row < 64) sh.outputs[row] = channel_factor(head.outputs[row]);
+            sh.hidden[row] = channel_factor(head.hidden1[row] + head.hidden2[row] - head.hidden);
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (apart & CK_HIDDEN) {  // W2 with what its hidden unit weighs in y
+                umma_wait(&sh.image, 0, &sh.abort);
+                ck_rescale(w2, w2 + kCkTile, 1, sh.hidden, nullptr, 128);
+                fence_proxy_async();
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+        }
         // a lane of the first warp issues the MMAs as well: while the producers fill the slots there is little else for it to do
         const bool issues = quarter == 0;
         auto first_layer = [&](int t) -> bool {
@@ -1470,7 +1522,7 @@ __global__ void __launch_bounds__(kFwThreads, 1) mlp_checkpoint_forward_kernel(c
                 float y[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]) * unit * rest;
-                if (outputs_apart) {
+                if (apart & CK_OUTPUTS) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) y[j] *= sh.outputs[c0 + j];
                 }
