@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kImageThreads) mlp_checkpoint_image_kernel(con
         __syncthreads();
         look([](float v) { return finite_magnitude(v); });
     }
-    const int e1 = min(binade(most[0]), 126), e2 = min(binade(most[1]), 126);
+    const int e1 = binade(most[0]), e2 = binade(most[1]);
     int apart1 = 0, apart2 = 0;
     if (t < 128) {
         apart1 = hidden1[t] = channel_unit(max(rows1[t], min(finite_magnitude(bias), (unsigned)(e1 + 127) << 23)), e1);
@@ -1179,7 +1179,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_weights_kernel(c
                 if (warp == 0) ok = ok && sums_of_w2(t);
             }
             if (!(ok = __shfl_sync(kFull, (int)ok, 0) != 0)) break;
-            // what the tile's sums are multiples of: products of powers of two, zero where they fall below the smallest number
+            // what the tile's sums are multiples of: products of powers of two, zero below the smallest number (sums below 2^-112 may be lost)
             auto scale = [](int e) { return power_of_two(max(min(e, 127), -126)) * power_of_two(max(min(e + 126, 0), -126)); };
             db += (partial[0] + partial[1] + (partial[2] + partial[3])) * scale(dyu + add2);
             if (!(ok = umma_wait(&sh.g1_full, t & 1, &sh.abort, kUmmaWaitNs, 50))) break;

@@ -153,3 +153,14 @@ def test_channels_without_a_value(rows, k, o):
     w2[2] = 0
     b1[5] = 0
     _check(w1, b1, w2, z, up, rows)
+
+
+# exponents of z, W1, W2 and the gradients of y; the outputs stay numbers
+@pytest.mark.parametrize("ez,e1,e2,eu", [(-90, 130, -5, -5), (100, -110, 0, 0), (-20, 0, 130, -100), (0, 0, -100, 110), (-60, -50, 60, 40), (60, 40, -80, -40),
+                                         (-40, 130, -40, 0), (0, 0, 0, -90), (0, 0, 0, 110)])
+def test_operands_of_any_size(ez, e1, e2, eu):
+    """Largest weights next to the largest number, and small ones against large inputs: units cover the range of 32 bits."""
+    w1, b1, w2 = _weights(66, 18, 9)
+    z, up = _rand(600, 66, seed=2), _rand(600, 18, seed=3)
+    times = lambda t, e: (t.double() * 2.0**e).float()  # (2^130 itself is no number of 32 bits)
+    _check(times(w1, e1), times(b1, e1 + ez), times(w2, e2), times(z, ez), times(up, eu), 300)
