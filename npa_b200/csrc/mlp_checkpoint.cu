@@ -618,10 +618,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
                 return t == 0 || umma_wait(&sh.copied[quarter + 2], (t - 1) & 1, &sh.abort);
             };
             auto put = [&](unsigned(&r)[16], int c0, auto full) {
-                if (far) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * rest * (apart & CK_INPUTS ? sh.inputs[c0 + j] : 1.f));
-                }
                 if constexpr (PIECES) {
                     float v[16];
 #pragma unroll
@@ -645,6 +641,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) mlp_checkpoint_dz_kernel(const 
             for (; c0 + 16 <= a.in; c0 += 32) block(c0, std::true_type());
             if (c0 < a.in) block(c0, std::false_type());
             emptied();
+            if (far)  // (this thread's own)
+#pragma unroll 1
+                for (c0 = 16 * half; c0 < a.in; c0 += c0 % 16 == 15 ? 17 : 1) row[c0] *= rest * (apart & CK_INPUTS ? sh.inputs[c0] : 1.f);
             fence_proxy_async();  // the copy reads these
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.staged[quarter]);
