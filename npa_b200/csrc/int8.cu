@@ -369,7 +369,8 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const __g
 }
 
 // ---- codes that the tensor cores cannot take as they lie ----------------------------------------------------------------
-// Rows into a pitch of multiples of 16 bytes, unsigned codes shifted to signed ones (p - 128, which flips the top bit).
+// Rows into a pitch of multiples of 16 bytes, unsigned codes shifted to the signed ones that the tensor cores are given (p - 128, which flips the
+// top bit).
 __global__ void __launch_bounds__(256) repack_codes_kernel(const uint8_t *__restrict__ from, long long from_pitch, long long rows, int cols, unsigned flip,
                                                            uint8_t *__restrict__ to, int to_pitch) {
     after_previous_kernel();

@@ -12,10 +12,13 @@
 //   * eight warps, two for a quarter of the rows, turn sums into h (64 units a thread, kept in registers between the maximum and the
 //     codes) and the second layer's sums into rows of y, which leave as one contiguous block.
 //
-// Measured (B200, us): 80 for 262,144 rows of 163 and 35 (the bytes alone: 32), 9.5 for 2,500 rows of 66 and 18.  The instructions bound it:
-// 20,500 a tile of 128 rows, issue slots 46 % taken, the tensor pipe 4 %.
+// Measured (B200, us): 80 for 262,144 rows of 163 and 35 (the bytes alone: 32), 9.5 for 2,500 rows of 66 and 18.  Nothing is full: 20,500
+// instructions a tile of 128 rows take 46 % of the issue slots, DRAM moves 2 TB/s, the tensor pipe is 4 % busy.  What is left is order: at more than
+// 128 inputs there is room for one buffer of codes, so that the converters wait for each tile's first product, and h, its maximum, the
+// partner's half, the codes and y of the tile before are one chain in the epilogue.
 //
-// The MMA takes signed codes on both sides: h's are shifted by 128, and 128 times the sum of w2's row comes back in the epilogue.
+// The MMA is given signed codes on both sides (i8_idesc; it would take either side unsigned): h's are shifted by 128, and 128 times the sum of
+// w2's row comes back in the epilogue.
 // Waits are bounded as in umma.cuh.
 #include "int8.cuh"
 #include "int8_tma.cuh"

@@ -132,9 +132,11 @@ def apply_mlp(module, z, checkpoint=False):
     """``module(z)``; with the fused weight-gradient backward when ``supported(module)``.
 
     ``checkpoint=True`` keeps for the backward, instead of ``z`` and the hidden layer in 32 bits (``4 (in + 128)`` bytes a
-    row), ``z`` in 8 bits (``rows8``) and the bits of the ReLU (``in + in / 32 + 16`` bytes a row, and for each call 67 to
-    132 KB of weights as the tensor cores read them): values and the gradients of ``z`` and of the bias are those of the plain
-    call to the rounding of 32-bit sums, the gradients of the two weight matrices see ``z`` rounded to 8 bits.
+    row), ``z`` in 8 bits (``rows8``) and the bits of the ReLU (``in + in / 32 + 16`` bytes a row, and for each call 68 to
+    133 KB of weights as the tensor cores read them): values and the gradients of ``z`` and of the bias are those of the plain
+    call to the rounding of 32-bit sums, the gradients of the two weight matrices see ``z`` rounded to 8 bits.  That holds for
+    rows, inputs, hidden units and outputs of any size, up to 2**100 apart, each to its own; within one of them numbers are held to
+    22 bits, and where they lie more than 2**11 below its largest to 2**-33 of that.
     It needs a ``supported`` module on the default engine, and is refused (``ValueError``) otherwise;
     without a gradient to record the call is the plain one."""
     if checkpoint and torch.is_grad_enabled():

@@ -97,8 +97,9 @@ def step_euler(model, x, s, grid, dt=1.0, update_prob=0.5, intermediate=False, n
     """``x, s, stats`` after one step; the particles come back in cell order, as in the reference.
 
     ``checkpoint=True`` keeps the perception rows in 8 bits for the backward, and of the hidden layer the bits of its ReLU
-    (``mlp.apply_mlp``): a long training rollout holds a fraction of the memory, and the gradients of the MLP's two weight
-    matrices see rounded rows.
+    (``mlp.apply_mlp``): the MLP holds an eighth to a sixth of what it would, a rollout of steps three fifths (neighbour lists and
+    the other operators' own make up the rest), and the gradients of the MLP's two weight matrices see rounded rows.  A step takes
+    5 to 30 % longer: it runs as single operators instead of one node, and works the hidden layer out again.
 
     ``wrap=True`` additionally applies ``grid.wrap_positions`` (the reference's trainers call it
     after the rollout, train.py:238); the 3D padding column is kept either way.
