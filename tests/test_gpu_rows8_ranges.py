@@ -164,3 +164,33 @@ def test_operands_of_any_size(ez, e1, e2, eu):
     z, up = _rand(600, 66, seed=2), _rand(600, 18, seed=3)
     times = lambda t, e: (t.double() * 2.0**e).float()  # (2^130 itself is no number of 32 bits)
     _check(times(w1, e1), times(b1, e1 + ez), times(w2, e2), times(z, ez), times(up, eu), 300)
+
+
+def test_what_is_not_finite_among_channels_apart():
+    """A NaN in one far group of z, an infinity in one column of the gradients: the other groups, columns and rows keep their own accuracy."""
+    w1, b1, w2 = _weights(100, 18, 7)
+    far = torch.exp2(torch.linspace(-30, 30, 4)).cuda().repeat_interleave(32)[:100]
+    w1 = w1 / far
+    z = ref.clear_of_the_corner(_rand(600, 100, seed=2) * far, w1, b1)[:300]
+    up = _rand(300, 18, seed=3) * _powers(18, "mixed", 6)
+    rows = torch.arange(300, device="cuda") != 5
+    truth, size = ref.mlp_with_checkpoint(z[rows], w1, b1, w2, up[rows]), _sizes(z[rows], w1, b1, w2, up[rows])
+    module = _module(w1, b1, w2)
+    bad = z.clone()
+    bad[5, 40] = float("nan")  # every hidden unit of the row is NaN, and dead (fmaxf)
+    y, dz, dw1, db1, dw2 = _run(module, bad, up)
+    columns = torch.arange(100, device="cuda") // 32 != 1
+    for name, a, t, m in (("y", y[rows], truth[0], size[0]), ("dz", dz[rows], truth[1], size[1]), ("dW1", dw1[:, columns], truth[2][:, columns], size[2][:, columns]),
+                          ("db1", db1, truth[3], size[3]), ("dW2", dw2, truth[4], size[4])):
+        assert ((a.double() - t).abs() <= BAR * m).all(), name
+    assert torch.isnan(dw1[:, ~columns]).all()
+    wild = up.clone()
+    wild[5, 2] = float("inf")
+    y, dz, dw1, db1, dw2 = _run(module, z, wild)
+    alive = (z.double() @ w1.double().t() + b1.double() > 0)[5]
+    truth, size = ref.mlp_with_checkpoint(z, w1, b1, w2, up), _sizes(z, w1, b1, w2, up)
+    others = torch.arange(18, device="cuda") != 2
+    for name, a, t, m in (("dz", dz[rows], truth[1][rows], size[1][rows]), ("dW1", dw1[~alive], truth[2][~alive], size[2][~alive]), ("db1", db1[~alive], truth[3][~alive], size[3][~alive]),
+                          ("dW2", dw2[others], truth[4][others], size[4][others])):
+        assert ((a.double() - t).abs() <= BAR * m).all(), name
+    assert not torch.isfinite(dw2[2]).all() and not torch.isfinite(db1[alive]).any()
