@@ -33,8 +33,8 @@
 //
 // Memory is the floor (B200, 262,144 rows of 163 and 35: 512 MB, 78 us) and not what bounds them: it is the way of a tile through
 // conversion, product, mask, product, one after another in what tensor and shared memory are left.  Measured there, us, each from a cold L2:
-// image 6, forward 143 (the 32-bit forward that leaves its hidden layer: 143), dz 89, weights 148, their sum over CTAs 5; the parts of a
-// tile's way stand at the kernels.  At 32,768 rows of 66 and 18: 6, 18, 15, 21 and 5, and the host takes 90 us a pass, 57 of them torch's engine for
+// image 6, forward 143 (the 32-bit forward that leaves its hidden layer: 143), dz 88, weights 147, their sum over CTAs 5; the parts of a
+// tile's way stand at the kernels.  At 32,768 rows of 66 and 18: 6, 18, 14, 21 and 5, and the host takes 90 us a pass, 57 of them torch's engine for
 // the backward.
 //
 // Waits are bounded as in umma.cuh; they report through npa_linear_tcgen05_status (bits 1024, 2048, 4096: MMA lane, producers, epilogue).
@@ -772,7 +772,7 @@ __device__ __forceinline__ bool ck_apart(const CkArgs &a, int header, unsigned c
     const unsigned most = __reduce_max_sync(kFull, group), small = __reduce_min_sync(kFull, group ? group : ~0u);
     return (header & (CK_INPUTS | CK_OUTPUTS)) || !a.looked || (all && field(all) - field(least) >= kApart) || (most && most - small >= kGroupsApart);
 }
-// The units of a CTA where something does, by the epilogue's threads.  (Out of line: instructions that run once come from memory.)
+// The units of a CTA where something does, by the epilogue's threads; ends with their barrier.
 __device__ __forceinline__ void ck_settle(CkWeightsShared &sh, const CkArgs &a, uint8_t *base, int ntile) {
     const CkHeader &head = *reinterpret_cast<const CkHeader *>(a.image);
     const int t = threadIdx.x, lane = t & 31, out = a.out, units = a.pitch / 16, header = head.apart;

@@ -6,7 +6,7 @@ from pathlib import Path
 import pytest
 
 CSRC = Path(__file__).resolve().parents[1] / "npa_b200" / "csrc"
-BARRIER = re.compile(r"__syncthreads\s*\(|bar\.sync|barrier\.sync|barrier\.cta")
+BARRIER = re.compile(r"__syncthreads|bar\.sync|barrier\.sync|barrier\.cta|\w+_barrier\s*\(\s*\)")
 WAIT = re.compile(r"umma_wait(_slow)?\s*\(")
 
 
